@@ -521,6 +521,45 @@ int msfwsi_blur_sharpen(const unsigned char* in, unsigned char* out, float* tmp,
 /* inv[r][perm[r][k]] = k: jigsaw_reverse_idx = argsort(jigsaw_idx) (src/utils/data/bcss.py:172) */
 int msfwsi_inverse_perm(const long* perm, long* inv, long rows, int K, void* stream);
 
+/* ---- 4-bit storage for frozen weights (csrc/mx4.hip) -------------------------------------------------------------
+ * Blocks of 32 elements of a row share a scale 2^(E - 127); elements are {0, .5, 1, 1.5, 2, 3, 4, 6} with a sign.  A row of
+ * `cols` elements takes G = ceil(cols / 256) groups (zeros behind the last column):
+ *   codes  [G][rows][128] bytes, element 2i of a group in the low, 2i + 1 in the high four bits of byte i
+ *   scales [G][rows][8]   bytes E; 255 = the block is NaN
+ * both 16-byte aligned.  These serve frozen layers beside the fp32 / 16-bit 1x1 convolutions (nn.Linear of
+ * src/models/backbone.py:12-31); the reference has no 4-bit storage: no parity to pin, the checks are against the formulas.
+ *   msfwsi_mx4_quantize:   x [rows][cols], rows `ld` elements apart, any alignment.  E = max(exponent field of the block's
+ *                          largest magnitude - 2, 0), 255 when it is not finite; to nearest, ties to the even code, saturating
+ *   msfwsi_mx4_dequantize: y [rows][cols] in `dtype`
+ *   msfwsi_mx4_gemm:       y[m][n] = sum_k a[m][k] b[n][k] (+ bias[n], fp32), both operands quantised, fp32 sums, y [M][N]
+ *   msfwsi_mx4_dgrad:      dx[m][k] = sum_n dy[m][n] w[n][k], w [N][cols] quantised; dy rows `ld` elements apart, dx [M][cols];
+ *                          the products are exact whatever dy's type */
+int msfwsi_mx4_quantize(int dtype, const void* x, long ld, long rows, long cols, void* codes, void* scales, void* stream);
+int msfwsi_mx4_dequantize(int dtype, const void* codes, const void* scales, long rows, long cols, void* y, void* stream);
+int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_scales, long M, const void* b_codes, const void* b_scales,
+                    long N, long cols, const float* bias, void* y, void* stream);
+int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, const void* codes, const void* scales, long N, long cols,
+                     int dx_dtype, void* dx, void* stream);
+
+/* ---- distillation from a teacher's largest logits (csrc/distill.hip: the formulas) ------------------------------------
+ * Logits [outer][classes][inner]: inner = 1 with rows `ld` elements apart, or contiguous maps (ld = classes * inner).  values /
+ * indices [outer][k][inner], rest and mask [outer * inner]; k <= 64.  No operator of the reference: no parity to pin.
+ *   msfwsi_top_logits:  the k largest (descending; ties by ascending index; NaN above all numbers), their indices, and
+ *                       rest = log sum over the others of exp(logit * inv_t)
+ *   msfwsi_distill_fwd: row_loss [rows] (0 where a row does not count), stats [rows][4] for the backward, loss[0] = sum or mean
+ *                       over the rows that count, loss[1] = the gradient's factor.  rest / mask may be NULL.
+ *                       outer = 0 writes loss alone
+ *   msfwsi_distill_bwd: dz [outer][classes][inner] contiguous = g * factor[1] * d loss_row / dz; g holds one value, or one per
+ *                       row with g_rows; factor (NULL = 1) is the forward's loss pair */
+int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, int classes, long inner, int k, float inv_t, float* values,
+                      int* indices, float* rest, void* stream);
+int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer, int classes, long inner, int k, const float* values,
+                       const int* indices, const float* rest, const unsigned char* mask, float temperature, int mean,
+                       float* stats, float* row_loss, float* loss, double* partials, void* stream);
+int msfwsi_distill_bwd(int dtype, const void* z, long ld, long outer, int classes, long inner, int k, const float* values,
+                       const int* indices, const float* rest, float temperature, const float* stats, const float* factor,
+                       const float* g, int g_rows, void* dz, void* stream);
+
 /* performance knobs (never change results): key 0 = minimum grid (in 256x128 tiles) from which the conv
  * kernels switch from the 128x128 / 4-wave tile to the 256x128 / 8-wave tile; key 1 = 0 disables the pure-DMA
  * (buffer_load ... lds) conv kernel, key 2 = 0 the linear-addressing weight-gradient path, key 4 = grid size (in

@@ -1667,3 +1667,185 @@ def dice_loss(logits, target, C1: int, classes, weight: float, loss_accum, dlogi
     _lib.check(lib.msfwsi_dice_loss(dt_of(logits), _p(logits), _p(target), M, int(C1), CP, mask, float(eps),
                                     float(smooth), float(weight), _p(sums), _p(loss_accum), _p(coef), _p(grad_scale),
                                     _p(dlogits), _stream()), "dice_loss")
+
+
+# ------------------------------------------------------------------------------------------------
+# frozen-teacher operators (csrc/mx4.hip, csrc/distill.hip).  Each wrapper launches on the current stream of the
+# operands' own device, whichever device is current.
+MX4_GROUP = 256  # elements of a row stored together: 128 code bytes, 8 scale bytes
+
+
+def _one_device(ref, *others):
+    for t in others:
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"operands on {ref.device} and {t.device}")
+
+
+def _rows2d(t, name):
+    """[rows, cols] with unit column stride: the row pitch in elements (rows may be slices of a wider tensor)"""
+    if not t.is_cuda:
+        raise _lib.MsfwsiHipError(f"{name}: expected a GPU tensor (no CPU path exists)")
+    if t.dim() != 2:
+        raise ValueError(f"{name}: expected [rows, cols], got {tuple(t.shape)}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the elements of a row must be adjacent")
+    ld = t.stride(0) if rows > 1 else cols
+    if ld < cols:
+        raise ValueError(f"{name}: rows overlap")
+    return rows, cols, ld
+
+
+def _dense(t, name, dtype, numel):
+    """contiguous, of any alignment (slices of a batch): for operands that are read element by element"""
+    if not t.is_cuda:
+        raise _lib.MsfwsiHipError(f"{name}: expected a GPU tensor (no CPU path exists)")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.numel() != numel:
+        raise ValueError(f"{name}: expected {numel} elements, got {t.numel()}")
+
+
+def _mx4_shape(codes, scales, cols, name):
+    if not codes.is_cuda:
+        raise _lib.MsfwsiHipError(f"{name}: expected GPU tensors (no CPU path exists)")
+    G = (int(cols) + MX4_GROUP - 1) // MX4_GROUP
+    if cols < 1 or codes.dim() != 3 or codes.shape[0] != G or codes.shape[2] != MX4_GROUP // 2:
+        raise ValueError(f"{name}: codes of {cols} columns must be [{G}, rows, 128], got {tuple(codes.shape)}")
+    rows = codes.shape[1]
+    _req(codes, name + ".codes", torch.uint8, G * rows * 128)
+    _req(scales, name + ".scales", torch.uint8, G * rows * 8)
+    _one_device(codes, scales)
+    return rows
+
+
+def mx4_quantize(x, codes, scales):
+    """x [rows, cols] (any row pitch) -> 4-bit codes [G, rows, 128] and scales [G, rows, 8]"""
+    lib = _lib.load()
+    rows, cols, ld = _rows2d(x, "x")
+    if _mx4_shape(codes, scales, cols, "out") != rows:
+        raise ValueError(f"out holds {codes.shape[1]} rows, x {rows}")
+    _one_device(x, codes)
+    with torch.cuda.device(x.device):
+        _lib.check(lib.msfwsi_mx4_quantize(dt_of(x), _p(x), ld, rows, cols, _p(codes), _p(scales), _stream()), "mx4_quantize")
+
+
+def mx4_dequantize(codes, scales, y):
+    """y [rows, cols] contiguous <- the values the codes stand for"""
+    lib = _lib.load()
+    rows, cols = y.shape
+    if _mx4_shape(codes, scales, cols, "x") != rows:
+        raise ValueError(f"y has {rows} rows, x {codes.shape[1]}")
+    _req(y, "y")
+    _one_device(y, codes)
+    with torch.cuda.device(y.device):
+        _lib.check(lib.msfwsi_mx4_dequantize(dt_of(y), _p(codes), _p(scales), rows, cols, _p(y), _stream()), "mx4_dequantize")
+
+
+def mx4_gemm(a_codes, a_scales, b_codes, b_scales, cols: int, y, bias=None):
+    """y [M, N] = a b^T (+ bias fp32 [N]) of two 4-bit operands with `cols` columns"""
+    lib = _lib.load()
+    M = _mx4_shape(a_codes, a_scales, cols, "a")
+    N = _mx4_shape(b_codes, b_scales, cols, "b")
+    if N == 0:
+        raise ValueError("b has no rows")
+    _req(y, "y", numel=M * N)
+    if bias is not None:
+        _dense(bias, "bias", torch.float32, N)
+    _one_device(y, a_codes, b_codes, bias)
+    with torch.cuda.device(y.device):
+        _lib.check(lib.msfwsi_mx4_gemm(dt_of(y), _p(a_codes), _p(a_scales), M, _p(b_codes), _p(b_scales), N, int(cols), _p(bias), _p(y),
+                                       _stream()), "mx4_gemm")
+    return y
+
+
+def mx4_dgrad(dy, codes, scales, dx):
+    """dx [M, cols] contiguous = dy [M, N] (any row pitch) times a 4-bit weight [N, cols]"""
+    lib = _lib.load()
+    M, N, ld = _rows2d(dy, "dy")
+    if _mx4_shape(codes, scales, dx.shape[1], "w") != N or N == 0:
+        raise ValueError(f"dy has {N} columns, w {codes.shape[1]} rows")
+    _req(dx, "dx", numel=M * dx.shape[1])
+    _one_device(dy, codes, dx)
+    with torch.cuda.device(dy.device):
+        _lib.check(lib.msfwsi_mx4_dgrad(dt_of(dy), _p(dy), ld, M, _p(codes), _p(scales), N, dx.shape[1], dt_of(dx), _p(dx), _stream()),
+                   "mx4_dgrad")
+    return dx
+
+
+TOP_LOGITS_MAX_K = 64
+
+
+def _logit_layout(z, name):
+    """[rows, C] (any row pitch) or contiguous [N, C, inner]: (outer, classes, inner, ld)"""
+    if z.dim() == 2:
+        rows, Cn, ld = _rows2d(z, name)
+        return rows, Cn, 1, ld
+    if z.dim() != 3:
+        raise ValueError(f"{name}: expected [rows, classes] or [N, classes, positions], got {tuple(z.shape)}")
+    if not z.is_cuda:
+        raise _lib.MsfwsiHipError(f"{name}: expected a GPU tensor (no CPU path exists)")
+    if not z.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    if z.shape[2] == 0:
+        return 0, z.shape[1], 1, z.shape[1]
+    return z.shape[0], z.shape[1], z.shape[2], z.shape[1] * z.shape[2]
+
+
+def _top_args(values, indices, rest, outer, inner, k):
+    _dense(values, "values", torch.float32, outer * k * inner)
+    _dense(indices, "indices", torch.int32, outer * k * inner)
+    if rest is not None:
+        _dense(rest, "rest", torch.float32, outer * inner)
+
+
+def top_logits(x, k: int, temperature: float, values, indices, rest):
+    """the k largest logits (values, indices [outer, k, inner]) and the log-sum-exp of the others (rest [outer * inner])"""
+    lib = _lib.load()
+    outer, Cn, inner, ld = _logit_layout(x, "x")
+    _top_args(values, indices, rest, outer, inner, k)
+    _one_device(x, values, indices, rest)
+    with torch.cuda.device(x.device):
+        _lib.check(lib.msfwsi_top_logits(dt_of(x), _p(x), ld, outer, Cn, inner, int(k), 1.0 / temperature, _p(values), _p(indices), _p(rest),
+                                         _stream()), "top_logits")
+
+
+def distill_fwd(z, values, indices, rest, mask, k: int, temperature: float, mean: bool):
+    """(row_loss [rows], loss fp32[2] = (sum or mean, gradient factor), stats [rows, 4] for distill_bwd)"""
+    lib = _lib.load()
+    outer, Cn, inner, ld = _logit_layout(z, "z")
+    _top_args(values, indices, rest, outer, inner, k)
+    rows = outer * inner
+    if mask is not None:
+        _dense(mask, "mask", torch.bool, rows)
+    _one_device(z, values, indices, rest, mask)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=z.device)
+    row_loss = torch.empty(rows, dtype=torch.float32, device=z.device)
+    loss = torch.empty(2, dtype=torch.float32, device=z.device)
+    partials = torch.empty(2, 2048, dtype=torch.float64, device=z.device)
+    with torch.cuda.device(z.device):
+        _lib.check(lib.msfwsi_distill_fwd(dt_of(z), _p(z), ld, outer, Cn, inner, int(k), _p(values), _p(indices), _p(rest), _p(mask),
+                                          float(temperature), int(bool(mean)), _p(stats), _p(row_loss), _p(loss), _p(partials), _stream()),
+                   "distill_fwd")
+    return row_loss, loss, stats
+
+
+def distill_bwd(z, values, indices, rest, k: int, temperature: float, stats, factor, g, dz):
+    """dz (contiguous, z's shape) = g (one value, or one per row) * factor[1] * d row_loss / dz"""
+    lib = _lib.load()
+    outer, Cn, inner, ld = _logit_layout(z, "z")
+    _top_args(values, indices, rest, outer, inner, k)
+    rows = outer * inner
+    _req(stats, "stats", torch.float32, rows * 4)
+    _opt(factor, "factor", torch.float32, 2)
+    if g.numel() not in (1, rows):
+        raise ValueError(f"g: expected 1 or {rows} values, got {g.numel()}")
+    _dense(g, "g", torch.float32, g.numel())
+    _req(dz, "dz", z.dtype, z.numel())
+    _one_device(z, values, indices, rest, stats, factor, g, dz)
+    with torch.cuda.device(z.device):
+        _lib.check(lib.msfwsi_distill_bwd(dt_of(z), _p(z), ld, outer, Cn, inner, int(k), _p(values), _p(indices), _p(rest), float(temperature),
+                                          _p(stats), _p(factor), _p(g), int(g.numel() != 1), _p(dz), _stream()), "distill_bwd")
+    return dz

@@ -9,9 +9,10 @@ published algorithm (losses/dice.py + losses/_functional.soft_dice_score) is res
 the loss value and d loss / d logits are computed by the HIP kernels of csrc/unet.hip; there is no CPU path."""
 from __future__ import annotations
 
-from typing import List, Optional
+from typing import List, NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import kernels as kn
@@ -61,3 +62,136 @@ class DiceLoss(torch.nn.Module):
         C1 = y_pred.shape[1]
         classes = list(range(C1)) if self.classes is None else list(self.classes)
         return _DiceFn.apply(y_pred, y_true.long().contiguous(), classes, self.eps, self.smooth)
+
+
+class TopLogits(NamedTuple):
+    """What a teacher's row of logits is kept as: its k largest logits (float32, descending), their class indices (int32; a
+    negative one marks padding) and rest = log sum over all other classes of exp(logit / T) (None: the list is taken as the
+    teacher's whole distribution).  The class dimension of values and indices lies where the logits had it."""
+
+    values: torch.Tensor
+    indices: torch.Tensor
+    rest: Optional[torch.Tensor] = None
+
+
+def _class_last(t: torch.Tensor, dim: int) -> torch.Tensor:
+    return t if dim == t.dim() - 1 else t.movedim(dim, -1)
+
+
+def _logit_view(logits: torch.Tensor, dim: int, what: str):
+    """(logits as [rows, C] or [N, C, positions], dim >= 0): rows where the classes are adjacent in memory (also a
+    channels-last map), maps where the positions are"""
+    if not logits.is_cuda:
+        raise _lib.MsfwsiHipError(f"{what} runs only on a HIP device (no CPU path)")
+    kn.dt_of(logits)
+    nd = logits.dim()
+    if nd == 0 or not -nd <= dim < nd:
+        raise ValueError(f"{what}: no dimension {dim} in {tuple(logits.shape)}")
+    dim = dim % nd
+    if dim not in (nd - 1, 1):
+        raise ValueError(f"{what}: the class dimension must be the last one or dimension 1")
+    if logits.shape[dim] == 0:
+        raise ValueError(f"{what}: no classes in {tuple(logits.shape)}")
+    last = _class_last(logits, dim)
+    if dim == nd - 1 or last.is_contiguous():
+        rows = last.reshape(-1, last.shape[-1])
+        if (rows.shape[1] > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
+            rows = rows.contiguous()
+        return rows, dim
+    return logits.contiguous().flatten(2), dim
+
+
+def _temperature(t: float) -> float:
+    t = float(t)
+    if not (0.0 < t < float("inf")):
+        raise ValueError(f"temperature must be positive and finite, got {t}")
+    return t
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, dim: int = -1) -> TopLogits:
+    """The k largest logits along `dim` (the last dimension, or 1 as in segmentation maps [N, C, H, W]) of a frozen teacher:
+    descending, equal ones by ascending class index, NaN above every number.  k <= 64; not differentiable.  `rest` is taken
+    at `temperature`, the one the loss will run at."""
+    view, dim = _logit_view(logits.detach(), dim, "top_logits")
+    t, k = _temperature(temperature), int(k)
+    if not 1 <= k <= min(kn.TOP_LOGITS_MAX_K, view.shape[1]):
+        raise ValueError(f"top_logits: k = {k} outside 1 ... {min(kn.TOP_LOGITS_MAX_K, view.shape[1])}")
+    outer, inner = view.shape[0], view.shape[2:]
+    values = torch.empty(outer, k, *inner, dtype=torch.float32, device=view.device)
+    indices = torch.empty(outer, k, *inner, dtype=torch.int32, device=view.device)
+    others = [n for i, n in enumerate(logits.shape) if i != dim]
+    rest = torch.empty(others, dtype=torch.float32, device=view.device)
+    kn.top_logits(view, k, t, values, indices, rest)
+    if view.dim() == 3:
+        shape = (outer, k) + tuple(logits.shape[2:])
+        return TopLogits(values.view(shape), indices.view(shape), rest)
+    if dim == logits.dim() - 1:
+        return TopLogits(values.view(*others, k), indices.view(*others, k), rest)
+    return TopLogits(values.view(*others, k).movedim(-1, dim), indices.view(*others, k).movedim(-1, dim), rest)
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, dim, values, indices, rest, mask, k, temperature, reduction):
+        view, _ = _logit_view(logits, dim, "TopLogitDistillLoss")
+        row_loss, loss, stats = kn.distill_fwd(view, values, indices, rest, mask, k, temperature, reduction == "mean")
+        ctx.save_for_backward(view, values, indices, rest, stats, loss)
+        ctx.meta = (logits.shape, dim, k, temperature, reduction)
+        if reduction == "none":
+            return row_loss.view([n for i, n in enumerate(logits.shape) if i != dim])
+        return loss[0].clone()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        view, values, indices, rest, stats, loss = ctx.saved_tensors
+        shape, dim, k, temperature, reduction = ctx.meta
+        dz = torch.empty(view.shape, dtype=view.dtype, device=view.device)
+        kn.distill_bwd(view, values, indices, rest, k, temperature, stats, loss if reduction == "mean" else None,
+                       g.detach().float().reshape(-1).contiguous(), dz)
+        if view.dim() == 2 and dim != len(shape) - 1:
+            dz = dz.view([n for i, n in enumerate(shape) if i != dim] + [shape[dim]]).movedim(-1, dim)
+        else:
+            dz = dz.view(shape)
+        return dz, None, None, None, None, None, None, None, None
+
+
+class TopLogitDistillLoss(torch.nn.Module):
+    """Distillation of a student from the top logits of a frozen teacher: T^2 times the Kullback-Leibler divergence between
+    the two softened distributions, with the classes outside the teacher's list taken as one.
+
+        teacher = top_logits(teacher_logits, k, temperature=T)
+        loss = TopLogitDistillLoss(temperature=T)(student_logits, teacher)
+
+    Without `teacher.rest` the teacher's distribution is its list alone, renormalised.  reduction: "mean" over the rows that
+    count, "sum", or "none" (one value per row).  A row does not count -- no loss, a zero gradient -- where `mask` (bool, the
+    logits' shape without the class dimension) is False or the teacher's list and rest are empty (all indices negative or all
+    values -inf); a mean over no rows is 0.  An index listed twice adds its shares; an index past the classes makes its row's
+    loss and gradient NaN.  dim: the class dimension, the last or 1."""
+
+    def __init__(self, temperature: float = 1.0, reduction: str = "mean", dim: int = -1):
+        super().__init__()
+        if reduction not in ("mean", "sum", "none"):
+            raise ValueError(f"reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+        self.temperature, self.reduction, self.dim = _temperature(temperature), reduction, int(dim)
+
+    def forward(self, logits: torch.Tensor, teacher: TopLogits, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        view, dim = _logit_view(logits.detach(), self.dim, "TopLogitDistillLoss")
+        values, indices, rest = teacher
+        others = torch.Size(n for i, n in enumerate(logits.shape) if i != dim)
+        if values.dim() != logits.dim() or values.shape != indices.shape or _class_last(values, dim).shape[:-1] != others:
+            raise ValueError(f"teacher of shapes {tuple(values.shape)}, {tuple(indices.shape)} for logits {tuple(logits.shape)}")
+        k = values.shape[dim]
+        if not 1 <= k <= kn.TOP_LOGITS_MAX_K:
+            raise ValueError(f"the teacher lists {k} classes; 1 ... {kn.TOP_LOGITS_MAX_K} are supported")
+        for name, t, dt in (("rest", rest, torch.float32), ("mask", mask, torch.bool)):
+            if t is not None and (t.shape != others or t.dtype != dt):
+                raise ValueError(f"{name} must be {dt} of shape {tuple(others)}, got {t.dtype} {tuple(t.shape)}")
+        if any(t is not None and t.requires_grad for t in (values, rest)) and torch.is_grad_enabled():
+            raise ValueError("the teacher is frozen: detach its values")
+        if values.dtype != torch.float32 or indices.dtype != torch.int32:
+            raise TypeError(f"teacher values must be float32 and indices int32, got {values.dtype}, {indices.dtype}")
+        if view.dim() == 2:
+            values, indices = _class_last(values, dim), _class_last(indices, dim)
+        rest, mask = (None if t is None else t.contiguous() for t in (rest, mask))
+        return _DistillFn.apply(logits, dim, values.contiguous(), indices.contiguous(), rest, mask, k, self.temperature, self.reduction)

@@ -1,0 +1,438 @@
+"""Top logits and the distillation loss against float64.
+
+Selection and order are exact.  Tolerances of the loss and its gradient, u = 2^-24 (half a step of fp32), A = the largest
+|logit / T| distance of a row, n = classes:
+  exponentials of arguments up to A are off by (A + 4) u relative (the argument's own rounding, then the function's), sums of n positive
+  terms by at most n / 16 further roundings of a lane plus the tree, logarithms by 4 u absolute: every log q and log p is off by
+  E = (3 A + n / 16 + 64) u absolute and every q, p by E relative.
+  loss <= T^2 (sum p + p_r) E + rounding = T^2 E + u |loss|;   gradient <= |g| T E (q_j + p_j), then rounded once to its type."""
+import math
+
+import pytest
+import torch
+
+from oracle import teacher_oracle as to
+
+FP = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+U = 2.0 ** -24
+
+
+def logits_of(rows, C, dt, seed, spread=3.0):
+    g = torch.Generator().manual_seed(seed)
+    return (spread * torch.randn(rows, C, generator=g)).to(dt)
+
+
+def error_of(z, T):
+    fin = torch.where(torch.isfinite(z.double()), z.double(), torch.zeros_like(z, dtype=torch.float64))
+    return (3 * float((fin.amax(1) - fin.amin(1)).max()) / T + z.shape[1] / 16 + 64) * U
+
+
+def check(z, values, indices, rest, mask, T, loss_rows, grad, dt, counts_scale=1.0):
+    """kernel rows and gradients (of the sum of rows times counts_scale) against the definition"""
+    want, wgrad, counts = to.distill(z.cpu(), values.cpu(), indices.cpu(), None if rest is None else rest.cpu(),
+                                     None if mask is None else mask.cpu(), T)
+    E = error_of(z.cpu(), T)
+    if loss_rows is not None:
+        got = loss_rows.cpu().double()
+        bad = ~torch.isfinite(want)
+        assert torch.equal(got[bad].isnan(), want[bad].isnan()) and torch.equal(got[bad & ~want.isnan()], want[bad & ~want.isnan()])
+        assert bool(((got - want)[~bad].abs() <= T * T * E + 2 * U * want[~bad].abs()).all())
+        assert bool((got[~counts] == 0).all())
+    got = grad.cpu().double()
+    nan = wgrad.isnan()
+    assert torch.equal(got.isnan(), nan)
+    assert bool((got[~counts] == 0).all())
+    # sum of the shares and of q bounds the size of what is subtracted
+    q = torch.softmax(z.cpu().double() / T, 1).nan_to_num(0.0)
+    p = torch.zeros(q.shape[0], q.shape[1] + 1, dtype=torch.float64)
+    idx = indices.cpu().long().clamp(min=-1)
+    logs = torch.where(idx >= 0, values.cpu().double() / T, torch.full(values.shape, -math.inf, dtype=torch.float64))
+    if rest is not None:
+        logs = torch.cat([logs, rest.cpu().double().view(-1, 1)], 1)
+    share = torch.softmax(logs, 1).nan_to_num(0.0)
+    p.scatter_add_(1, torch.where((idx >= 0) & (idx < q.shape[1]), idx, q.shape[1]), share[:, :idx.shape[1]])
+    p = p[:, :-1]
+    spread = share[:, idx.shape[1]:].sum(1, keepdim=True) * torch.softmax(torch.where(p > 0, -math.inf, z.cpu().double() / T), 1).nan_to_num(0.0)
+    size = T * counts_scale * (q + p + spread)
+    tiny = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}[dt]
+    lim = size * E * 2 + torch.finfo(dt).eps / 2 * (wgrad * counts_scale).abs() * (1 + 1e-5) + tiny
+    err = (got - wgrad * counts_scale)[~nan].abs()
+    assert bool((err <= lim[~nan]).all()), float((err / lim[~nan]).max())
+
+
+# ---- CPU -------------------------------------------------------------------------------------------------------------
+def test_oracle_by_hand_and_by_differences():
+    v, i, r = to.top_logits(torch.tensor([[1.0, 3.0, 3.0, math.nan, -math.inf]]), 3, 1.0)
+    assert i.tolist() == [[3, 1, 2]] and v[0, 1:].tolist() == [3.0, 3.0] and abs(float(r) - 1.0) < 1e-15
+    # two classes listed in full: the loss is the divergence itself
+    z, t = torch.tensor([[0.3, -0.2]]), torch.tensor([[2.0, 1.0]])
+    loss, grad, counts = to.distill(z, t, torch.tensor([[0, 1]]), None, None, 1.0)
+    p, q = torch.softmax(t.double(), 1), torch.softmax(z.double(), 1)
+    assert abs(float(loss) - float((p * (p / q).log()).sum())) < 1e-15 and torch.allclose(grad, q - p) and bool(counts.all())
+    z = logits_of(4, 9, torch.float32, 1).double()
+    values, indices, rest = to.top_logits(logits_of(4, 9, torch.float32, 2), 3, 2.0)
+    indices[1, 2], indices[2] = indices[1, 0], -1
+    _, grad, _ = to.distill(z, values, indices, rest, None, 2.0)
+    for c in range(9):
+        h = torch.zeros_like(z)
+        h[:, c] = 1e-5
+        up, dn = (to.distill(z + s * h, values, indices, rest, None, 2.0)[0] for s in (1, -1))
+        assert torch.allclose((up - dn) / 2e-5, grad[:, c], atol=1e-8)
+
+
+def test_refusals_without_a_gpu(hip_lib):
+    from msf_wsi_amd import _lib, losses
+
+    with pytest.raises(_lib.MsfwsiHipError):
+        losses.top_logits(torch.zeros(2, 5), 2)
+    with pytest.raises(_lib.MsfwsiHipError):
+        losses.TopLogitDistillLoss()(torch.zeros(2, 5), losses.TopLogits(torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int32)))
+    for t in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError):
+            losses.TopLogitDistillLoss(temperature=t)
+    with pytest.raises(ValueError):
+        losses.TopLogitDistillLoss(reduction="batchmean")
+    assert hip_lib.msfwsi_top_logits(0, None, 5, 1, 5, 1, 6, 1.0, None, None, None, None) == -1       # k > classes
+    assert hip_lib.msfwsi_top_logits(0, None, 5, 1, 5, 1, 2, 1.0, None, None, None, None) == -1       # no memory
+    assert hip_lib.msfwsi_top_logits(0, None, 4, 2, 5, 1, 2, 1.0, None, None, None, None) == -1       # rows overlap
+    assert hip_lib.msfwsi_top_logits(0, None, 5, 0, 5, 1, 2, 1.0, None, None, None, None) == 0        # no rows
+    assert hip_lib.msfwsi_distill_fwd(0, None, 5, 1, 5, 1, 65, None, None, None, None, 1.0, 1, None, None, None, None, None) == -1
+    assert hip_lib.msfwsi_distill_bwd(3, None, 5, 1, 5, 1, 2, None, None, None, 1.0, None, None, None, 0, None, None) == -1
+
+
+# ---- GPU: selection --------------------------------------------------------------------------------------------------
+ROWS = [(1, 1, 1), (3, 2, 2), (5, 33, 7), (70, 64, 3), (4, 65, 64), (9, 257, 33), (33, 1000, 10), (2, 1001, 64), (3, 8191, 32), (2, 65536, 16),
+        (1, 65539, 64), (2, 131072, 5)]
+
+
+def same_top(x, k, T, got):
+    v, i, r = to.top_logits(x, k, T)
+    assert torch.equal(got.indices.cpu().long(), i)
+    assert torch.equal(got.values.cpu().double().nan_to_num(nan=9e9), v.nan_to_num(nan=9e9))
+    rest = got.rest.cpu().double()
+    fin = torch.isfinite(r)
+    assert torch.equal(rest[~fin].nan_to_num(nan=9e9), r[~fin].nan_to_num(nan=9e9))
+    E = error_of(x, T)
+    assert bool(((rest - r)[fin].abs() <= E + 2 * U * r[fin].abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("rows,C,k", ROWS)
+def test_top_logits_rows(hip_lib, dt, rows, C, k):
+    from msf_wsi_amd import losses
+
+    x = logits_of(rows, C, FP[dt], rows + C + k)
+    same_top(x, k, 0.5, losses.top_logits(x.cuda(), k, temperature=0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [40, 1000, 20011])
+@pytest.mark.parametrize("kind", ["ascending", "descending", "equal", "few", "masked", "nan", "zeros", "one block"])
+def test_top_logits_orders(hip_lib, kind, C):
+    """orders and ties that a selection by thresholds or by halves could trip over"""
+    from msf_wsi_amd import losses
+
+    g = torch.Generator().manual_seed(C)
+    k = 33
+    if kind == "ascending":
+        x = torch.arange(C).float().repeat(2, 1) / 64 - 5
+    elif kind == "descending":
+        x = -torch.arange(C).float().repeat(2, 1) / 64
+    elif kind == "equal":
+        x = torch.full((2, C), -1.5)
+    elif kind == "few":                      # three values: long ties across the border
+        x = torch.randint(0, 3, (2, C), generator=g).float()
+    elif kind == "masked":                   # fewer finite logits than k; a row with none
+        x = torch.full((2, C), -math.inf)
+        x[0, C // 2:C // 2 + 5] = torch.randn(5, generator=g)
+    elif kind == "nan":
+        x = torch.randn(3, C, generator=g)
+        x[0, 7], x[1, C - 1], x[1, 3], x[2, 11], x[2, 12] = math.nan, -math.nan, math.inf, math.inf, -math.inf
+        x[1, 5:39] = math.nan                # more of them than k: rest is NaN
+    elif kind == "zeros":                    # -0 and +0 are equal
+        x = torch.where(torch.rand(2, C, generator=g) < 0.5, -0.0, 0.0)
+    else:                                    # every large value next to the others
+        x = torch.randn(2, C, generator=g)
+        x[:, 2:38] += 50.0
+    same_top(x, k, 1.0, losses.top_logits(x.cuda(), k))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("shape,k", [((2, 6, 9, 7), 6), ((3, 21, 16, 16), 4), ((1, 64, 5), 16), ((2, 40, 300), 20), ((4, 3, 1, 1), 2)])
+def test_top_logits_maps(hip_lib, dt, shape, k):
+    from msf_wsi_amd import losses
+
+    x = logits_of(shape[0] * math.prod(shape[2:]), shape[1], FP[dt], sum(shape)).view(shape[0], *shape[2:], shape[1]).movedim(-1, 1)
+    last = x.movedim(1, -1).reshape(-1, shape[1])
+    for form in [x.contiguous().cuda(), x.cuda()] + ([x.contiguous(memory_format=torch.channels_last).cuda()] if x.dim() == 4 else []):
+        got = losses.top_logits(form, k, temperature=2.0, dim=1)
+        assert got.values.shape == (shape[0], k) + shape[2:] and got.rest.shape == (shape[0],) + shape[2:]
+        flat = losses.TopLogits(got.values.movedim(1, -1).reshape(-1, k), got.indices.movedim(1, -1).reshape(-1, k), got.rest.reshape(-1))
+        same_top(last, k, 2.0, flat)
+
+
+@pytest.mark.gpu
+def test_top_logits_slices_and_refusals(hip_lib):
+    from msf_wsi_amd import losses
+
+    wide = logits_of(6, 1050, torch.bfloat16, 3)
+    part = wide.cuda()[:, 3:1034]
+    same_top(wide[:, 3:1034], 20, 1.0, losses.top_logits(part, 20))
+    assert losses.top_logits(torch.zeros(0, 7, device="cuda"), 3).values.shape == (0, 3)
+    assert losses.top_logits(torch.zeros(2, 7, 0, device="cuda"), 3, dim=1).indices.shape == (2, 3, 0)
+    one = losses.top_logits(torch.tensor([1.0, 5.0, 2.0], device="cuda"), 2)
+    assert one.indices.tolist() == [1, 2] and one.rest.shape == ()
+    x = torch.zeros(2, 70, device="cuda")
+    for bad in (0, 65, 71):
+        with pytest.raises(ValueError):
+            losses.top_logits(x, bad)
+    with pytest.raises(ValueError):
+        losses.top_logits(torch.zeros(2, 3, 4, 5, device="cuda"), 1, dim=2)
+    with pytest.raises(TypeError):
+        losses.top_logits(x.double(), 3)
+    with pytest.raises(ValueError):
+        losses.top_logits(x, 3, temperature=0.0)
+
+
+# ---- GPU: the loss ---------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("with_rest", [False, True])
+@pytest.mark.parametrize("rows,C,k", ROWS)
+def test_loss_rows(hip_lib, dt, with_rest, rows, C, k):
+    from msf_wsi_amd import losses
+
+    T = 2.0
+    z, t = logits_of(rows, C, FP[dt], rows + C), logits_of(rows, C, torch.float32, rows * C + k)
+    v, i, r = to.top_logits(t, k, T)
+    teacher = losses.TopLogits(v.float().cuda(), i.int().cuda(), r.float().cuda() if with_rest else None)
+    g = torch.Generator().manual_seed(k)
+    mask = torch.rand(rows, generator=g) < 0.7 if rows > 3 else None
+    cm = None if mask is None else mask.cuda()
+    zc = z.cuda().requires_grad_()
+    rows_loss = losses.TopLogitDistillLoss(T, "none")(zc, teacher, cm)
+    grad, = torch.autograd.grad(rows_loss, zc, torch.ones(rows, device="cuda"))
+    check(z, teacher.values, teacher.indices, teacher.rest, mask, T, rows_loss.detach(), grad, FP[dt])
+    total = losses.TopLogitDistillLoss(T, "sum")(zc, teacher, cm)
+    mean = losses.TopLogitDistillLoss(T)(zc, teacher, cm)
+    n = rows if mask is None else int(mask.sum())
+    want = float(rows_loss.detach().double().sum())
+    assert abs(float(total) - want) <= 2 * U * abs(want) + 1e-30 and abs(float(mean) - want / max(n, 1)) <= 4 * U * abs(want) + 1e-30
+    sgrad, = torch.autograd.grad(total, zc, torch.tensor(256.0, device="cuda"))
+    check(z, teacher.values, teacher.indices, teacher.rest, mask, T, None, sgrad, FP[dt], 256.0)
+    mgrad, = torch.autograd.grad(mean, zc, torch.tensor(256.0, device="cuda"))
+    check(z, teacher.values, teacher.indices, teacher.rest, mask, T, None, mgrad, FP[dt], 256.0 / max(n, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("shape,k", [((2, 6, 9, 7), 6), ((3, 21, 16, 16), 4), ((1, 64, 5), 16), ((2, 40, 300), 20)])
+def test_loss_maps(hip_lib, dt, shape, k):
+    from msf_wsi_amd import losses
+
+    T, n = 1.0, shape[0] * math.prod(shape[2:])
+    z, t = logits_of(n, shape[1], FP[dt], 5), logits_of(n, shape[1], torch.float32, 6)
+    v, i, r = to.top_logits(t, k, T)
+    mask = torch.rand(n, generator=torch.Generator().manual_seed(1)) < 0.5
+
+    def to_map(a, last):
+        return a.view(shape[0], *shape[2:], last).movedim(-1, 1)
+
+    where = (shape[0],) + shape[2:]
+    teacher = losses.TopLogits(to_map(v.float(), k).cuda(), to_map(i.int(), k).contiguous().cuda(), r.float().view(where).cuda())
+    zm = to_map(z, shape[1])
+    for form in [zm.contiguous(), zm] + ([zm.contiguous(memory_format=torch.channels_last)] if zm.dim() == 4 else []):
+        zc = form.cuda().requires_grad_()
+        row = losses.TopLogitDistillLoss(T, "none", dim=1)(zc, teacher, mask.view(where).cuda())
+        assert row.shape == where
+        grad, = torch.autograd.grad(row.sum(), zc)
+        check(z, v.float(), i, r.float(), mask, T, row.detach().reshape(-1), grad.movedim(1, -1).reshape(n, -1), FP[dt])
+
+
+def special_case():
+    """one row for every way the inputs can be odd; (z, values, indices, rest, mask)"""
+    C, k = 300, 4
+    z, t = logits_of(16, C, torch.float32, 11), logits_of(16, C, torch.float32, 12)
+    v, i, r = to.top_logits(t, k, 1.0)
+    v, i, r = v.float(), i.int(), r.float()
+    mask = torch.ones(16, dtype=torch.bool)
+    i[1] = -1                                               # padding only, but a rest: everything is the rest
+    i[2], r[2] = -1, -math.inf                              # nothing at all
+    v[3], r[3] = -math.inf, -math.inf                       # listed classes without mass, no rest
+    i[4, 2:] = -1                                           # a shorter list
+    i[5, 1] = i[5, 0]                                       # the same class twice
+    z[6, 50:] = -math.inf                                   # masked student classes, listed ones among them
+    i[6] = torch.tensor([3, 7, 200, 9], dtype=torch.int32)
+    z[7] = -math.inf                                        # a student row that is masked out whole
+    z[8, 17], mask[8] = math.nan, False                     # NaN where nothing counts
+    v[8], i[8], r[8] = math.nan, 10 ** 9, math.nan
+    i[9, 3] = C                                             # past the classes
+    z[10, 5] = math.nan                                     # NaN that counts
+    v[11, 2] = -math.inf                                    # a listed class without mass
+    z[12] = z[12].abs().neg() - 1e4                         # far from zero
+    z[13, int(i[13, 0])] = 80.0                             # sure of the first class: almost nothing left for the others
+    z[14] = torch.finfo(torch.float32).min                  # a mask of the type's lowest value
+    z[14, 3:9] = 0.5
+    i[14], v[14] = torch.tensor([3, 4, 5, 6], dtype=torch.int32), 0.0
+    return z, v, i, r, mask
+
+
+@pytest.mark.gpu
+def test_loss_odd_rows(hip_lib):
+    from msf_wsi_amd import losses
+
+    z, v, i, r, mask = special_case()
+    for layout in ("rows", "maps"):
+        zl, vl, il = (a.t()[None].contiguous() if layout == "maps" else a for a in (z, v, i))
+        shape = (1, 16) if layout == "maps" else (16,)
+        zc = zl.cuda().requires_grad_()
+        crit = losses.TopLogitDistillLoss(1.0, "none", dim=1 if layout == "maps" else -1)
+        row = crit(zc, losses.TopLogits(vl.cuda(), il.cuda(), r.view(shape).cuda()), mask.view(shape).cuda())
+        grad, = torch.autograd.grad(row, zc, torch.ones_like(row))
+        row, grad = row.detach().reshape(-1), (grad[0].t() if layout == "maps" else grad)
+        want, wgrad, counts = to.distill(z, v, i, r, mask, 1.0)
+        assert counts.tolist() == [True, True] + [False] * 2 + [True] * 4 + [False] + [True] * 7
+        assert row.isnan().tolist() == [j in (9, 10) for j in range(16)]
+        assert torch.isinf(row).tolist() == [j in (6, 7) for j in range(16)]
+        fin = [0, 1, 4, 5, 11, 12, 13, 14, 15]
+        for j in (2, 3, 8):
+            assert float(row[j]) == 0.0 and float(grad[j].abs().max()) == 0.0
+        zz = torch.where(torch.isfinite(z[fin]), z[fin], torch.zeros(()))
+        near = zz.clone()
+        near[fin.index(14)] = near[fin.index(14)].clamp(min=-100)      # the size of the error there is that of the finite part
+        E = error_of(near, 1.0)
+        assert bool(((row[fin].cpu().double() - want[fin]).abs() <= E + 2 * U * want[fin].abs()).all())
+        assert bool(((grad[fin].cpu().double() - wgrad[fin]).abs() <= 4 * E).all())
+        # the row with masked classes: finite gradients, zero outside list and mask
+        assert bool(torch.isfinite(grad[6]).all()) and float(grad[6, 250]) == 0.0
+        assert bool(((grad[6].cpu().double() - wgrad[6]).abs() <= 4 * E).all()) and bool(((grad[7].cpu().double() - wgrad[7]).abs() <= 4 * E).all())
+        assert grad[9].isnan().all() and grad[10].isnan().all()
+        crit = losses.TopLogitDistillLoss(1.0, "mean", dim=1 if layout == "maps" else -1)
+        keep = mask.clone()
+        keep[[6, 7, 9, 10]] = False
+        m = crit(zc, losses.TopLogits(vl.cuda(), il.cuda(), r.view(shape).cuda()), keep.view(shape).cuda())
+        assert abs(float(m) - float(row[fin].double().mean())) <= 4 * U * float(row[fin].double().mean())
+        none = crit(zc, losses.TopLogits(vl.cuda(), il.cuda(), r.view(shape).cuda()), torch.zeros(shape, dtype=torch.bool, device="cuda"))
+        gone, = torch.autograd.grad(none, zc)
+        assert float(none) == 0.0 and float(gone.abs().max()) == 0.0
+
+
+@pytest.mark.gpu
+def test_loss_per_row_gradients_slices_and_repeats(hip_lib):
+    from msf_wsi_amd import losses
+
+    z, t = logits_of(12, 517, torch.bfloat16, 21), logits_of(12, 517, torch.float32, 22)
+    v, i, r = to.top_logits(t, 5, 0.5)
+    v, i, r = v.float().cuda(), i.int().cuda(), r.float().cuda()
+    w = torch.randn(12, generator=torch.Generator().manual_seed(2)).cuda()
+    crit = losses.TopLogitDistillLoss(0.5, "none")
+    wide = torch.zeros(12, 531, dtype=torch.bfloat16, device="cuda")
+    wide[:, 7:524] = z.cuda()
+    part = wide[:, 7:524].requires_grad_()
+    zc = z.cuda().requires_grad_()
+    a, b = crit(zc, losses.TopLogits(v, i, r)), crit(part, losses.TopLogits(v, i, r))
+    ga, gb = torch.autograd.grad(a, zc, w)[0], torch.autograd.grad(b, part, w)[0]
+    assert torch.equal(a, b) and torch.equal(ga, gb)
+    for again in range(3):                                   # the same call gives the same bits
+        assert torch.equal(crit(zc, losses.TopLogits(v, i, r)), a)
+    one = torch.autograd.grad(crit(zc, losses.TopLogits(v, i, r)), zc, torch.ones(12, device="cuda"))[0]
+    assert bool(((ga.double() - one.double() * w.double()[:, None]).abs() <= 2.0 ** -7 * (one.double() * w.double()[:, None]).abs() + 1e-30).all())
+    zs = z.cuda()[3:9].detach().requires_grad_()             # slices of a batch, at any alignment
+    part = crit(zs, losses.TopLogits(v[3:9], i[3:9], r[3:9]), torch.ones(12, dtype=torch.bool, device="cuda")[5:11])
+    assert torch.equal(part, a[3:9])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = crit(zc, losses.TopLogits(v, i, r))
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(other, a)
+
+
+@pytest.mark.gpu
+def test_loss_empty_and_refused(hip_lib):
+    from msf_wsi_amd import losses
+
+    f32, i32 = dict(device="cuda"), dict(device="cuda", dtype=torch.int32)
+    z = torch.zeros(0, 9, requires_grad=True, **f32)
+    loss = losses.TopLogitDistillLoss()(z, losses.TopLogits(torch.zeros(0, 2, **f32), torch.zeros(0, 2, **i32)))
+    loss.backward()
+    assert float(loss) == 0.0 and z.grad.shape == (0, 9)
+    z = torch.zeros(3, 9, requires_grad=True, **f32)
+    v, i = torch.zeros(3, 2, **f32), torch.zeros(3, 2, **i32)
+    crit, TL = losses.TopLogitDistillLoss(), losses.TopLogits
+    for bad in (TL(v[:2], i[:2]), TL(v, i[:, :1]), TL(v, i, torch.zeros(2, **f32)), TL(v, i, torch.zeros(3, device="cuda", dtype=torch.float64)),
+                TL(torch.zeros(3, 65, **f32), torch.zeros(3, 65, **i32)), TL(torch.zeros(3, 0, **f32), torch.zeros(3, 0, **i32)),
+                TL(v.clone().requires_grad_(), i)):
+        with pytest.raises(ValueError):
+            crit(z, bad)
+    for bad in (TL(v, i.long()), TL(v.half(), i)):
+        with pytest.raises(TypeError):
+            crit(z, bad)
+    with pytest.raises(ValueError):
+        crit(z, TL(v, i), torch.ones(3, device="cuda"))
+    with pytest.raises(TypeError):
+        crit(z.double(), TL(v, i))
+    with pytest.raises(ValueError):
+        losses.TopLogitDistillLoss(dim=2)(torch.zeros(2, 3, 4, 5, **f32), TL(v, i))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,dim", [((40, 1000), -1), ((2, 21, 24, 24), 1), ((3, 70001), -1)])
+def test_captured_selection_and_loss(hip_lib, shape, dim):
+    from msf_wsi_amd import losses
+
+    C = shape[dim]
+    t = logits_of(math.prod(shape) // C, C, torch.bfloat16, 30).cuda().view(shape)
+    z = logits_of(math.prod(shape) // C, C, torch.bfloat16, 31).cuda().view(shape).requires_grad_()
+    crit = losses.TopLogitDistillLoss(2.0, dim=dim)
+
+    def step():
+        top = losses.top_logits(t, 8, 2.0, dim=dim)
+        loss = crit(z, top)
+        return tuple(top) + (loss.detach(), torch.autograd.grad(loss, z)[0])
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (32, 33, 34):
+        with torch.no_grad():
+            t.copy_(logits_of(math.prod(shape) // C, C, torch.bfloat16, seed).view(shape))
+            z.copy_(logits_of(math.prod(shape) // C, C, torch.bfloat16, seed + 9).view(shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@pytest.mark.gpu
+def test_frozen_teacher_chain(hip_lib):
+    """as they are used together: a 4-bit teacher head, its top logits, the loss of a student that ends in a 4-bit head of its
+    own, and the gradient of the student's features against float64 through the same 4-bit values"""
+    from msf_wsi_amd import losses, quant
+
+    torch.manual_seed(3)
+    head = torch.nn.Linear(512, 1500).cuda()
+    teacher, student = quant.MX4Linear.from_linear(head), quant.MX4Linear.from_linear(torch.nn.Linear(512, 1500).cuda())
+    feats = torch.randn(24, 512, device="cuda")
+    with torch.no_grad():
+        top = losses.top_logits(teacher(feats), 12, temperature=2.0)
+    x = torch.randn(24, 512, device="cuda", requires_grad=True)
+    logits = student(x)
+    loss = losses.TopLogitDistillLoss(2.0)(logits, top)
+    loss.backward()
+    w = quant.MX4Tensor(student.codes, student.scales, 512).dequantize().cpu().double()
+    y = to.mx4_round(x.detach().cpu())[0] @ w.t() + student.bias.cpu().double()
+    rows, grad, _ = to.distill(y, top.values.cpu(), top.indices.cpu(), top.rest.cpu(), None, 2.0)
+    # the logits' own error (520 * 2^-23 of their mass) moves log q by twice as much, the gradient by as much of q
+    mass = to.mx4_round(x.detach().cpu())[0].abs() @ w.abs().t() + student.bias.cpu().double().abs()
+    dy = 520 * 2.0 ** -23 * float(mass.max())
+    assert abs(float(loss) - float(rows.mean())) <= 4.0 * (2 * dy / 2.0 + error_of(y, 2.0))
+    want = grad @ w / 24
+    lim = (2 * dy + 2 * error_of(y, 2.0)) * 2.0 * 3 * float(w.abs().max()) / 24 + 1508 * 3 * 2.0 ** -23 * float((grad.abs() @ w.abs()).max()) / 24
+    assert float((x.grad.cpu().double() - want).abs().max()) <= lim

@@ -1,0 +1,322 @@
+"""4-bit storage and its products against float64.
+
+Quantisation is compared bit for bit: every step of it is exact but the one rounding.  Products: the products of the 4-bit
+values are exact and each of the cols additions in fp32 is off by at most one step (2^-23) of a partial sum that is at most
+sum |a b|; the result is then rounded once to its type (half a step, eps / 2, and in fp16 half a subnormal step, 2^-25)."""
+import math
+
+import pytest
+import torch
+
+from oracle import teacher_oracle as to
+
+FP = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+TINY = {torch.float32: 2.0 ** -150, torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}
+
+
+def features(rows, cols, dt, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(rows, cols, generator=g) * torch.exp(torch.randn(cols, generator=g))).to(dt)
+
+
+def bound(terms, mass, want, dt):
+    """mass = sum |a b| of every output"""
+    return (terms + 8) * 2.0 ** -23 * mass + torch.finfo(dt).eps / 2 * want.abs() * (1 + 1e-6) + TINY[dt]
+
+
+# ---- CPU: the oracle on cases checked by hand, refusals --------------------------------------------------------------
+def test_oracle_by_hand():
+    x = torch.zeros(1, 64)
+    x[0, :9] = torch.tensor([7.9, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -5.01])   # scale 1: floor(log2 7.9) = 2
+    x[0, 32] = 2.0 ** -140
+    v, code = to.mx4_round(x)
+    assert code.tolist() == [[127, 0]]
+    assert v[0, :9].tolist() == [6.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, -6.0]
+    assert float(v[0, 32]) == 0.0                                                  # 2^-13 of the smallest scale 2^-127
+    codes, scales = to.mx4_pack(x)
+    assert codes.shape == (1, 1, 128) and codes[0, 0, :5].tolist() == [0x07, 0x22, 0x44, 0x66, 0x0F]
+    assert scales[0, 0, :2].tolist() == [127, 0]
+
+
+def test_refusals_without_a_gpu():
+    from msf_wsi_amd import _lib, quant
+
+    with pytest.raises(_lib.MsfwsiHipError):
+        quant.quantize_mx4(torch.zeros(2, 32))
+    with pytest.raises(_lib.MsfwsiHipError):
+        quant.MX4Tensor(torch.zeros(1, 2, 128, dtype=torch.uint8), torch.zeros(1, 2, 8, dtype=torch.uint8), 32)
+    with pytest.raises(TypeError):
+        quant.mx4_linear(torch.zeros(2, 32), torch.zeros(3, 32))
+
+
+def test_c_entry_checks(hip_lib):
+    """bad sizes come back as an error code before anything is launched"""
+    assert hip_lib.msfwsi_mx4_quantize(7, None, 32, 1, 32, None, None, None) == -1
+    assert hip_lib.msfwsi_mx4_quantize(0, None, 32, 1, 32, None, None, None) == -1     # no memory
+    assert hip_lib.msfwsi_mx4_quantize(0, None, 16, 2, 32, None, None, None) == -1     # rows overlap
+    assert hip_lib.msfwsi_mx4_quantize(0, None, 32, 0, 32, None, None, None) == 0      # no rows
+    assert hip_lib.msfwsi_mx4_dequantize(0, None, None, 1, 0, None, None) == -1
+    assert hip_lib.msfwsi_mx4_dgrad(0, None, 4, 1, None, None, 0, 32, 0, None, None) == -1
+
+
+# ---- GPU -------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 256), (3, 31), (7, 33), (9, 255), (5, 257), (130, 1001), (64, 2048), (17, 4608)])
+def test_quantize_bit_for_bit(hip_lib, dt, rows, cols):
+    from msf_wsi_amd import quant
+
+    x = features(rows, cols, FP[dt], rows * 7919 + cols)
+    codes, scales = to.mx4_pack(x)
+    q = quant.quantize_mx4(x.cuda())
+    assert torch.equal(q.scales.cpu(), scales)
+    assert torch.equal(q.codes.cpu(), codes)
+    v, _ = to.mx4_round(x)
+    assert torch.equal(q.dequantize().cpu().double(), v)
+    assert torch.equal(q.dequantize(torch.bfloat16).cpu(), v.to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_quantize_every_border_and_scale(hip_lib):
+    """all midpoints and their neighbours under every scale an fp32 block can take, subnormal blocks among them"""
+    from msf_wsi_amd import quant
+
+    mids = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0])
+    line = torch.cat([mids, torch.nextafter(mids, torch.tensor(0.0)), torch.nextafter(mids, torch.tensor(9.0))])
+    block = torch.zeros(32)
+    block[:27], block[27:31], block[31] = line, torch.tensor([4.0, 0.0, -0.5, 1e-3]), -7.5
+    rows = []
+    for e in range(-149, 126):
+        rows.append(torch.ldexp(block.double(), torch.tensor(e)).float())
+    x = torch.stack(rows)
+    q = quant.quantize_mx4(x.cuda())
+    codes, scales = to.mx4_pack(x)
+    assert torch.equal(q.scales.cpu(), scales) and torch.equal(q.codes.cpu(), codes)
+    assert torch.equal(q.dequantize().cpu().double(), to.mx4_round(x)[0])
+
+
+@pytest.mark.gpu
+def test_quantize_nonfinite_and_empty(hip_lib):
+    from msf_wsi_amd import quant
+
+    x = torch.ones(4, 96)
+    x[0, 5], x[1, 40], x[2, 95] = math.nan, math.inf, -math.inf
+    x[3] = 0.0
+    q = quant.quantize_mx4(x.cuda())
+    assert q.scales[0, :, :3].tolist() == [[255, 125, 125], [125, 255, 125], [125, 125, 255], [0, 0, 0]]
+    back = q.dequantize().cpu()
+    assert back[0, :32].isnan().all() and back[1, 32:64].isnan().all() and back[2, 64:].isnan().all()
+    assert int(back.isnan().sum()) == 96 and float(back[3].abs().max()) == 0.0
+    none = quant.quantize_mx4(torch.zeros(0, 40, device="cuda"))
+    assert none.shape == (0, 40) and none.dequantize().shape == (0, 40)
+    w = quant.quantize_mx4(x[3:].cuda())
+    assert quant.mx4_linear(torch.zeros(0, 96, device="cuda"), w).shape == (0, 1)
+    y = quant.mx4_linear(x.cuda(), quant.quantize_mx4(torch.ones(2, 96, device="cuda"))).cpu()
+    assert y[:3].isnan().all() and y[3].tolist() == [0.0, 0.0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("offset,pitch", [(0, 300), (1, 301), (3, 517)])
+def test_quantize_slices(hip_lib, dt, offset, pitch):
+    """rows of a wider tensor at any alignment: the same codes as of a copy"""
+    from msf_wsi_amd import quant
+
+    base = features(11, pitch + 8, FP[dt], pitch).cuda()
+    part = base[:, offset:offset + 291]
+    a, b = quant.quantize_mx4(part), quant.quantize_mx4(part.contiguous())
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales)
+    t = base[:, :11].t()
+    assert torch.equal(quant.quantize_mx4(t).codes, quant.quantize_mx4(t.contiguous()).codes)
+
+
+SIZES = [(1, 1, 1), (1, 256, 1000), (2, 513, 33), (5, 64, 7), (31, 255, 65), (33, 1001, 129), (64, 2048, 512), (130, 300, 257), (257, 4608, 300),
+         (300, 256, 1), (1, 18432, 40), (16, 9216, 64), (520, 2304, 391)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_linear_forward_and_gradient(hip_lib, dt, M, K, N):
+    from msf_wsi_amd import quant
+
+    dt = FP[dt]
+    g = torch.Generator().manual_seed(M * 31 + K * 7 + N)
+    x = features(M, K, dt, M + K)
+    w = torch.randn(N, K, generator=g) / math.sqrt(K)
+    bias = torch.randn(N, generator=g) if N % 2 else None
+    dy = torch.randn(M, N, generator=g).to(dt)
+    xq, wq = to.mx4_round(x)[0].cuda(), to.mx4_round(w)[0].cuda()
+    b64 = 0.0 if bias is None else bias.double().cuda()
+    want = xq @ wq.t() + b64
+    mass = xq.abs() @ wq.abs().t() + (0.0 if bias is None else b64.abs())
+    w4 = quant.quantize_mx4(w.cuda())
+    xc = x.cuda().requires_grad_()
+    y = quant.mx4_linear(xc, w4, None if bias is None else bias.cuda())
+    assert y.dtype == dt and y.shape == (M, N)
+    assert bool(((y.double() - want).abs() <= bound(K, mass, want, dt)).all())
+    dx, = torch.autograd.grad(y, xc, dy.cuda())
+    d64 = dy.double().cuda()
+    want, mass = d64 @ wq, d64.abs() @ wq.abs()
+    assert dx.dtype == dt and dx.shape == (M, K)
+    # an fp32 gradient is multiplied in three parts: three additions for each of the N terms
+    assert bool(((dx.double() - want).abs() <= bound(3 * N, mass, want, dt)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out", list(FP))
+def test_linear_of_quantized_input_and_other_output_type(hip_lib, out):
+    from msf_wsi_amd import quant
+
+    x, w = features(40, 600, torch.bfloat16, 1).cuda(), features(70, 600, torch.float32, 2).cuda() / 25
+    w4 = quant.quantize_mx4(w)
+    a = quant.mx4_linear(x, w4, out_dtype=FP[out])
+    b = quant.mx4_linear(quant.quantize_mx4(x), w4, out_dtype=FP[out])
+    assert a.dtype == FP[out] and torch.equal(a, b)
+    assert quant.mx4_linear(quant.quantize_mx4(x), w4).dtype == torch.float32
+
+
+@pytest.mark.gpu
+def test_weights_of_very_different_size(hip_lib):
+    """scales up to 2^100 apart, in both operands' directions: every block's own scale counts"""
+    from msf_wsi_amd import quant
+
+    x = features(20, 512, torch.float32, 5)
+    w = features(48, 512, torch.float32, 6)
+    x[:, ::64] *= 2.0 ** -40
+    w[::3] *= 2.0 ** 50
+    w[1::3] *= 2.0 ** -50
+    xq, wq = to.mx4_round(x)[0], to.mx4_round(w)[0]
+    want, mass = xq @ wq.t(), xq.abs() @ wq.abs().t()
+    xc = x.cuda().requires_grad_()
+    y = quant.mx4_linear(xc, quant.quantize_mx4(w.cuda()))
+    assert bool(((y.cpu().double() - want).abs() <= bound(512, mass, want, torch.float32)).all())
+    for dt in FP.values():
+        dy = features(20, 48, dt, 7).clamp(-100, 100)
+        xc = x.to(torch.float32).cuda().requires_grad_()
+        y = quant.mx4_linear(xc, quant.quantize_mx4(w.cuda()), out_dtype=dt)
+        dx, = torch.autograd.grad(y, xc, dy.cuda())
+        want, mass = dy.double() @ wq, dy.double().abs() @ wq.abs()
+        assert bool(((dx.cpu().double() - want).abs() <= bound(3 * 48, mass, want, torch.float32)).all()), dt
+
+
+@pytest.mark.gpu
+def test_gradient_by_differences(hip_lib):
+    """the layer behind the rounding of x is linear: a step of x that stays on the 4-bit values moves y by exactly dx"""
+    from msf_wsi_amd import quant
+
+    levels = torch.tensor(to.LEVELS)
+    g = torch.Generator().manual_seed(3)
+    x = levels[torch.randint(0, 7, (6, 288), generator=g)].cuda()
+    x[:, ::32] = 6.0                                        # fixes every block's scale at 1
+    w4 = quant.quantize_mx4((torch.randn(10, 288, generator=g) / 16).cuda())
+    c = torch.randn(6, 10, generator=g).cuda()
+    xr = x.clone().requires_grad_()
+    dx, = torch.autograd.grad((quant.mx4_linear(xr, w4) * c).sum(), xr)
+    step = torch.zeros_like(x)
+    step[:, 1] = torch.where(x[:, 1] < 2, 0.5, torch.where(x[:, 1] < 4, 1.0, 2.0))
+    moved = ((quant.mx4_linear(x + step, w4).double() - quant.mx4_linear(x, w4).double()) * c.double()).sum()
+    mass = (x.double().abs() + step.double()) @ w4.dequantize().double().abs().t()
+    assert abs(float(moved) - float((dx * step).double().sum())) <= 4 * 300 * 2.0 ** -23 * float((mass * c.double().abs()).sum())
+
+
+@pytest.mark.gpu
+def test_layouts_streams_and_batches(hip_lib):
+    from msf_wsi_amd import quant
+
+    w4 = quant.quantize_mx4(features(96, 320, torch.float32, 8).cuda())
+    x = features(30, 320, torch.bfloat16, 9).cuda()
+    want = quant.mx4_linear(x, w4)
+    assert torch.equal(quant.mx4_linear(x.view(5, 6, 320), w4).view(30, 96), want)
+    wide = torch.zeros(30, 333, dtype=x.dtype, device="cuda")
+    wide[:, 5:325] = x
+    part = wide[:, 5:325].requires_grad_()
+    y = quant.mx4_linear(part, w4)
+    assert torch.equal(y, want)
+    full, = torch.autograd.grad(y, part, torch.ones_like(y))
+    xr = x.clone().requires_grad_()
+    some, = torch.autograd.grad(quant.mx4_linear(xr, w4).sum(), xr)     # an expanded gradient: one value for all
+    assert torch.equal(full, some)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = quant.mx4_linear(x, w4)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(other, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(1, 2304, 700), (40, 600, 300), (300, 1024, 520)])
+def test_captured_forward_and_backward(hip_lib, M, K, N):
+    from msf_wsi_amd import quant
+
+    w4 = quant.quantize_mx4(features(N, K, torch.float32, 8).cuda() / 30)
+    x = features(M, K, torch.bfloat16, 9).cuda().requires_grad_()
+    dy = features(M, N, torch.bfloat16, 10).cuda()
+
+    def both():
+        y = quant.mx4_linear(x, w4)
+        return y.detach(), torch.autograd.grad(y, x, dy)[0]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        both()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, dx = both()
+    for seed in (11, 12, 13):
+        with torch.no_grad():
+            x.copy_(features(M, K, torch.bfloat16, seed))
+            dy.copy_(features(M, N, torch.bfloat16, seed + 50))
+        graph.replay()
+        torch.cuda.synchronize()
+        ey, edx = both()
+        assert torch.equal(y, ey) and torch.equal(dx, edx)
+
+
+@pytest.mark.gpu
+def test_refusals(hip_lib):
+    from msf_wsi_amd import _lib, quant
+
+    w4 = quant.quantize_mx4(torch.ones(8, 64, device="cuda"))
+    with pytest.raises(ValueError):
+        quant.mx4_linear(torch.zeros(2, 63, device="cuda"), w4)
+    with pytest.raises(TypeError):
+        quant.mx4_linear(torch.zeros(2, 64, device="cuda", dtype=torch.float64), w4)
+    with pytest.raises(TypeError):
+        quant.quantize_mx4(torch.zeros(2, 64, device="cuda", dtype=torch.int32))
+    with pytest.raises(_lib.MsfwsiHipError):
+        quant.mx4_linear(torch.zeros(2, 64), w4)
+    with pytest.raises(ValueError):
+        quant.mx4_linear(torch.zeros(2, 64, device="cuda"), w4, torch.zeros(8, device="cuda", requires_grad=True))
+    with pytest.raises(TypeError):
+        quant.mx4_linear(torch.zeros(2, 64, device="cuda"), w4, torch.zeros(8, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        quant.mx4_linear(torch.zeros(2, 64, device="cuda"), w4, torch.zeros(7, device="cuda"))
+    with pytest.raises(ValueError):
+        quant.MX4Tensor(w4.codes, w4.scales, 257)
+    with pytest.raises(ValueError):
+        quant.MX4Tensor(w4.codes, w4.scales[:, :4].contiguous(), 64)
+    with pytest.raises(ValueError):
+        quant.quantize_mx4(torch.zeros(3, 0, device="cuda"))
+    x = torch.zeros(2, 64, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(quant.mx4_linear(x, w4).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_module_and_state(hip_lib):
+    from msf_wsi_amd import quant
+
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(200, 70).cuda()
+    layer = quant.MX4Linear.from_linear(lin)
+    x = torch.randn(9, 200, device="cuda")
+    want = quant.mx4_linear(x, quant.quantize_mx4(lin.weight), lin.bias.detach())
+    assert torch.equal(layer(x), want)
+    other = quant.MX4Linear.from_linear(torch.nn.Linear(200, 70).cuda())
+    other.load_state_dict(layer.state_dict())
+    assert torch.equal(other(x), want) and not list(layer.parameters())
