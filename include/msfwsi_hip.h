@@ -545,14 +545,17 @@ int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, const void* 
  * Logits [outer][classes][inner]: inner = 1 with rows `ld` elements apart, or contiguous maps (ld = classes * inner).  values /
  * indices [outer][k][inner], rest and mask [outer * inner]; k <= 64.  No operator of the reference: no parity to pin.
  *   msfwsi_top_logits:  the k largest (descending; ties by ascending index; NaN above all numbers), their indices, and
- *                       rest = log sum over the others of exp(logit * inv_t)
- *   msfwsi_distill_fwd: row_loss [rows] (0 where a row does not count), stats [rows][4] for the backward, loss[0] = sum or mean
+ *                       rest = log sum over the others of exp(logit * inv_t).  workspace: msfwsi_top_logits_workspace
+ *                       bytes, 16-byte aligned (a host call; NULL when it says 0)
+ *   msfwsi_distill_fwd: row_loss [rows] or NULL (0 where a row does not count), stats [rows][4] (16-byte aligned) for the
+ *                       backward, partials [2048][2] scratch, loss[0] = sum or mean
  *                       over the rows that count, loss[1] = the gradient's factor.  rest / mask may be NULL.
  *                       outer = 0 writes loss alone
  *   msfwsi_distill_bwd: dz [outer][classes][inner] contiguous = g * factor[1] * d loss_row / dz; g holds one value, or one per
  *                       row with g_rows; factor (NULL = 1) is the forward's loss pair */
+int msfwsi_top_logits_workspace(int dtype, long outer, int classes, long inner, int k, long* bytes);
 int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, int classes, long inner, int k, float inv_t, float* values,
-                      int* indices, float* rest, void* stream);
+                      int* indices, float* rest, void* workspace, void* stream);
 int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer, int classes, long inner, int k, const float* values,
                        const int* indices, const float* rest, const unsigned char* mask, float temperature, int mean,
                        float* stats, float* row_loss, float* loss, double* partials, void* stream);

@@ -115,7 +115,8 @@ SIGNATURES = {
     "msfwsi_mx4_dequantize": [_i, _vp, _vp, _l, _l, _vp, _vp],
     "msfwsi_mx4_gemm": [_i, _vp, _vp, _l, _vp, _vp, _l, _l, _vp, _vp, _vp],
     "msfwsi_mx4_dgrad": [_i, _vp, _l, _l, _vp, _vp, _l, _l, _i, _vp, _vp],
-    "msfwsi_top_logits": [_i, _vp, _l, _l, _i, _l, _i, _f, _vp, _vp, _vp, _vp],
+    "msfwsi_top_logits_workspace": [_i, _l, _i, _l, _i, _vp],
+    "msfwsi_top_logits": [_i, _vp, _l, _l, _i, _l, _i, _f, _vp, _vp, _vp, _vp, _vp],
     "msfwsi_distill_fwd": [_i, _vp, _l, _l, _i, _l, _i, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _vp, _vp, _vp],
     "msfwsi_distill_bwd": [_i, _vp, _l, _l, _i, _l, _i, _vp, _vp, _vp, _f, _vp, _vp, _vp, _i, _vp, _vp],
     "msfwsi_set_tuning": [_i, _l],

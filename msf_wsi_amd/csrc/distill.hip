@@ -25,7 +25,15 @@
 namespace {
 
 constexpr int kT = 256;
-constexpr int kMaxK = 64;
+constexpr int kMaxK = 64;        // = the lanes of a wave: lane i holds entry i of a teacher's list
+constexpr int kMaxParts = 2048;  // workgroups of the forward at most; each leaves one (sum, count) pair
+constexpr int kCand = 512;       // candidates a selection ranks at once
+constexpr int kSeg = 65536;      // classes whose list membership is held as bits at a time
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// 2^x and log2 x as the hardware has them (1 ulp; results below 2^-126 are flushed: sums are taken relative to their largest term)
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
 
 // fp32 -> int of the same order; -0 equals +0, every NaN is the largest
 __device__ __forceinline__ int order_of(float x) {
@@ -33,225 +41,790 @@ __device__ __forceinline__ int order_of(float x) {
     const int b = (int)__float_as_uint(x + 0.f);
     return b ^ ((b >> 31) & 0x7fffffff);
 }
-__device__ __forceinline__ float value_of(int order) {  // 0x80000000, below every number, stands for nothing: -inf
-    if (order == (int)0x80000000) return -INFINITY;
+constexpr int kNothing = (int)0x80000000;  // the order of an empty slot, below every number's
+__device__ __forceinline__ float value_of(int order) {
+    if (order == kNothing) return -INFINITY;
     return __uint_as_float((unsigned)(order ^ ((order >> 31) & 0x7fffffff)));
 }
+// (order, index) as one number: larger logits first, equal ones by ascending index; unique within a row
 __device__ __forceinline__ long key_of(float x, int idx) { return ((long)order_of(x) << 32) | (unsigned)(0x7fffffff - idx); }
+__device__ __forceinline__ int index_of(long key) { return 0x7fffffff - (int)(unsigned)key; }
+constexpr long kNoKey = (long)0x8000000000000000L;
 
-template <typename V, typename OP>
-__device__ __forceinline__ V block_all(V v, V* buf, OP op) {
+// sum of 2^((x - m) c) over some logits x: c = log2(e) / T, m the largest of them.  Nothing: m = -inf, s = 0; a NaN among them
+// makes s NaN.  The difference is taken before the product, so logits far from zero keep their precision.
+struct Sum {
+    float m, s;
+};
+__device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
+    const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
+    return {m, a.s * exp2_((a.m - ref) * c) + b.s * exp2_((b.m - ref) * c)};
+}
+__device__ __forceinline__ Sum one(float x) { return {x, x == -INFINITY ? 0.f : 1.f}; }
+__device__ __forceinline__ float log_of(Sum v, float inv_t) { return v.s == 0.f ? -INFINITY : v.m * inv_t + log2_(v.s) * kLn2; }
+__device__ __forceinline__ Sum wave_join(Sum v, float c) {
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = op(v, __shfl_xor(v, off, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = buf[0];
-    for (int i = 1; i < kT / 64; ++i) v = op(v, buf[i]);
+    for (int off = 32; off > 0; off >>= 1) v = join(v, {__shfl_xor(v.m, off, 64), __shfl_xor(v.s, off, 64)}, c);
     return v;
 }
-struct OpMax {
-    __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
-    __device__ long operator()(long a, long b) const { return a > b ? a : b; }
-};
-struct OpAdd {
-    __device__ float operator()(float a, float b) const { return a + b; }
-};
-
-template <typename T>
-__global__ void __launch_bounds__(kT) top_logits_kernel(const T* __restrict__ x, long ld, int C, long inner, int k, float inv_t,
-                                                        float* __restrict__ values, int* __restrict__ indices, float* __restrict__ rest) {
-    __shared__ long lbuf[kT / 64];
-    __shared__ float fbuf[kT / 64];
-    const long o = blockIdx.x / inner, i = blockIdx.x % inner;
-    const T* p = x + o * ld + i;
-    long last = 0x7fffffffffffffffL;
-    for (int s = 0; s < k; ++s) {
-        long best = (long)0x8000000000000000L;
-        for (int c = threadIdx.x; c < C; c += kT) {
-            const long key = key_of(load_elem<T>(p, c * inner), c);
-            if (key < last && key > best) best = key;
-        }
-        last = block_all(best, lbuf, OpMax());
-        if (threadIdx.x == 0) {
-            const int c = 0x7fffffff - (int)(unsigned)last;
-            values[(o * k + s) * inner + i] = load_elem<T>(p, c * inner);
-            indices[(o * k + s) * inner + i] = c;
-        }
+// over the workgroup; every thread has the result
+template <int NT>
+__device__ __forceinline__ Sum block_join(Sum v, Sum* buf, float c) {
+    v = wave_join(v, c);
+    if constexpr (NT > 64) {
+        if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = buf[0];
+        for (int i = 1; i < NT / 64; ++i) v = join(v, buf[i], c);
+        __syncthreads();
     }
-    long most = (long)0x8000000000000000L;  // the largest of the others, NaN on top
-    float sum = 0.f;
-    for (int c = threadIdx.x; c < C; c += kT) {
-        const long key = key_of(load_elem<T>(p, c * inner), c);
-        if (key < last && key > most) most = key;
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float o = __shfl_xor(v, off, 64);
+        v = v != v || o <= v ? v : o;  // NaN stays
     }
-    most = block_all(most, lbuf, OpMax());
-    const float top = value_of((int)(most >> 32));
-    const float m = top == -INFINITY ? 0.f : top;
-    for (int c = threadIdx.x; c < C; c += kT) {
-        const float v = load_elem<T>(p, c * inner);
-        if (key_of(v, c) < last) sum += expf((v - m) * inv_t);
-    }
-    sum = block_all(sum, fbuf, OpAdd());
-    if (threadIdx.x == 0) rest[blockIdx.x] = top == INFINITY ? top : m * inv_t + logf(sum);
+    return v;
 }
 
-// the teacher's distribution of one row, in LDS: p[i] (0 for padding), p_r; false when the row holds nothing
-struct Teacher {
-    float p[kMaxK], logp[kMaxK];
-    int idx[kMaxK];
-    float pr, logpr;
-    int holds, bad;
-};
-__device__ __forceinline__ void teacher_row(Teacher& t, const float* __restrict__ values, const int* __restrict__ indices,
-                                            const float* __restrict__ rest, long row, long o, long i, long inner, int k, int C, float inv_t) {
-    if (threadIdx.x == 0) {
-        float top = -INFINITY, sum = 0.f;
-        int bad = 0;
-        const float r = rest != nullptr ? rest[row] : -INFINITY;
-        top = r;
-        for (int s = 0; s < k; ++s) {
-            const int c = indices[(o * k + s) * inner + i];
-            const float v = c < 0 ? -INFINITY : values[(o * k + s) * inner + i] * inv_t;
-            bad |= c >= C;
-            t.idx[s] = c;
-            t.logp[s] = v;
-            top = v != v ? v : v > top ? v : top;
-        }
-        const float m = top == -INFINITY ? 0.f : top;
-        for (int s = 0; s < k; ++s) sum += expf(t.logp[s] - m);
-        sum += expf(r - m);
-        const float L = m + logf(sum);
-        for (int s = 0; s < k; ++s) {
-            t.logp[s] -= L;
-            t.p[s] = expf(t.logp[s]);
-        }
-        t.logpr = r - L;
-        t.pr = expf(t.logpr);
-        t.holds = top != -INFINITY;
-        t.bad = bad;
-    }
-    __syncthreads();
-}
-
+// 16 bytes of a row at any alignment; elements past the row are -inf
 template <typename T>
-__global__ void __launch_bounds__(kT) distill_fwd_kernel(const T* __restrict__ z, long ld, int C, long inner, int k,
-                                                         const float* __restrict__ values, const int* __restrict__ indices,
-                                                         const float* __restrict__ rest, const unsigned char* __restrict__ mask, float temp,
-                                                         float inv_t, float4* __restrict__ stats, float* __restrict__ row_loss) {
-    __shared__ Teacher t;
-    __shared__ float buf[kT / 64];
-    const long row = blockIdx.x, o = row / inner, i = row % inner;
-    teacher_row(t, values, indices, rest, row, o, i, inner, k, C, inv_t);
-    if (!t.holds || (mask != nullptr && mask[row] == 0)) {
-        if (threadIdx.x == 0) stats[row] = make_float4(0.f, 0.f, 0.f, 0.f), row_loss[row] = 0.f;
+struct __attribute__((packed, aligned(sizeof(T)))) Unaligned16 {
+    unsigned x, y, z, w;
+};
+template <typename T>
+__device__ __forceinline__ uint4 load_chunk(const T* __restrict__ p, int c, int n) {
+    constexpr int VEC = ElemTraits<T>::VEC;
+    if (c + VEC <= n) {
+        const Unaligned16<T> u = *reinterpret_cast<const Unaligned16<T>*>(p + c);
+        return make_uint4(u.x, u.y, u.z, u.w);
+    }
+    float f[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) f[e] = c + e < n ? load_elem<T>(p, c + e) : -INFINITY;
+    return pack16<T>(f);
+}
+// keeps hipcc from carrying the unpacked forms of a register chunk (2x its size, more with their keys) from one walk to the next
+__device__ __forceinline__ void unknown(uint4& v) { asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w)); }
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* __restrict__ p, int c, int n, const float* f) {
+    constexpr int VEC = ElemTraits<T>::VEC;
+    if (c + VEC <= n) {
+        const uint4 v = pack16<T>(f);
+        *reinterpret_cast<Unaligned16<T>*>(p + c) = {v.x, v.y, v.z, v.w};
         return;
     }
-    const T* p = z + o * ld + i;
-    float top = -INFINITY;
-    for (int c = threadIdx.x; c < C; c += kT) top = fmaxf(top, load_elem<T>(p, c * inner));
-    top = block_all(top, buf, OpMax());
-    const float m = top == -INFINITY ? 0.f : top;
-    float all = 0.f, spare = 0.f;
-    for (int c = threadIdx.x; c < C; c += kT) {
-        const float e = expf((load_elem<T>(p, c * inner) - m) * inv_t);
-        bool listed = false;
-        for (int s = 0; s < k; ++s) listed |= t.idx[s] == c;
-        all += e;
-        spare += listed ? 0.f : e;
-    }
-    all = block_all(all, buf, OpAdd());
-    spare = block_all(spare, buf, OpAdd());
-    if (threadIdx.x == 0) {
-        const float ls = all == 0.f ? 0.f : logf(all), lr = logf(spare);
-        float loss = t.pr != 0.f ? t.pr * (t.logpr - (lr - ls)) : 0.f;
-        for (int s = 0; s < k; ++s)
-            if (t.idx[s] >= 0 && t.idx[s] < C && t.p[s] != 0.f)
-                loss += t.p[s] * (t.logp[s] - ((load_elem<T>(p, t.idx[s] * inner) - m) * inv_t - ls));
-        row_loss[row] = t.bad ? NAN : temp * temp * loss;
-        stats[row] = make_float4(t.bad ? NAN : m, ls, spare == 0.f ? 0.f : lr, spare == 0.f ? 2.f : 1.f);
-    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e)
+        if (c + e < n) store_elem<T>(p, c + e, f[e]);
 }
 
-// loss[0] = sum or mean of the rows that count, loss[1] = the factor of the gradient (1 / their number for the mean)
-__global__ void __launch_bounds__(kT) distill_reduce_kernel(const float4* __restrict__ stats, const float* __restrict__ row_loss, long rows,
-                                                            int mean, float* __restrict__ loss) {
-    __shared__ double sums[kT], counts[kT];
-    double s = 0.0, n = 0.0;
-    for (long r = threadIdx.x; r < rows; r += kT)
-        if (stats[r].w != 0.f) s += (double)row_loss[r], n += 1.0;
-    sums[threadIdx.x] = s;
-    counts[threadIdx.x] = n;
+// ---------------------------------------------------------------------------------------------------------------------
+// Selection, rows of adjacent classes.  A workgroup holds one segment of a row in registers (read once): NT threads x NCH
+// chunks of 16 bytes.  The k-th largest of the NT threads' maxima is a lower bound of the k-th largest element, found by
+// one wave bit by bit with ballots; what is not below it goes into a list -- barely more than k elements unless large
+// logits crowd into few threads or tie -- and is ranked by counting.  Everything else is summed for `rest` on the same walk.
+// A list that runs over (long ties, a masked-out segment) sends the segment through k rounds of a plain maximum instead.
+// Rows longer than a segment leave their segments' lists and sums to a merge.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int NT, int NCH>
+__global__ void __launch_bounds__(NT) top_segment_kernel(const T* __restrict__ x, long ld, int C, int nseg, int k, float inv_t,
+                                                         float* __restrict__ values, int* __restrict__ indices, float* __restrict__ rest,
+                                                         long* __restrict__ part_keys, Sum* __restrict__ part_sums) {
+    constexpr int VEC = ElemTraits<T>::VEC;
+    __shared__ long cand[kCand];
+    __shared__ int maxima[NT];
+    __shared__ Sum buf[NT / 64];
+    __shared__ long lbuf[NT / 64];
+    __shared__ int count, bound;
+    const int t = threadIdx.x;
+    const long row = blockIdx.x / nseg;
+    const int seg = (int)(blockIdx.x % nseg), c0 = seg * (NT * NCH * VEC), n = min(C - c0, NT * NCH * VEC), want = min(k, n);
+    const T* p = x + row * ld + c0;
+    const float c = inv_t * kLog2e;
+    long* keys_out = part_keys + (long)blockIdx.x * k;
+
+    uint4 raw[NCH];
+    float f[VEC], top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) raw[j] = load_chunk<T>(p, (j * NT + t) * VEC, n);
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        unpack16<T>(raw[j], f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[e]);
+    }
+    maxima[t] = order_of(top);
+    if (t == 0) count = 0;
+    __syncthreads();
+    if (t < 64) {
+        int m[NT / 64];
+#pragma unroll
+        for (int i = 0; i < NT / 64; ++i) m[i] = maxima[i * 64 + t];
+        // the 20 highest bits: 16-bit types whole, fp32 to 2^-11 of its value; a lower bound is all that is needed
+        int b = kNothing;
+#pragma unroll 1
+        for (int bit = 31; bit >= 12; --bit) {
+            const int raised = bit == 31 ? 0 : b | (1 << bit);
+            int above = 0;
+#pragma unroll
+            for (int i = 0; i < NT / 64; ++i) above += __popcll(__ballot(m[i] >= raised));
+            if (above >= k) b = raised;
+        }
+        if (t == 0) bound = b;
+    }
+    __syncthreads();
+    const int b = bound;
+    // an order below that of -inf (too few maxima, or cut-off bits) leaves nothing out
+    const float lim = b <= (int)0x807fffff ? -INFINITY : value_of(b);
+    const float ref = lim == -INFINITY ? 0.f : lim;
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NCH; ++j) {
+        unknown(raw[j]);
+        unpack16<T>(raw[j], f);
+        float high = f[0];
+#pragma unroll
+        for (int e = 1; e < VEC; ++e) high = fmaxf(high, f[e]);
+        if (high < lim) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += exp2_((f[e] - ref) * c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int at = (j * NT + t) * VEC + e;
+                if (at >= n) continue;
+                if (f[e] < lim) {
+                    s += exp2_((f[e] - ref) * c);
+                } else {
+                    const int slot = atomicAdd(&count, 1);
+                    if (slot < kCand) cand[slot] = key_of(f[e], c0 + at);
+                }
+            }
+        }
+    }
+    const Sum below = block_join<NT>({s == 0.f ? -INFINITY : ref, s}, buf, c);
+    __syncthreads();
+    const int got = count;
+    Sum left = {-INFINITY, 0.f};
+    // The list decides when it holds every candidate.  The sum decides unless a NaN went by in it, or it is so small against its
+    // reference that terms of it may have been flushed
+    if (got <= kCand && (got >= n || below.s >= 1e-30f)) {
+        for (int i = t; i < got; i += NT) {
+            const long key = cand[i];
+            int rank = 0;
+            for (int q = 0; q < got; ++q) rank += cand[q] > key;
+            if (rank >= want) {
+                left = join(left, one(value_of((int)(key >> 32))), c);
+            } else if (nseg == 1) {
+                values[row * k + rank] = value_of((int)(key >> 32));
+                indices[row * k + rank] = index_of(key);
+            } else {
+                keys_out[rank] = key;
+            }
+        }
+        left = join(below, block_join<NT>(left, buf, c), c);
+    } else {
+        long last = 0x7fffffffffffffffL;
+        for (int r = 0; r < want; ++r) {
+            long best = kNoKey;
+            int mine = t;
+            asm volatile("" : "+v"(mine));  // its elements' keys are formed anew in every round
+#pragma unroll
+            for (int j = 0; j < NCH; ++j) {
+                unknown(raw[j]);
+                unpack16<T>(raw[j], f);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int at = (j * NT + mine) * VEC + e;
+                    const long key = key_of(f[e], c0 + at);
+                    if (at < n && key < last && key > best) best = key;
+                }
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) {
+                const long o = __shfl_xor(best, off, 64);
+                best = o > best ? o : best;
+            }
+            if constexpr (NT > 64) {
+                if ((t & 63) == 0) lbuf[t >> 6] = best;
+                __syncthreads();
+                best = lbuf[0];
+                for (int i = 1; i < NT / 64; ++i) best = lbuf[i] > best ? lbuf[i] : best;
+                __syncthreads();
+            }
+            last = best;
+            if (t == 0) {
+                if (nseg == 1) {
+                    values[row * k + r] = value_of((int)(last >> 32));
+                    indices[row * k + r] = index_of(last);
+                } else {
+                    keys_out[r] = last;
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            unknown(raw[j]);
+            unpack16<T>(raw[j], f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int at = (j * NT + t) * VEC + e;
+                if (at < n && key_of(f[e], c0 + at) < last) left = join(left, one(f[e]), c);
+            }
+        }
+        left = block_join<NT>(left, buf, c);
+    }
+    if (t == 0) {
+        if (nseg == 1) rest[row] = log_of(left, inv_t);
+        else part_sums[blockIdx.x] = left;
+    }
+    if (nseg > 1)
+        for (int r = want + t; r < k; r += NT) keys_out[r] = kNoKey;
+}
+
+// One wave per row: the segments' sorted lists are merged by k rounds over their heads; what is left of them joins `rest`.
+__global__ void __launch_bounds__(64) top_merge_kernel(const long* __restrict__ part_keys, const Sum* __restrict__ part_sums, int nseg, int k,
+                                                       float inv_t, float* __restrict__ values, int* __restrict__ indices,
+                                                       float* __restrict__ rest) {
+    extern __shared__ int head[];  // entry i belongs to lane i % 64 alone
+    const int l = threadIdx.x;
+    const long row = blockIdx.x;
+    const long* keys = part_keys + row * nseg * k;
+    const float c = inv_t * kLog2e;
+    long mine = kNoKey;
+    int from = -1;
+    for (int i = l; i < nseg; i += 64) {
+        head[i] = 0;
+        if (keys[(long)i * k] > mine) mine = keys[(long)i * k], from = i;
+    }
+    for (int r = 0; r < k; ++r) {
+        long best = mine;
+        for (int off = 1; off < 64 && off < nseg; off <<= 1) {
+            const long o = __shfl_xor(best, off, 64);
+            best = o > best ? o : best;
+        }
+        best = __shfl(best, 0, 64);
+        if (mine == best && from >= 0) {
+            values[row * k + r] = value_of((int)(best >> 32));
+            indices[row * k + r] = index_of(best);
+            head[from]++;
+            mine = kNoKey;
+            from = -1;
+            for (int i = l; i < nseg; i += 64)
+                if (head[i] < k && keys[(long)i * k + head[i]] > mine) mine = keys[(long)i * k + head[i]], from = i;
+        }
+    }
+    Sum sum = {-INFINITY, 0.f};
+    for (int i = l; i < nseg; i += 64) {
+        sum = join(sum, part_sums[row * nseg + i], c);
+        for (int r = head[i]; r < k; ++r) {
+            const long key = keys[(long)i * k + r];
+            if (key != kNoKey) sum = join(sum, one(value_of((int)(key >> 32))), c);
+        }
+    }
+    sum = wave_join(sum, c);
+    if (l == 0) rest[row] = log_of(sum, inv_t);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Selection, one thread per row: maps (neighbouring threads, neighbouring positions) and rows of a few classes.  The list is
+// kept sorted in registers; every class throws one value out of it (itself, a displaced one or an empty slot), which goes to
+// the running sum for `rest`, so the logits are read once.
+// ---------------------------------------------------------------------------------------------------------------------
+template <typename T, int KM>
+__global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x, long ld, int C, long inner, long rows, int k, float inv_t,
+                                                        float* __restrict__ values, int* __restrict__ indices, float* __restrict__ rest) {
+    const float c = inv_t * kLog2e;
+    const long row = blockIdx.x * (long)kT + threadIdx.x;
+    if (row >= rows) return;
+    const long o = (unsigned)row / (unsigned)inner, i = row - o * inner;  // rows fit 31 bits
+    const T* p = x + o * ld + i;
+    int v[KM], at[KM];
+#pragma unroll
+    for (int s = 0; s < KM; ++s) v[s] = kNothing, at[s] = 0;
+    Sum sum = {-INFINITY, 0.f};
+#pragma unroll 4
+    for (int j = 0; j < C; ++j) {
+        int a = order_of(load_elem<T>(p, j * inner)), ai = j;
+        bool in = false;
+#pragma unroll
+        for (int s = 0; s < KM; ++s)
+            if (s < k) {
+                const int ov = v[s], oi = at[s];
+                in = in || a > ov;
+                v[s] = in ? a : ov;
+                at[s] = in ? ai : oi;
+                a = in ? ov : a;
+                ai = in ? oi : ai;
+            }
+        const float out = value_of(a);
+        if (out != -INFINITY) {
+            const float d = out - sum.m, e = exp2_(-fabsf(d) * c);
+            sum.s = d > 0.f ? fmaf(sum.s, e, 1.f) : sum.s + e;
+            sum.m = fmaxf(sum.m, out);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < KM; ++s)
+        if (s < k) {
+            values[(o * k + s) * inner + i] = value_of(v[s]);
+            indices[(o * k + s) * inner + i] = at[s];
+        }
+    rest[row] = log_of(sum, inv_t);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// The loss.  What the backward keeps of a row, in four floats: the largest logit m and ls = log2 of sum 2^((z_j - m) c) over all
+// classes, and the same (mt, lt) over the unlisted ones.  Two maxima, because the unlisted classes may lie so far below the
+// listed ones that their sum relative to m would vanish.  A sum is at least 1, its logarithm at least 0: ls = -1 marks a row that
+// does not count.
+// ---------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float4 row_stats(Sum unlisted, Sum all) {
+    const float m = all.m == -INFINITY ? 0.f : all.m;
+    return make_float4(m, all.s == 0.f ? 0.f : log2_(all.s), unlisted.m == -INFINITY ? m : unlisted.m,
+                       unlisted.s == 0.f ? 0.f : log2_(unlisted.s));
+}
+__device__ __forceinline__ bool row_counts(const float4& st) { return st.y != -1.f; }
+
+// (sum, count) of the rows that count, one pair per workgroup, joined in a fixed order
+template <int NT>
+__device__ __forceinline__ void leave_part(double s, double n, double* __restrict__ parts) {
+    __shared__ double buf[2][NT / 64];
+    s = wave_sum_d(s);
+    n = wave_sum_d(n);
+    if ((threadIdx.x & 63) == 0) buf[0][threadIdx.x >> 6] = s, buf[1][threadIdx.x >> 6] = n;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < kT; ++i) s += sums[i], n += counts[i];
-        const double f = mean ? 1.0 / (n > 0.0 ? n : 1.0) : 1.0;
+        for (int i = 1; i < NT / 64; ++i) s += buf[0][i], n += buf[1][i];
+        parts[2 * blockIdx.x] = s;
+        parts[2 * blockIdx.x + 1] = n;
+    }
+}
+// loss[0] = sum or mean of the rows that count, loss[1] = the factor of the gradient (1 / their number for the mean)
+__global__ void __launch_bounds__(kT) distill_finish_kernel(const double* __restrict__ parts, int n, int mean, float* __restrict__ loss) {
+    __shared__ double sums[kT / 64], counts[kT / 64];
+    double s = 0.0, m = 0.0;
+    for (int i = threadIdx.x; i < n; i += kT) s += parts[2 * i], m += parts[2 * i + 1];
+    s = wave_sum_d(s);
+    m = wave_sum_d(m);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s, counts[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kT / 64; ++i) s += sums[i], m += counts[i];
+        const double f = mean ? 1.0 / (m > 0.0 ? m : 1.0) : 1.0;
         loss[0] = (float)(s * f);
         loss[1] = (float)f;
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kT) distill_bwd_kernel(const T* __restrict__ z, long ld, int C, long inner, int k,
+// Rows of adjacent classes, a workgroup per row (64 threads for short rows: one wave, no barriers between waves).  Lane i of
+// every wave holds entry i of the teacher's list; the classes it lists are a bit set in LDS, one byte (fp32: half a byte) per
+// 16-byte chunk.  One walk over the row sums the unlisted classes; the listed ones are gathered.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z, long ld, int C, long rows, int k,
+                                                         const float* __restrict__ values, const int* __restrict__ indices,
+                                                         const float* __restrict__ rest, const unsigned char* __restrict__ mask, float temp,
+                                                         float inv_t, float4* __restrict__ stats, float* __restrict__ row_loss,
+                                                         double* __restrict__ parts) {
+    constexpr int VEC = ElemTraits<T>::VEC;
+    constexpr int SEG = NT == 64 ? 4096 : kSeg;
+    constexpr int U = 4;  // chunks in flight per thread
+    __shared__ unsigned bits[SEG / 32];
+    __shared__ Sum buf[NT / 64];
+    const int t = threadIdx.x, lane = t & 63;
+    const float c = inv_t * kLog2e;
+    for (int i = t; i < SEG / 32; i += NT) bits[i] = 0;
+    double lsum = 0.0, lcount = 0.0;
+    for (long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* p = z + row * ld;
+        const int idx = lane < k ? indices[row * k + lane] : -1;
+        const float v = idx >= 0 ? values[row * k + lane] : -INFINITY, r = rest != nullptr ? rest[row] * temp : -INFINITY;
+        const float vtop = wave_max(v != v || r <= v ? v : r);
+        if (vtop == -INFINITY || (mask != nullptr && mask[row] == 0)) {
+            if (t == 0) {
+                stats[row] = make_float4(0.f, -1.f, 0.f, 0.f);
+                if (row_loss != nullptr) row_loss[row] = 0.f;
+            }
+            continue;
+        }
+        Sum sum = {-INFINITY, 0.f};
+        for (int s0 = 0; s0 < C; s0 += SEG) {
+            const int n = min(C - s0, SEG);
+            const bool here = t < 64 && idx >= s0 && idx - s0 < n;
+            __syncthreads();
+            if (here) atomicOr(&bits[(idx - s0) >> 5], 1u << ((idx - s0) & 31));
+            __syncthreads();
+            for (int a = t * VEC; a < n; a += U * NT * VEC) {
+                float f[U][VEC];
+                float top = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int at = a + u * NT * VEC;
+                    unpack16<T>(load_chunk<T>(p + s0, at, n), f[u]);  // past the row: all -inf
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int at = a + u * NT * VEC;
+                    const unsigned w = at < n ? (bits[at >> 5] >> (at & 31)) & ((1u << VEC) - 1u) : 0u;
+                    if (w) {
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) f[u][e] = (w >> e) & 1u ? -INFINITY : f[u][e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[u][e]);
+                }
+                const float m = fmaxf(sum.m, top), ref = m == -INFINITY ? 0.f : m;
+                float s = sum.s * exp2_((sum.m - ref) * c);
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) s += exp2_((f[u][e] - ref) * c);
+                sum = {m, s};
+            }
+            __syncthreads();
+            if (here) bits[(idx - s0) >> 5] = 0;
+        }
+        const Sum unlisted = block_join<NT>(sum, buf, c);
+        if (t < 64) {
+            const bool valid = idx >= 0 && idx < C, bad = __any(idx >= C);
+            const float zi = valid ? load_elem<T>(p, idx) : -INFINITY;
+            bool first = valid;
+            for (int q = 0; q < k; ++q) {
+                const int other = __shfl(idx, q, 64);  // by every lane: a lane that sits out cannot be read either
+                first = first && (q >= lane || other != idx);
+            }
+            const Sum all = join(unlisted, wave_join(first ? one(zi) : Sum{-INFINITY, 0.f}, c), c);
+            float4 st = row_stats(unlisted, all);
+            if (bad) st.x = st.z = NAN;
+            // teacher, in base-2 units relative to its largest entry
+            const float lv = (v - vtop) * c, lr = (r - vtop) * c;
+            const float L = log2_(wave_sum(lane < k ? exp2_(lv) : 0.f) + exp2_(lr));
+            const float pi = lane < k ? exp2_(lv - L) : 0.f, pr = exp2_(lr - L);
+            float term = pi != 0.f ? pi * ((lv - L) - ((zi - st.x) * c - st.y)) : 0.f;
+            if (lane == 0 && pr != 0.f) {
+                const float lq = unlisted.s == 0.f ? -INFINITY : (st.z - st.x) * c + st.w - st.y;
+                term += pr * ((lr - L) - lq);
+            }
+            const float loss = temp * temp * kLn2 * wave_sum(term);
+            if (t == 0) {
+                stats[row] = st;
+                if (row_loss != nullptr) row_loss[row] = bad ? NAN : loss;
+                lsum += (double)(bad ? NAN : loss);
+                lcount += 1.0;
+            }
+        }
+    }
+    if (t == 0) parts[2 * blockIdx.x] = lsum, parts[2 * blockIdx.x + 1] = lcount;
+}
+
+// The unlisted form goes over the whole row; behind a barrier the lanes that hold the list put the listed classes right.
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z, long ld, int C, long rows, int k,
                                                          const float* __restrict__ values, const int* __restrict__ indices,
                                                          const float* __restrict__ rest, float temp, float inv_t,
                                                          const float4* __restrict__ stats, const float* __restrict__ factor,
                                                          const float* __restrict__ g, int g_rows, T* __restrict__ dz) {
-    __shared__ Teacher t;
-    const long row = blockIdx.x, o = row / inner, i = row % inner;
+    constexpr int VEC = ElemTraits<T>::VEC;
+    constexpr int U = 4;
+    const int t = threadIdx.x, lane = t & 63;
+    const float c = inv_t * kLog2e;
+    const long row = blockIdx.x;
+    const T* p = z + row * ld;
+    T* d = dz + row * (long)C;
     const float4 st = stats[row];
-    T* d = dz + o * C * inner + i;
-    if (st.w == 0.f) {
-        for (int c = threadIdx.x; c < C; c += kT) store_elem<T>(d, c * inner, 0.f);
+    if (!row_counts(st)) {
+        float f[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = 0.f;
+        for (int a = t * VEC; a < C; a += NT * VEC) store_chunk<T>(d, a, C, f);
         return;
     }
-    teacher_row(t, values, indices, rest, row, o, i, inner, k, C, inv_t);
-    const T* p = z + o * ld + i;
+    const int idx = lane < k ? indices[row * k + lane] : -1;
+    const float v = idx >= 0 ? values[row * k + lane] : -INFINITY, r = rest != nullptr ? rest[row] * temp : -INFINITY;
+    const float vtop = wave_max(v != v || r <= v ? v : r);
+    const float lv = (v - vtop) * c, lr = (r - vtop) * c;
+    const float L = log2_(wave_sum(lane < k ? exp2_(lv) : 0.f) + exp2_(lr));
+    const float pi = lane < k ? exp2_(lv - L) : 0.f, pr = exp2_(lr - L);
     const float gs = g[g_rows ? row : 0] * (factor != nullptr ? factor[1] : 1.f) * temp;
-    const float outside = (st.w == 2.f ? 0.f : expf(st.z - st.y)) - t.pr;
-    for (int c = threadIdx.x; c < C; c += kT) {
-        const float a = (load_elem<T>(p, c * inner) - st.x) * inv_t;
-        bool listed = false;
-        float sum = 0.f;
-        for (int s = 0; s < k; ++s)
-            if (t.idx[s] == c) listed = true, sum += t.p[s];
-        store_elem<T>(d, c * inner, gs * (listed ? expf(a - st.y) - sum : expf(a - st.z) * outside));
+    const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - pr);
+    for (int a = t * VEC; a < C; a += U * NT * VEC) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = load_chunk<T>(p, a + u * NT * VEC, C);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float f[VEC];
+            unpack16<T>(raw[u], f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) f[e] = outside * exp2_((f[e] - st.z) * c - st.w);
+            store_chunk<T>(d, a + u * NT * VEC, C, f);
+        }
     }
+    __syncthreads();
+    if (t >= 64) return;
+    float share = 0.f;  // of all entries with this lane's class
+    for (int q = 0; q < k; ++q) {
+        const int other = __shfl(idx, q, 64);
+        const float po = __shfl(pi, q, 64);
+        share += other == idx ? po : 0.f;
+    }
+    if (idx >= 0 && idx < C) store_elem<T>(d, idx, gs * (exp2_((load_elem<T>(p, idx) - st.x) * c - st.y) - share));
+}
+
+// One thread per row: maps, and rows of a few classes.  KM > 0: lists of up to KM entries whose indices stay in registers;
+// KM = 0: any length, read again where needed.
+template <int KM>
+struct List {
+    int idx[KM > 0 ? KM : 1];
+    const int* ip;
+    const float* vp;
+    long inner;
+    int k;
+    __device__ __forceinline__ void open(const float* values, const int* indices, long o, long i, long inner_, int k_) {
+        ip = indices + o * k_ * inner_ + i;
+        vp = values + o * k_ * inner_ + i;
+        inner = inner_;
+        k = k_;
+        if constexpr (KM > 0) {
+#pragma unroll
+            for (int s = 0; s < KM; ++s) idx[s] = s < k ? ip[s * inner] : -1;
+        }
+    }
+    __device__ __forceinline__ int index(int s) const {
+        if constexpr (KM > 0) return idx[s];
+        else return ip[s * inner];
+    }
+    __device__ __forceinline__ float value(int s) const { return index(s) >= 0 ? vp[s * inner] : -INFINITY; }
+};
+#define LIST_FOR(S) _Pragma("clang loop unroll_count(KM > 0 ? KM : 1)") for (int S = 0; S < (KM > 0 ? KM : list.k); ++S) if (KM == 0 || S < list.k)
+
+template <typename T, int KM>
+__global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restrict__ z, long ld, int C, long inner, long rows, int k,
+                                                                const float* __restrict__ values, const int* __restrict__ indices,
+                                                                const float* __restrict__ rest, const unsigned char* __restrict__ mask,
+                                                                float temp, float inv_t, float4* __restrict__ stats,
+                                                                float* __restrict__ row_loss, double* __restrict__ parts) {
+    constexpr int U = 8;
+    const float c = inv_t * kLog2e;
+    double lsum = 0.0, lcount = 0.0;
+    for (long row = blockIdx.x * (long)kT + threadIdx.x; row < rows; row += (long)gridDim.x * kT) {
+        const long o = (unsigned)row / (unsigned)inner, i = row - o * inner;  // rows fit 31 bits
+        const T* p = z + o * ld + i;
+        List<KM> list;
+        list.open(values, indices, o, i, inner, k);
+        const float r = rest != nullptr ? rest[row] * temp : -INFINITY;
+        float vtop = r;
+        bool bad = false;
+        LIST_FOR(s) {
+            const float v = list.value(s);
+            vtop = vtop != vtop || v <= vtop ? vtop : v;
+            bad |= list.index(s) >= C;
+        }
+        if (vtop == -INFINITY || (mask != nullptr && mask[row] == 0)) {
+            stats[row] = make_float4(0.f, -1.f, 0.f, 0.f);
+            if (row_loss != nullptr) row_loss[row] = 0.f;
+            continue;
+        }
+        Sum un = {-INFINITY, 0.f}, in = {-INFINITY, 0.f};
+        for (int c0 = 0; c0 < C; c0 += U) {
+            float f[U];
+            unsigned w = 0;
+#pragma unroll
+            for (int e = 0; e < U; ++e) f[e] = c0 + e < C ? load_elem<T>(p, (c0 + e) * inner) : -INFINITY;
+            LIST_FOR(s) {
+                const unsigned at = (unsigned)(list.index(s) - c0);
+                w |= at < U ? 1u << at : 0u;
+            }
+            float mu = un.m, mi = in.m;
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                const bool listed = (w >> e) & 1u;
+                mu = fmaxf(mu, listed ? -INFINITY : f[e]);
+                mi = fmaxf(mi, listed ? f[e] : -INFINITY);
+            }
+            const float ru = mu == -INFINITY ? 0.f : mu, ri = mi == -INFINITY ? 0.f : mi;
+            float su = un.s * exp2_((un.m - ru) * c), si = in.s * exp2_((in.m - ri) * c);
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                const bool listed = (w >> e) & 1u;
+                const float x = exp2_((f[e] - (listed ? ri : ru)) * c);
+                su += listed ? 0.f : x;
+                si += listed ? x : 0.f;
+            }
+            un = {mu, su};
+            in = {mi, si};
+        }
+        float4 st = row_stats(un, join(un, in, c));
+        if (bad) st.x = st.z = NAN;
+        const float lr = (r - vtop) * c;
+        float total = exp2_(lr);
+        LIST_FOR(s) total += exp2_((list.value(s) - vtop) * c);
+        const float L = log2_(total), pr = exp2_(lr - L);
+        float loss = 0.f;
+        if (pr != 0.f) loss = pr * ((lr - L) - (un.s == 0.f ? -INFINITY : (st.z - st.x) * c + st.w - st.y));
+        LIST_FOR(s) {
+            const float lp = (list.value(s) - vtop) * c - L, pi = exp2_(lp);
+            const int at = list.index(s);
+            if (pi != 0.f && at >= 0 && at < C) loss += pi * (lp - ((load_elem<T>(p, at * inner) - st.x) * c - st.y));
+        }
+        loss = bad ? NAN : temp * temp * kLn2 * loss;
+        stats[row] = st;
+        if (row_loss != nullptr) row_loss[row] = loss;
+        lsum += (double)loss;
+        lcount += 1.0;
+    }
+    leave_part<kT>(lsum, lcount, parts);
+}
+
+template <typename T, int KM>
+__global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restrict__ z, long ld, int C, long inner, long rows, int k,
+                                                                const float* __restrict__ values, const int* __restrict__ indices,
+                                                                const float* __restrict__ rest, float temp, float inv_t,
+                                                                const float4* __restrict__ stats, const float* __restrict__ factor,
+                                                                const float* __restrict__ g, int g_rows, T* __restrict__ dz) {
+    constexpr int U = 8;
+    const float c = inv_t * kLog2e;
+    const long row = blockIdx.x * (long)kT + threadIdx.x;
+    if (row >= rows) return;
+    const long o = (unsigned)row / (unsigned)inner, i = row - o * inner;  // rows fit 31 bits
+    const T* p = z + o * ld + i;
+    T* d = dz + o * C * inner + i;
+    const float4 st = stats[row];
+    if (!row_counts(st)) {
+        for (int j = 0; j < C; ++j) store_elem<T>(d, j * inner, 0.f);
+        return;
+    }
+    List<KM> list;
+    list.open(values, indices, o, i, inner, k);
+    const float r = rest != nullptr ? rest[row] * temp : -INFINITY;
+    float vtop = r;
+    LIST_FOR(s) {
+        const float v = list.value(s);
+        vtop = vtop != vtop || v <= vtop ? vtop : v;
+    }
+    const float lr = (r - vtop) * c;
+    float total = exp2_(lr);
+    LIST_FOR(s) total += exp2_((list.value(s) - vtop) * c);
+    const float L = log2_(total);
+    const float gs = g[g_rows ? row : 0] * (factor != nullptr ? factor[1] : 1.f) * temp;
+    const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - exp2_(lr - L));
+    for (int c0 = 0; c0 < C; c0 += U) {
+        float f[U];
+#pragma unroll
+        for (int e = 0; e < U; ++e) f[e] = c0 + e < C ? load_elem<T>(p, (c0 + e) * inner) : 0.f;
+#pragma unroll
+        for (int e = 0; e < U; ++e)
+            if (c0 + e < C) store_elem<T>(d, (c0 + e) * inner, outside * exp2_((f[e] - st.z) * c - st.w));
+    }
+    LIST_FOR(s) {  // the same thread: these stores come after the ones above
+        const int at = list.index(s);
+        if (at >= 0 && at < C) {
+            const int self = at;
+            float share = 0.f;
+            LIST_FOR(q) share += list.index(q) == self ? exp2_((list.value(q) - vtop) * c - L) : 0.f;
+            store_elem<T>(d, at * inner, gs * (exp2_((load_elem<T>(p, at * inner) - st.x) * c - st.y) - share));
+        }
+    }
+}
+
+// rows that one thread takes: maps (their classes are not adjacent), and rows so short that a wave would idle
+bool by_thread(int classes, long inner) { return inner > 1 || classes <= 32; }
+
+bool layout_ok(long outer, int classes, long inner, long ld) {
+    return outer >= 0 && classes > 0 && inner > 0 && (outer <= 1 || ld >= classes * inner) && (inner == 1 || ld == classes * inner) &&
+           (outer == 0 || inner <= 0x7fffffffL / outer);
+}
+
+// a row's segments: 64 threads x 4 chunks where a row fits, else 256 threads x 8 chunks
+int segments(int dtype, int classes) {
+    const int vec = msfwsi_vec_of(dtype);
+    return classes <= 64 * 4 * vec ? 1 : (classes + 256 * 8 * vec - 1) / (256 * 8 * vec);
 }
 
 }  // namespace
 
 #define ST(s) reinterpret_cast<hipStream_t>(s)
 
-static bool layout_ok(long outer, int classes, long inner, long ld) {
-    return outer >= 0 && classes > 0 && inner > 0 && (outer <= 1 || ld >= classes * inner) && (inner == 1 || ld == classes * inner) &&
-           (outer == 0 || inner <= 0xffffffL / outer);  // a grid holds fewer than 2^32 threads
+extern "C" int msfwsi_top_logits_workspace(int dtype, long outer, int classes, long inner, int k, long* bytes) {
+    MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && bytes && outer >= 0 && classes > 0 && inner > 0 && k > 0 && k <= kMaxK);
+    const int nseg = segments(dtype, classes);
+    *bytes = by_thread(classes, inner) || nseg == 1 ? 0 : outer * nseg * (k + 1L) * 8;
+    return MSFWSI_OK;
 }
 
 extern "C" int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, int classes, long inner, int k, float inv_t, float* values,
-                                 int* indices, float* rest, void* stream) {
+                                 int* indices, float* rest, void* workspace, void* stream) {
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && layout_ok(outer, classes, inner, ld) && k > 0 && k <= kMaxK && k <= classes && inv_t > 0.f);
     if (outer == 0) return MSFWSI_OK;
     MSFWSI_CHECK_ARG(x && values && indices && rest);
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(top_logits_kernel<T>, dim3((unsigned)(outer * inner)), dim3(kT), 0, ST(stream), (const T*)x, ld,
-                                            classes, inner, k, inv_t, values, indices, rest));
+    if (by_thread(classes, inner)) {
+        const long rows = outer * inner, blocks = (rows + kT - 1) / kT;
+#define TOP_THREAD(KM)                                                                                                        \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((top_thread_kernel<T, KM>), dim3((unsigned)blocks), dim3(kT), 0, ST(stream),     \
+                                            (const T*)x, ld, classes, inner, rows, k, inv_t, values, indices, rest))
+        if (k <= 4) TOP_THREAD(4);
+        else if (k <= 16) TOP_THREAD(16);
+        else TOP_THREAD(64);
+        return msfwsi_launch_status();
+    }
+    const int nseg = segments(dtype, classes);
+    if (nseg > 4096 || outer > 0xffffffL / nseg) return MSFWSI_EUNSUPPORTED;  // heads of a merge in LDS; a grid holds < 2^32 threads
+    MSFWSI_CHECK_ARG(nseg == 1 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0));
+    long* keys = (long*)workspace;
+    Sum* sums = (Sum*)(keys + outer * nseg * (long)k);
+#define TOP_ROWS(NT, NCH)                                                                                                            \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((top_segment_kernel<T, NT, NCH>), dim3((unsigned)(outer * nseg)), dim3(NT), 0, ST(stream), \
+                                            (const T*)x, ld, classes, nseg, k, inv_t, values, indices, rest, keys, sums))
+    if (classes <= 64 * 4 * msfwsi_vec_of(dtype)) TOP_ROWS(64, 4);
+    else TOP_ROWS(256, 8);
+    const int rc = msfwsi_launch_status();
+    if (rc != MSFWSI_OK || nseg == 1) return rc;
+    hipLaunchKernelGGL(top_merge_kernel, dim3((unsigned)outer), dim3(64), nseg * sizeof(int), ST(stream), keys, sums, nseg, k, inv_t, values,
+                       indices, rest);
     return msfwsi_launch_status();
 }
+
+// how many threads take a row of adjacent classes: a wave up to 2048 classes; a large workgroup where rows are too few to fill
+// the machine with small ones
+static int row_threads(long rows, int classes) { return classes <= 2048 ? 64 : rows < 512 && classes >= 16384 ? 1024 : 256; }
 
 extern "C" int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer, int classes, long inner, int k, const float* values,
                                   const int* indices, const float* rest, const unsigned char* mask, float temperature, int mean, float* stats,
                                   float* row_loss, float* loss, double* partials, void* stream) {
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && layout_ok(outer, classes, inner, ld) && k > 0 && k <= kMaxK && temperature > 0.f);
     MSFWSI_CHECK_ARG(loss && partials);
+    long blocks = 0;
     if (outer > 0) {
-        MSFWSI_CHECK_ARG(z && values && indices && stats && row_loss);
-        MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(distill_fwd_kernel<T>, dim3((unsigned)(outer * inner)), dim3(kT), 0, ST(stream), (const T*)z, ld,
-                                                classes, inner, k, values, indices, rest, mask, temperature, 1.f / temperature, (float4*)stats,
-                                                row_loss));
+        MSFWSI_CHECK_ARG(z && values && indices && stats && (reinterpret_cast<uintptr_t>(stats) & 15) == 0);
+        const long rows = outer * inner, units = by_thread(classes, inner) ? (rows + kT - 1) / kT : rows;
+        const long each = (units + kMaxParts - 1) / kMaxParts;
+        blocks = (units + each - 1) / each;
+        const float inv_t = 1.f / temperature;
+        if (by_thread(classes, inner)) {
+#define FWD_THREAD(KM)                                                                                                                   \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((distill_thread_fwd_kernel<T, KM>), dim3((unsigned)blocks), dim3(kT), 0, ST(stream),        \
+                                            (const T*)z, ld, classes, inner, rows, k, values, indices, rest, mask, temperature, inv_t, \
+                                            (float4*)stats, row_loss, partials))
+            if (k <= 4) FWD_THREAD(4);
+            else if (k <= 16) FWD_THREAD(16);
+            else FWD_THREAD(0);
+        } else {
+#define FWD_ROWS(NT)                                                                                                                 \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((distill_fwd_kernel<T, NT>), dim3((unsigned)blocks), dim3(NT), 0, ST(stream),           \
+                                            (const T*)z, ld, classes, rows, k, values, indices, rest, mask, temperature, inv_t,     \
+                                            (float4*)stats, row_loss, partials))
+            const int nt = row_threads(rows, classes);
+            if (nt == 64) FWD_ROWS(64);
+            else if (nt == 256) FWD_ROWS(256);
+            else FWD_ROWS(1024);
+        }
         const int rc = msfwsi_launch_status();
         if (rc != MSFWSI_OK) return rc;
     }
-    hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), dim3(kT), 0, ST(stream), (const float4*)stats, row_loss, outer * inner, mean, loss);
+    hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(kT), 0, ST(stream), partials, (int)blocks, mean, loss);
     return msfwsi_launch_status();
 }
 
@@ -260,9 +833,27 @@ extern "C" int msfwsi_distill_bwd(int dtype, const void* z, long ld, long outer,
                                   const float* g, int g_rows, void* dz, void* stream) {
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && layout_ok(outer, classes, inner, ld) && k > 0 && k <= kMaxK && temperature > 0.f);
     if (outer == 0) return MSFWSI_OK;
-    MSFWSI_CHECK_ARG(z && values && indices && stats && g && dz);
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(distill_bwd_kernel<T>, dim3((unsigned)(outer * inner)), dim3(kT), 0, ST(stream), (const T*)z, ld,
-                                            classes, inner, k, values, indices, rest, temperature, 1.f / temperature, (const float4*)stats,
-                                            factor, g, g_rows, (T*)dz));
+    MSFWSI_CHECK_ARG(z && values && indices && stats && (reinterpret_cast<uintptr_t>(stats) & 15) == 0 && g && dz);
+    const long rows = outer * inner;
+    const float inv_t = 1.f / temperature;
+    if (by_thread(classes, inner)) {
+#define BWD_THREAD(KM)                                                                                                                      \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((distill_thread_bwd_kernel<T, KM>), dim3((unsigned)((rows + kT - 1) / kT)), dim3(kT), 0,       \
+                                            ST(stream), (const T*)z, ld, classes, inner, rows, k, values, indices, rest, temperature,     \
+                                            inv_t, (const float4*)stats, factor, g, g_rows, (T*)dz))
+        if (k <= 4) BWD_THREAD(4);
+        else if (k <= 16) BWD_THREAD(16);
+        else BWD_THREAD(0);
+        return msfwsi_launch_status();
+    }
+    const int nt = row_threads(rows, classes);
+    if (rows > 0xffffffffL / nt) return MSFWSI_EUNSUPPORTED;  // a grid holds fewer than 2^32 threads
+#define BWD_ROWS(NT)                                                                                                                      \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((distill_bwd_kernel<T, NT>), dim3((unsigned)rows), dim3(NT), 0, ST(stream), (const T*)z, ld, \
+                                            classes, rows, k, values, indices, rest, temperature, inv_t, (const float4*)stats, factor,   \
+                                            g, g_rows, (T*)dz))
+    if (nt == 64) BWD_ROWS(64);
+    else if (nt == 256) BWD_ROWS(256);
+    else BWD_ROWS(1024);
     return msfwsi_launch_status();
 }

@@ -1807,13 +1807,16 @@ def top_logits(x, k: int, temperature: float, values, indices, rest):
     outer, Cn, inner, ld = _logit_layout(x, "x")
     _top_args(values, indices, rest, outer, inner, k)
     _one_device(x, values, indices, rest)
+    need = C.c_long()
+    _lib.check(lib.msfwsi_top_logits_workspace(dt_of(x), outer, Cn, inner, int(k), C.byref(need)), "top_logits_workspace")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
     with torch.cuda.device(x.device):
         _lib.check(lib.msfwsi_top_logits(dt_of(x), _p(x), ld, outer, Cn, inner, int(k), 1.0 / temperature, _p(values), _p(indices), _p(rest),
-                                         _stream()), "top_logits")
+                                         _p(ws), _stream()), "top_logits")
 
 
-def distill_fwd(z, values, indices, rest, mask, k: int, temperature: float, mean: bool):
-    """(row_loss [rows], loss fp32[2] = (sum or mean, gradient factor), stats [rows, 4] for distill_bwd)"""
+def distill_fwd(z, values, indices, rest, mask, k: int, temperature: float, mean: bool, per_row: bool = True):
+    """(row_loss [rows] or None, loss fp32[2] = (sum or mean, gradient factor), stats [rows, 4] for distill_bwd)"""
     lib = _lib.load()
     outer, Cn, inner, ld = _logit_layout(z, "z")
     _top_args(values, indices, rest, outer, inner, k)
@@ -1822,7 +1825,7 @@ def distill_fwd(z, values, indices, rest, mask, k: int, temperature: float, mean
         _dense(mask, "mask", torch.bool, rows)
     _one_device(z, values, indices, rest, mask)
     stats = torch.empty(rows, 4, dtype=torch.float32, device=z.device)
-    row_loss = torch.empty(rows, dtype=torch.float32, device=z.device)
+    row_loss = torch.empty(rows, dtype=torch.float32, device=z.device) if per_row else None
     loss = torch.empty(2, dtype=torch.float32, device=z.device)
     partials = torch.empty(2, 2048, dtype=torch.float64, device=z.device)
     with torch.cuda.device(z.device):

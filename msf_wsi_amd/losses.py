@@ -134,7 +134,7 @@ class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, dim, values, indices, rest, mask, k, temperature, reduction):
         view, _ = _logit_view(logits, dim, "TopLogitDistillLoss")
-        row_loss, loss, stats = kn.distill_fwd(view, values, indices, rest, mask, k, temperature, reduction == "mean")
+        row_loss, loss, stats = kn.distill_fwd(view, values, indices, rest, mask, k, temperature, reduction == "mean", reduction == "none")
         ctx.save_for_backward(view, values, indices, rest, stats, loss)
         ctx.meta = (logits.shape, dim, k, temperature, reduction)
         if reduction == "none":
