@@ -533,13 +533,17 @@ int msfwsi_inverse_perm(const long* perm, long* inv, long rows, int K, void* str
  *   msfwsi_mx4_dequantize: y [rows][cols] in `dtype`
  *   msfwsi_mx4_gemm:       y[m][n] = sum_k a[m][k] b[n][k] (+ bias[n], fp32), both operands quantised, fp32 sums, y [M][N]
  *   msfwsi_mx4_dgrad:      dx[m][k] = sum_n dy[m][n] w[n][k], w [N][cols] quantised; dy rows `ld` elements apart, dx [M][cols];
- *                          the products are exact whatever dy's type */
+ *                          the products are exact whatever dy's type.  N <= 2^21
+ *   msfwsi_mx4_*_workspace:  host calls; *bytes = what the launch with the same arguments needs at `workspace` (16-byte
+ *                          aligned; NULL when it is 0) */
 int msfwsi_mx4_quantize(int dtype, const void* x, long ld, long rows, long cols, void* codes, void* scales, void* stream);
 int msfwsi_mx4_dequantize(int dtype, const void* codes, const void* scales, long rows, long cols, void* y, void* stream);
+int msfwsi_mx4_gemm_workspace(long M, long N, long cols, long* bytes);
 int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_scales, long M, const void* b_codes, const void* b_scales,
-                    long N, long cols, const float* bias, void* y, void* stream);
+                    long N, long cols, const float* bias, void* y, void* workspace, void* stream);
+int msfwsi_mx4_dgrad_workspace(int dy_dtype, const void* dy, long ld, long M, long N, long cols, long* bytes);
 int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, const void* codes, const void* scales, long N, long cols,
-                     int dx_dtype, void* dx, void* stream);
+                     int dx_dtype, void* dx, void* workspace, void* stream);
 
 /* ---- distillation from a teacher's largest logits (csrc/distill.hip: the formulas) ------------------------------------
  * Logits [outer][classes][inner]: inner = 1 with rows `ld` elements apart, or contiguous maps (ld = classes * inner).  values /

@@ -113,8 +113,10 @@ SIGNATURES = {
     "msfwsi_panel_dgrad": [_desc, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _f, _vp, _vp, _i, _vp],
     "msfwsi_mx4_quantize": [_i, _vp, _l, _l, _l, _vp, _vp, _vp],
     "msfwsi_mx4_dequantize": [_i, _vp, _vp, _l, _l, _vp, _vp],
-    "msfwsi_mx4_gemm": [_i, _vp, _vp, _l, _vp, _vp, _l, _l, _vp, _vp, _vp],
-    "msfwsi_mx4_dgrad": [_i, _vp, _l, _l, _vp, _vp, _l, _l, _i, _vp, _vp],
+    "msfwsi_mx4_gemm_workspace": [_l, _l, _l, _vp],
+    "msfwsi_mx4_gemm": [_i, _vp, _vp, _l, _vp, _vp, _l, _l, _vp, _vp, _vp, _vp],
+    "msfwsi_mx4_dgrad_workspace": [_i, _vp, _l, _l, _l, _l, _vp],
+    "msfwsi_mx4_dgrad": [_i, _vp, _l, _l, _vp, _vp, _l, _l, _i, _vp, _vp, _vp],
     "msfwsi_top_logits_workspace": [_i, _l, _i, _l, _i, _vp],
     "msfwsi_top_logits": [_i, _vp, _l, _l, _i, _l, _i, _f, _vp, _vp, _vp, _vp, _vp],
     "msfwsi_distill_fwd": [_i, _vp, _l, _l, _i, _l, _i, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _vp, _vp, _vp],

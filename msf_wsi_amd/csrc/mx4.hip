@@ -13,6 +13,8 @@
 #include "common.h"
 #include "../../include/msfwsi_hip.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kGroup = 256;             // elements of a row that are stored together
@@ -84,19 +86,27 @@ __global__ void __launch_bounds__(kT) mx4_dequantize_kernel(const unsigned* __re
         if (c + e < cols) store_elem<T>(y, r * cols + c + e, code_value(w >> (4 * e)) * s);
 }
 
-// y = a b^T (+ bias): 32 x 32 outputs per workgroup, the groups dealt over its four waves and joined in LDS.
-// A 32x32x64 step takes 32 elements of row (lane & 31) from each lane; which 32 is free as long as both operands agree, so
-// half h of the wave takes block 4h + s in step s: its four scales are then one aligned dword and step s reads byte s of it.
-template <typename T>
-__global__ void __launch_bounds__(kT) mx4_gemm_kernel(const unsigned char* __restrict__ a, const unsigned char* __restrict__ as, long M,
-                                                      const unsigned char* __restrict__ b, const unsigned char* __restrict__ bs, long N,
-                                                      int G, const float* __restrict__ bias, T* __restrict__ y, unsigned nt) {
-    __shared__ float part[4][32 * 33];
+// One 32x32x64 step takes 32 elements of row (lane & 31) of either operand from each lane.  Which 32 is free as long as both
+// operands agree: half h of the wave takes block 4h + S of a group in step S, so its four scales are one aligned dword, of which
+// step S reads byte S.
+template <int S>
+__device__ __forceinline__ void mx4_step(f32x16& acc, const int4& a, int sa, const int4& b, int sb) {
+    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4((i32x8){a.x, a.y, a.z, a.w, 0, 0, 0, 0}, (i32x8){b.x, b.y, b.z, b.w, 0, 0, 0, 0},
+                                                          acc, 4, 4, S, sa, S, sb);
+}
+
+// Few rows: 32 x 32 outputs per workgroup straight from memory, the groups dealt over its NW waves and joined in LDS.  Bound
+// by reading b once; nothing is shared between workgroups, so nothing is staged.
+template <typename T, int NW>
+__global__ void __launch_bounds__(NW * 64) mx4_gemm_kernel(const unsigned char* __restrict__ a, const unsigned char* __restrict__ as, long M,
+                                                           const unsigned char* __restrict__ b, const unsigned char* __restrict__ bs, long N,
+                                                           int G, const float* __restrict__ bias, T* __restrict__ y, unsigned nt) {
+    __shared__ float part[NW][32 * 33];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
     const long m0 = (long)(blockIdx.x / nt) * 32, n0 = (long)(blockIdx.x % nt) * 32;
     const long m = min(m0 + (lane & 31), M - 1), n = min(n0 + (lane & 31), N - 1);
     f32x16 acc = {0.f};
-    for (int g = w; g < G; g += 4) {
+    for (int g = w; g < G; g += NW) {
         const long ra = g * M + m, rb = g * N + n;
         const int sa = *reinterpret_cast<const int*>(as + ra * 8 + h * 4), sb = *reinterpret_cast<const int*>(bs + rb * 8 + h * 4);
         int4 fa[4], fb[4];
@@ -105,75 +115,440 @@ __global__ void __launch_bounds__(kT) mx4_gemm_kernel(const unsigned char* __res
             fa[s] = *reinterpret_cast<const int4*>(a + ra * kGroupBytes + (4 * h + s) * 16);
             fb[s] = *reinterpret_cast<const int4*>(b + rb * kGroupBytes + (4 * h + s) * 16);
         }
-#define MX4_STEP(S)                                                                                                          \
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4((i32x8){fa[S].x, fa[S].y, fa[S].z, fa[S].w, 0, 0, 0, 0},           \
-                                                          (i32x8){fb[S].x, fb[S].y, fb[S].z, fb[S].w, 0, 0, 0, 0}, acc, 4, 4, \
-                                                          S, sa, S, sb)
-        MX4_STEP(0);
-        MX4_STEP(1);
-        MX4_STEP(2);
-        MX4_STEP(3);
+        mx4_step<0>(acc, fa[0], sa, fb[0], sb);
+        mx4_step<1>(acc, fa[1], sa, fb[1], sb);
+        mx4_step<2>(acc, fa[2], sa, fb[2], sb);
+        mx4_step<3>(acc, fa[3], sa, fb[3], sb);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) part[w][((i & 3) + 8 * (i >> 2) + 4 * h) * 33 + (lane & 31)] = acc[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < 1024; i += kT) {
+    for (int i = threadIdx.x; i < 1024; i += NW * 64) {
         const int r = i >> 5, c = i & 31;
         if (m0 + r >= M || n0 + c >= N) continue;
-        float v = (part[0][r * 33 + c] + part[1][r * 33 + c]) + (part[2][r * 33 + c] + part[3][r * 33 + c]);
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < NW; ++q) v += part[q][r * 33 + c];
         if (bias != nullptr) v += bias[n0 + c];
         store_elem<T>(y, (m0 + r) * N + n0 + c, v);
     }
 }
 
-// dx = dy W: 32 rows x 32 columns (one scale block) per workgroup, the rows of W dealt over its four waves.  W widens to
-// bf16 exactly (two mantissa bits); dy in fp16 / fp32 is cut into 2 / 3 bf16 parts that add up to it exactly, so every
-// product is exact and the sums are fp32.
-template <typename T, typename TO>
-__global__ void __launch_bounds__(kT) mx4_dgrad_kernel(const T* __restrict__ dy, long ld, long M, const unsigned char* __restrict__ codes,
-                                                       const unsigned char* __restrict__ scales, long N, long cols, TO* __restrict__ dx,
-                                                       unsigned kt) {
-    constexpr int PARTS = sizeof(T) == 4 ? 3 : __is_same(T, _Float16) ? 2 : 1;
-    __shared__ float part[4][32 * 33];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5, l = lane & 31;
-    const long m0 = (long)(blockIdx.x / kt) * 32, k0 = (long)(blockIdx.x % kt) * 32;
-    const long m = min(m0 + l, M - 1), g = k0 / kGroup;
-    const int kb = (int)(k0 % kGroup) / 32;
-    f32x16 acc = {0.f};
-    for (long n0 = w * 16; n0 < N; n0 += 64) {
-        bf16x8 fa[PARTS], fb;
-        float v[8];
-        load8<T>(dy + m * ld + n0 + h * 8, N - n0 - h * 8, v);
+// 4 bytes per lane global -> LDS, the small form of lds_dma16_buf (common.h: the rules for its waits hold here too)
+__device__ __forceinline__ void lds_dma4_buf(__amdgpu_buffer_rsrc_t rsrc, void* lds_wave_base, int voff) {
+    const unsigned lds = (unsigned)(__UINTPTR_TYPE__)(__attribute__((address_space(3))) char*)lds_wave_base;
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(lds), "v"(voff), "s"(rsrc)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const unsigned char* p, long bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p), 0, (int)bytes, 0x00020000);
+}
+// everything this wave has asked for has arrived, and it is done reading the stage it leaves; then all waves
+__device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Tiles go to the XCDs in contiguous runs (xcd_remap), inside a run in columns of 8 row tiles: a run then shares few row and
+// column tiles in its L2.
+__device__ __forceinline__ void tile_of(unsigned id, unsigned mt, unsigned nt, unsigned& m, unsigned& n) {
+    const unsigned wide = 8 * nt, first = id / wide * 8, deep = min(mt - first, 8u), in = id % wide;
+    m = first + in % deep;
+    n = in / deep;
+}
+
+// Many rows: TM x TN outputs per workgroup of WM x WN waves, one group of 256 elements (128 bytes of every row) per step, two
+// stages in LDS filled by DMA.  A row's eight 16-byte chunks lie at (chunk ^ (row & 7)): the eight rows that a read
+// touches at a time then fall on eight different bank groups.  `split` > 0 deals the groups over gridDim.y workgroups that
+// leave fp32 sums for a join.
+template <typename T, int TM, int TN, int WM, int WN>
+__global__ void __launch_bounds__(WM* WN * 64) mx4_tile_kernel(const unsigned char* __restrict__ a, const unsigned char* __restrict__ as, long M,
+                                                               const unsigned char* __restrict__ b, const unsigned char* __restrict__ bs,
+                                                               long N, int G, int per_split, const float* __restrict__ bias,
+                                                               T* __restrict__ y, float* __restrict__ sums, unsigned mt, unsigned nt) {
+    constexpr int NW = WM * WN, FM = TM / WM / 32, FN = TN / WN / 32;
+    constexpr int kStage = (TM + TN) * (kGroupBytes + 8);
+    __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, l = lane & 31;
+    unsigned tm, tn;
+    tile_of(xcd_remap(blockIdx.x, gridDim.x), mt, nt, tm, tn);
+    const long m0 = (long)tm * TM, n0 = (long)tn * TN;
+    const long mrows = min((long)TM, M - m0), nrows = min((long)TN, N - n0);
+    const int g0 = blockIdx.y * per_split, g1 = min(G, g0 + per_split);
+    const int chunk = (lane >> 3) * kGroupBytes + (((lane & 7) ^ (lane >> 3)) << 4);
+
+    auto fill = [&](int g, char* st) {
+        const __amdgpu_buffer_rsrc_t ra = buffer_of(a + (g * M + m0) * kGroupBytes, mrows * kGroupBytes);
+        const __amdgpu_buffer_rsrc_t rb = buffer_of(b + (g * N + n0) * kGroupBytes, nrows * kGroupBytes);
+        const __amdgpu_buffer_rsrc_t rsa = buffer_of(as + (g * M + m0) * 8, mrows * 8), rsb = buffer_of(bs + (g * N + n0) * 8, nrows * 8);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float left = v[e];
+        for (int i = 0; i < TM / 8 / NW; ++i) lds_dma16_buf(ra, st + (i * NW + w) * 1024, (i * NW + w) * 1024 + chunk, 0);
+#pragma unroll
+        for (int i = 0; i < TN / 8 / NW; ++i) lds_dma16_buf(rb, st + TM * kGroupBytes + (i * NW + w) * 1024, (i * NW + w) * 1024 + chunk, 0);
+        char* sc = st + (TM + TN) * kGroupBytes;
+#pragma unroll
+        for (int i = 0; i < TM / 32 / NW; ++i) lds_dma4_buf(rsa, sc + (i * NW + w) * 256, (i * NW + w) * 256 + lane * 4);
+#pragma unroll
+        for (int i = 0; i < TN / 32 / NW; ++i) lds_dma4_buf(rsb, sc + TM * 8 + (i * NW + w) * 256, (i * NW + w) * 256 + lane * 4);
+    };
+    f32x16 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    const int wm = w / WN, wn = w % WN;
+    const int arow = wm * (TM / WM) + l, brow = wn * (TN / WN) + l;
+    auto compute = [&](const char* st) {
+        const char* pa = st + arow * kGroupBytes;
+        const char* pb = st + (TM + brow) * kGroupBytes;
+        const char* sc = st + (TM + TN) * kGroupBytes + h * 4;
+        int sa[FM], sb[FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) sa[i] = *reinterpret_cast<const int*>(sc + (arow + i * 32) * 8);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) sb[j] = *reinterpret_cast<const int*>(sc + (TM + brow + j * 32) * 8);
+        auto step = [&](auto sc_) {
+            constexpr int S = decltype(sc_)::value;
+            const int at = ((4 * h + S) ^ (l & 7)) << 4;
+            int4 fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const int4*>(pa + i * 32 * kGroupBytes + at);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const int4*>(pb + j * 32 * kGroupBytes + at);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) mx4_step<S>(acc[i][j], fa[i], sa[i], fb[j], sb[j]);
+        };
+        step(std::integral_constant<int, 0>());
+        step(std::integral_constant<int, 1>());
+        step(std::integral_constant<int, 2>());
+        step(std::integral_constant<int, 3>());
+    };
+
+    fill(g0, smem);
+    for (int g = g0; g < g1; ++g) {
+        char* cur = smem + ((g - g0) & 1) * kStage;
+        stage_barrier();
+        if (g + 1 < g1) fill(g + 1, smem + ((g - g0 + 1) & 1) * kStage);
+        compute(cur);
+    }
+    float* part = sums + (long)blockIdx.y * M * N;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const long n = n0 + brow + j * 32;
+        if (n >= N) continue;
+        const float add = sums == nullptr && bias != nullptr ? bias[n] : 0.f;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const long m = m0 + wm * (TM / WM) + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
+                if (m >= M) continue;
+                if (sums != nullptr) part[m * N + n] = acc[i][j][e];
+                else store_elem<T>(y, m * N + n, acc[i][j][e] + add);
+            }
+    }
+}
+
+// y = the sum of `splits` fp32 partial results (+ bias of the column)
+template <typename T>
+__global__ void __launch_bounds__(kT) mx4_join_kernel(const float* __restrict__ sums, int splits, long total, long N, const float* __restrict__ bias,
+                                                      T* __restrict__ y) {
+    for (long i = blockIdx.x * (long)kT + threadIdx.x; i < total; i += (long)gridDim.x * kT) {
+        float v = 0.f;
+        for (int s = 0; s < splits; ++s) v += sums[s * total + i];
+        if (bias != nullptr) v += bias[i % N];
+        store_elem<T>(y, i, v);
+    }
+}
+
+// dy in the form the gradient's tiles take: `parts` matrices [M][pitch] of 16-bit values, zeros behind the last column.  fp32 is
+// cut into three bf16 parts that add up to it exactly (each takes the next 8 bits); 16-bit types are copied.
+template <typename T, int PARTS>
+__global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy, long ld, long M, long N, long pitch, unsigned short* __restrict__ out) {
+    const long total = M * pitch;
+    for (long i = blockIdx.x * (long)kT + threadIdx.x; i < total; i += (long)gridDim.x * kT) {
+        const long m = i / pitch, n = i - m * pitch;
+        if constexpr (PARTS == 1) {
+            out[i] = n < N ? reinterpret_cast<const unsigned short*>(dy)[m * ld + n] : 0;
+        } else {
+            float left = n < N ? load_elem<T>(dy, m * ld + n) : 0.f;
 #pragma unroll
             for (int p = 0; p < PARTS; ++p) {
-                const float top = p + 1 < PARTS ? __uint_as_float(__float_as_uint(left) & 0xffff0000u) : left;
-                fa[p][e] = (__bf16)top;
-                left = top == left ? 0.f : left - top;
+                const unsigned top = __float_as_uint(left) & 0xffff0000u;  // towards zero: never past the largest number
+                out[p * total + i] = (unsigned short)(left != left ? 0x7fc0u : top >> 16);
+                left = left != left || __uint_as_float(top) == left ? 0.f : left - __uint_as_float(top);
             }
-            const long n = n0 + h * 8 + e;
-            float c = 0.f;
-            if (n < N)
-                c = code_value(codes[(g * N + n) * kGroupBytes + kb * 16 + (l >> 1)] >> (4 * (l & 1))) * scale_value(scales[(g * N + n) * 8 + kb]);
-            fb[e] = (__bf16)c;
+        }
+    }
+}
+
+// dx = dy W for a frozen W: 256 rows x 256 columns (one group of W's) per workgroup of 8 waves, 64 rows of W a step.  dy comes
+// by DMA like the tiles above; W's codes (8 KB a step) are widened to 16 bits on the way into LDS [n][column] and read transposed
+// (ds_read_b64_tr_b16).  The scale of a weight varies along the sum, so it is applied while widening -- relative to the
+// largest scale of its 32 columns over this workgroup's rows of W, which the outputs are multiplied with in the end:
+// nothing can overflow, and bf16 keeps weights down to 2^-126 of the largest.  fp16 holds scales that are at most 2^26 apart
+// exactly; where a workgroup finds them further apart it cuts each dy value into two bf16 parts (8 + 3 bits) instead.
+template <typename T, bool CUT>
+__device__ __forceinline__ void dgrad_mma(f32x16& acc, const uint4& a, const uint4& b) {
+    if constexpr (!CUT) {
+        mma32<T>(acc, __builtin_bit_cast(typename MmaFrag<T>::type, a), __builtin_bit_cast(typename MmaFrag<T>::type, b));
+    } else {
+        float f[8];
+        unpack16<_Float16>(a, f);
+        bf16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float top = __uint_as_float(__float_as_uint(f[e]) & 0xffff0000u);
+            hi[e] = (__bf16)top;
+            lo[e] = (__bf16)(top == f[e] ? 0.f : f[e] - top);
+        }
+        mma32<__bf16>(acc, hi, __builtin_bit_cast(bf16x8, b));
+        mma32<__bf16>(acc, lo, __builtin_bit_cast(bf16x8, b));
+    }
+}
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+template <typename T, int SEL>
+__device__ __forceinline__ unsigned widen2(unsigned codes, float scale) {
+    if constexpr (__is_same(T, _Float16)) return __builtin_bit_cast(unsigned, (f16x2)__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, SEL));
+    else return __builtin_bit_cast(unsigned, (bf16x2)__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, SEL));
+}
+template <typename T>
+__device__ __forceinline__ uint4 widen8(unsigned codes, float scale) {
+    return make_uint4(widen2<T, 0>(codes, scale), widen2<T, 1>(codes, scale), widen2<T, 2>(codes, scale), widen2<T, 3>(codes, scale));
+}
+
+struct DgradArgs {
+    const unsigned char *dy, *codes, *scales;
+    long pitch, M, N, width, part_bytes;  // pitch in bytes; width = dy's columns, N (copied: N rounded up to 8); a part = a whole [M][pitch]
+    int parts, steps, per_split;   // steps of 64 rows of W, times the parts
+    long cols;
+    void* dx;
+    float* sums;
+    unsigned mt, kt;
+};
+
+constexpr int kDA = 256 * 128, kDB = 64 * 512;  // bytes of one stage: dy [256][64], W [64][256]
+
+template <typename T, bool CUT>
+__device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const int* __restrict__ emax, f32x16 (&acc)[4][2], long m0, long g,
+                                           int s0, int s1) {
+    typedef typename std::conditional<CUT, __bf16, T>::type TW;
+    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, l = lane & 31;
+    const int nsteps = p.steps / p.parts;
+    const long mrows = min(256L, p.M - m0);
+    const int row8 = lane >> 3, chunk = (lane & 7) ^ row8;
+    auto fill_a = [&](int s, char* st) {
+        const int part = s / nsteps;
+        const long n0 = (s - part * nsteps) * 64L;
+        const __amdgpu_buffer_rsrc_t ra = buffer_of(p.dy + part * p.part_bytes + m0 * p.pitch + n0 * 2, (mrows - 1) * p.pitch + (p.width - n0) * 2);
+        const bool inside = n0 + chunk * 8 < p.width;  // whole chunks: the width is a multiple of 8
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = (i * 8 + w) * 8;
+            lds_dma16_buf(ra, st + r * 128, inside ? (int)((r + row8) * p.pitch) + chunk * 16 : (int)0x80000000, 0);
+        }
+    };
+    // a thread takes block kb of one row of W: 16 bytes of codes, one scale
+    const int nr = t >> 3, kb = t & 7;
+    auto load_b = [&](int s, uint4& c, int& e) {
+        const long n = (s % nsteps) * 64L + nr;
+        if (n < p.N) {
+            c = *reinterpret_cast<const uint4*>(p.codes + (g * p.N + n) * kGroupBytes + kb * 16);
+            e = p.scales[(g * p.N + n) * 8 + kb];
+        } else {
+            c = make_uint4(0, 0, 0, 0);
+            e = 0;
+        }
+    };
+    const int base = emax[kb];
+    auto store_b = [&](const uint4& c, int e, char* st) {
+        const int x = e == 255 ? 255 : max(e - base + (CUT || !__is_same(T, _Float16) ? 127 : 140), 0);
+        const float scale = __uint_as_float((unsigned)x << 23);
+        char* q = st + nr * 512 + ((kb ^ (nr & 3)) << 6);
+        *reinterpret_cast<uint4*>(q) = widen8<TW>(c.x, scale);
+        *reinterpret_cast<uint4*>(q + 16) = widen8<TW>(c.y, scale);
+        *reinterpret_cast<uint4*>(q + 32) = widen8<TW>(c.z, scale);
+        *reinterpret_cast<uint4*>(q + 48) = widen8<TW>(c.w, scale);
+    };
+    const int wm = w >> 2, wn = w & 3, li = lane & 15, gr = lane >> 4;
+    const int brow = (gr >> 1) * 8 + (li >> 2);  // + 16 ks (+ 4): the swizzle depends on the two lowest bits alone
+    int boff[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int cb = (wn * 64 + j * 32 + (gr & 1) * 16 + (li & 3) * 4) * 2;
+        boff[j] = brow * 512 + ((((cb >> 6) ^ (brow & 3)) << 6) | (cb & 63));
+    }
+    auto compute = [&](const char* sa, const char* sb) {
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            uint4 fa[4], fb[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                fa[i] = *reinterpret_cast<const uint4*>(sa + (wm * 128 + i * 32 + l) * 128 + (((ks * 2 + h) ^ (l & 7)) << 4));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const char* q = sb + boff[j] + ks * 16 * 512;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q));
+                const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q + 4 * 512));
+                fb[j] = __builtin_bit_cast(uint4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) dgrad_mma<T, CUT>(acc[i][j], fa[i], fb[j]);
+        }
+    };
+
+    uint4 c;
+    int e;
+    load_b(s0, c, e);
+    store_b(c, e, smem + 2 * kDA);
+    fill_a(s0, smem);
+    load_b(min(s0 + 1, s1 - 1), c, e);
+    for (int s = s0; s < s1; ++s) {
+        const int cur = (s - s0) & 1;
+        stage_barrier();
+        if (s + 1 < s1) {
+            store_b(c, e, smem + 2 * kDA + (cur ^ 1) * kDB);  // its codes arrived before the barrier
+            fill_a(s + 1, smem + (cur ^ 1) * kDA);
+            load_b(min(s + 2, s1 - 1), c, e);
+        }
+        compute(smem + cur * kDA, smem + 2 * kDA + cur * kDB);
+    }
+}
+
+template <typename T, typename TO>
+__global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
+    __shared__ __attribute__((aligned(1024))) char smem[2 * (kDA + kDB)];
+    __shared__ int emax[8], emin[8];
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6, h = lane >> 5, l = lane & 31;
+    unsigned tm, tk;
+    tile_of(xcd_remap(blockIdx.x, gridDim.x), p.mt, p.kt, tm, tk);
+    const long m0 = tm * 256L, k0 = tk * 256L, g = tk;
+    const int s0 = blockIdx.y * p.per_split, s1 = min(p.steps, s0 + p.per_split);
+    // the range of the scales, over all rows of W (a split that covered some of them alone could use a range of its own; the
+    // whole range serves every part of dy)
+    if (t < 8) emax[t] = 0, emin[t] = 255;
+    __syncthreads();
+    {
+        int hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hi[i] = 0, lo[i] = 255;
+        for (long n = t; n < p.N; n += 512) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p.scales + (g * p.N + n) * 8);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int x = ((i < 4 ? v.x : v.y) >> (8 * (i & 3))) & 255;
+                hi[i] = max(hi[i], x == 255 ? 0 : x);
+                lo[i] = min(lo[i], x == 0 ? 255 : x);  // E = 0 stands for zeros in all but the smallest of weights
+            }
         }
 #pragma unroll
-        for (int p = 0; p < PARTS; ++p) mma32<__bf16>(acc, fa[p], fb);
+        for (int i = 0; i < 8; ++i) atomicMax(&emax[i], hi[i]), atomicMin(&emin[i], lo[i]);
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) part[w][((i & 3) + 8 * (i >> 2) + 4 * h) * 33 + l] = acc[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < 1024; i += kT) {
-        const int r = i >> 5, c = i & 31;
-        if (m0 + r >= M || k0 + c >= cols) continue;
-        store_elem<TO>(dx, (m0 + r) * cols + k0 + c, (part[0][r * 33 + c] + part[1][r * 33 + c]) + (part[2][r * 33 + c] + part[3][r * 33 + c]));
+    f32x16 acc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    int bias = 127;
+    if constexpr (__is_same(T, _Float16)) {
+        bool wide = false;
+        for (int i = 0; i < 8; ++i) wide |= emax[i] - emin[i] > 26;
+        if (wide) {
+            dgrad_loop<T, true>(p, smem, emax, acc, m0, g, s0, s1);
+        } else {
+            dgrad_loop<T, false>(p, smem, emax, acc, m0, g, s0, s1);
+            bias = 140;
+        }
+    } else {
+        dgrad_loop<T, false>(p, smem, emax, acc, m0, g, s0, s1);
+    }
+    const int wm = w >> 2, wn = w & 3;
+    float* part = p.sums + (long)blockIdx.y * p.M * p.cols;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int kc = wn * 64 + j * 32;
+        const long k = k0 + kc + l;
+        if (k >= p.cols) continue;
+        const int up = emax[kc >> 5] - bias;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const long m = m0 + wm * 128 + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
+                if (m >= p.M) continue;
+                const float v = ldexpf(acc[i][j][e], up);
+                if (p.sums != nullptr) part[m * p.cols + k] = v;
+                else store_elem<TO>((TO*)p.dx, m * p.cols + k, v);
+            }
     }
 }
 
 long groups_of(long cols) { return (cols + kGroup - 1) / kGroup; }
-bool grid_ok(long blocks) { return blocks > 0 && blocks <= 0xffffffL; }  // a grid holds fewer than 2^32 threads
+bool grid_ok(long blocks, int threads = kT) { return blocks > 0 && blocks <= 0xffffffffL / threads; }  // a grid holds fewer than 2^32 threads
+
+// How the work of y = a b^T is cut.
+struct GemmPlan {
+    int tile;        // 0: few rows, straight from memory; else the edge of a square tile
+    long mt, nt;
+    int splits, per_split;
+};
+constexpr long kCus = 256;
+GemmPlan gemm_plan(long M, long N, long G) {
+    GemmPlan p = {0, (M + 31) / 32, (N + 31) / 32, 1, (int)G};
+    if (M <= 32) return p;
+    const long big = ((M + 255) / 256) * ((N + 255) / 256);
+    p.tile = big >= kCus ? 256 : 128;
+    p.mt = (M + p.tile - 1) / p.tile;
+    p.nt = (N + p.tile - 1) / p.tile;
+    const long tiles = p.mt * p.nt;
+    if (p.tile == 128 && tiles < kCus) {  // two such workgroups run on a CU; a part keeps at least 4 steps
+        long s = (2 * kCus) / tiles;
+        if (s > G / 4) s = G / 4;
+        if (s > 1) {
+            p.per_split = (int)((G + s - 1) / s);
+            p.splits = (int)((G + p.per_split - 1) / p.per_split);
+        }
+    }
+    return p;
+}
+
+struct DgradPlan {
+    long mt, kt, pitch;  // pitch of the copied parts in elements, 0: dy is taken as it lies
+    int parts, steps, splits, per_split;
+};
+DgradPlan dgrad_plan(int dtype, const void* dy, long ld, long M, long N, long cols) {
+    DgradPlan p = {(M + 255) / 256, groups_of(cols), 0, dtype == MSFWSI_DT_F32 ? 3 : 1, 0, 1, 0};
+    // DMA takes 16-byte chunks of rows, and a tile's rows lie within 2 GB
+    if (dtype == MSFWSI_DT_F32 || N % 8 != 0 || (M > 1 && ld % 8 != 0) || ld > (1L << 21) || (reinterpret_cast<uintptr_t>(dy) & 15)) p.pitch = (N + 7) / 8 * 8;
+    p.steps = p.parts * (int)((N + 63) / 64);
+    p.per_split = p.steps;
+    const long tiles = p.mt * p.kt;
+    if (tiles < kCus) {
+        long s = kCus / tiles;
+        if (s > p.steps / 8) s = p.steps / 8;
+        if (s > 1) {
+            p.per_split = (int)((p.steps + s - 1) / s);
+            p.splits = (p.steps + p.per_split - 1) / p.per_split;
+        }
+    }
+    return p;
+}
+long round16(long bytes) { return (bytes + 15) / 16 * 16; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+unsigned stride_grid(long items) {
+    const long b = (items + kT - 1) / kT;
+    return (unsigned)(b > 8 * kCus ? 8 * kCus : b);
+}
 
 }  // namespace
 
@@ -183,7 +558,7 @@ extern "C" int msfwsi_mx4_quantize(int dtype, const void* x, long ld, long rows,
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && rows >= 0 && cols > 0 && (rows <= 1 || ld >= cols));
     if (rows == 0) return MSFWSI_OK;
     const long G = groups_of(cols);
-    MSFWSI_CHECK_ARG(x && codes && scales && G <= 65535 && grid_ok((rows + 7) / 8));
+    MSFWSI_CHECK_ARG(x && codes && scales && aligned16(codes) && aligned16(scales) && G <= 65535 && grid_ok((rows + 7) / 8));
     MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_quantize_kernel<T>, dim3((unsigned)((rows + 7) / 8), (unsigned)G), dim3(kT), 0, ST(stream),
                                             (const T*)x, ld, rows, cols, (unsigned*)codes, (unsigned*)scales));
     return msfwsi_launch_status();
@@ -193,40 +568,104 @@ extern "C" int msfwsi_mx4_dequantize(int dtype, const void* codes, const void* s
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && rows >= 0 && cols > 0);
     if (rows == 0) return MSFWSI_OK;
     const long G = groups_of(cols);
-    MSFWSI_CHECK_ARG(y && codes && scales && G <= 65535 && grid_ok((rows + 7) / 8));
+    MSFWSI_CHECK_ARG(y && codes && scales && aligned16(codes) && aligned16(scales) && G <= 65535 && grid_ok((rows + 7) / 8));
     MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_dequantize_kernel<T>, dim3((unsigned)((rows + 7) / 8), (unsigned)G), dim3(kT), 0, ST(stream),
                                             (const unsigned*)codes, (const unsigned char*)scales, rows, cols, (T*)y));
     return msfwsi_launch_status();
 }
 
+extern "C" int msfwsi_mx4_gemm_workspace(long M, long N, long cols, long* bytes) {
+    MSFWSI_CHECK_ARG(bytes && M >= 0 && N > 0 && cols > 0 && groups_of(cols) <= 0x7fffffffL);
+    const GemmPlan p = gemm_plan(M, N, groups_of(cols));
+    *bytes = p.splits > 1 ? p.splits * M * N * 4 : 0;
+    return MSFWSI_OK;
+}
+
 extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_scales, long M, const void* b_codes, const void* b_scales,
-                               long N, long cols, const float* bias, void* y, void* stream) {
+                               long N, long cols, const float* bias, void* y, void* workspace, void* stream) {
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && M >= 0 && N > 0 && cols > 0);
     if (M == 0) return MSFWSI_OK;
-    const long mt = (M + 31) / 32, nt = (N + 31) / 32, G = groups_of(cols);
-    MSFWSI_CHECK_ARG(a_codes && a_scales && b_codes && b_scales && y && G <= 0x7fffffffL && nt <= 0x7fffffffL && mt <= 0x7fffffffL && grid_ok(mt * nt));
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_gemm_kernel<T>, dim3((unsigned)(mt * nt)), dim3(kT), 0, ST(stream),
-                                            (const unsigned char*)a_codes, (const unsigned char*)a_scales, M, (const unsigned char*)b_codes,
-                                            (const unsigned char*)b_scales, N, (int)G, bias, (T*)y, (unsigned)nt));
+    const long G = groups_of(cols);
+    MSFWSI_CHECK_ARG(a_codes && a_scales && b_codes && b_scales && y && G <= 0x7fffffffL);
+    MSFWSI_CHECK_ARG(aligned16(a_codes) && aligned16(a_scales) && aligned16(b_codes) && aligned16(b_scales));
+    const GemmPlan p = gemm_plan(M, N, G);
+    MSFWSI_CHECK_ARG(p.splits == 1 || (workspace && aligned16(workspace)));
+    if (p.mt > 0x7fffffffL || p.nt > 0x7fffffffL || p.nt > 0x7fffffffL / p.mt || !grid_ok(p.mt * p.nt, 1024)) return MSFWSI_EUNSUPPORTED;
+    const unsigned char *a = (const unsigned char*)a_codes, *as = (const unsigned char*)a_scales;
+    const unsigned char *b = (const unsigned char*)b_codes, *bs = (const unsigned char*)b_scales;
+    const unsigned mt = (unsigned)p.mt, nt = (unsigned)p.nt;
+    if (p.tile == 0) {
+#define MX4_ROWS(NW) \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((mx4_gemm_kernel<T, NW>), dim3(mt* nt), dim3(NW * 64), 0, ST(stream), a, as, M, b, bs, N, (int)G, bias, (T*)y, nt))
+        MX4_ROWS(4);
+        return msfwsi_launch_status();
+    }
+    float* sums = p.splits > 1 ? (float*)workspace : nullptr;
+#define MX4_TILE(TM, WM, WN)                                                                                                                   \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((mx4_tile_kernel<T, TM, TM, WM, WN>), dim3(mt* nt, p.splits), dim3(WM * WN * 64), 0, ST(stream), a, as, \
+                                            M, b, bs, N, (int)G, p.per_split, bias, (T*)y, sums, mt, nt))
+    if (p.tile == 256) MX4_TILE(256, 2, 4);
+    else MX4_TILE(128, 2, 2);
+    const int rc = msfwsi_launch_status();
+    if (rc != MSFWSI_OK || p.splits == 1) return rc;
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_join_kernel<T>, dim3(stride_grid(M * N)), dim3(kT), 0, ST(stream), sums, p.splits, M * N, N, bias, (T*)y));
     return msfwsi_launch_status();
 }
 
+extern "C" int msfwsi_mx4_dgrad_workspace(int dy_dtype, const void* dy, long ld, long M, long N, long cols, long* bytes) {
+    MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dy_dtype) && bytes && M >= 0 && N > 0 && cols > 0);
+    const DgradPlan p = dgrad_plan(dy_dtype, dy, ld, M > 0 ? M : 1, N, cols);
+    *bytes = round16(p.parts * M * p.pitch * 2) + (p.splits > 1 ? p.splits * M * cols * 4 : 0);
+    return MSFWSI_OK;
+}
+
 extern "C" int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, const void* codes, const void* scales, long N, long cols,
-                                int dx_dtype, void* dx, void* stream) {
+                                int dx_dtype, void* dx, void* workspace, void* stream) {
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dy_dtype) && msfwsi_dtype_ok(dx_dtype) && M >= 0 && N > 0 && cols > 0 && (M <= 1 || ld >= N));
     if (M == 0) return MSFWSI_OK;
-    const long mt = (M + 31) / 32, kt = (cols + 31) / 32;
-    MSFWSI_CHECK_ARG(dy && codes && scales && dx && kt <= 0x7fffffffL && mt <= 0x7fffffffL && grid_ok(mt * kt));
-#define MX4_DGRAD(TO)                                                                                                              \
-    MSFWSI_WITH_T(dy_dtype, hipLaunchKernelGGL((mx4_dgrad_kernel<T, TO>), dim3((unsigned)(mt * kt)), dim3(kT), 0, ST(stream),     \
-                                               (const T*)dy, ld, M, (const unsigned char*)codes, (const unsigned char*)scales, N, \
-                                               cols, (TO*)dx, (unsigned)kt))
-    if (dx_dtype == MSFWSI_DT_BF16) {
-        MX4_DGRAD(__bf16);
-    } else if (dx_dtype == MSFWSI_DT_F16) {
-        MX4_DGRAD(_Float16);
-    } else {
-        MX4_DGRAD(float);
+    MSFWSI_CHECK_ARG(dy && codes && scales && dx && aligned16(codes) && aligned16(scales));
+    const DgradPlan p = dgrad_plan(dy_dtype, dy, ld, M, N, cols);
+    MSFWSI_CHECK_ARG((p.pitch == 0 && p.splits == 1) || (workspace && aligned16(workspace)));
+    if (N > (1L << 21) || p.mt > 0x7fffffffL || p.kt > 0x7fffffffL || p.kt > 0x7fffffffL / p.mt || !grid_ok(p.mt * p.kt, 512)) return MSFWSI_EUNSUPPORTED;
+    const long copied = p.parts * M * p.pitch * 2;
+    if (p.pitch != 0) {
+        unsigned short* out = (unsigned short*)workspace;
+        if (dy_dtype == MSFWSI_DT_F32)
+            hipLaunchKernelGGL((mx4_parts_kernel<float, 3>), dim3(stride_grid(M * p.pitch)), dim3(kT), 0, ST(stream), (const float*)dy, ld, M, N, p.pitch, out);
+        else
+            hipLaunchKernelGGL((mx4_parts_kernel<__bf16, 1>), dim3(stride_grid(M * p.pitch)), dim3(kT), 0, ST(stream), (const __bf16*)dy, ld, M, N, p.pitch, out);
+        const int rc = msfwsi_launch_status();
+        if (rc != MSFWSI_OK) return rc;
     }
+    DgradArgs d;
+    d.dy = p.pitch != 0 ? (const unsigned char*)workspace : (const unsigned char*)dy;
+    d.codes = (const unsigned char*)codes;
+    d.scales = (const unsigned char*)scales;
+    d.pitch = (p.pitch != 0 ? p.pitch : ld) * 2;
+    d.M = M;
+    d.N = N;
+    d.width = p.pitch != 0 ? p.pitch : N;
+    d.part_bytes = M * p.pitch * 2;
+    d.parts = p.parts;
+    d.steps = p.steps;
+    d.per_split = p.per_split;
+    d.cols = cols;
+    d.dx = dx;
+    d.sums = p.splits > 1 ? (float*)((char*)workspace + round16(copied)) : nullptr;
+    d.mt = (unsigned)p.mt;
+    d.kt = (unsigned)p.kt;
+    const dim3 grid((unsigned)(p.mt * p.kt), p.splits);
+#define MX4_DGRAD(TO)                                                                                                  \
+    do {                                                                                                               \
+        if (dy_dtype == MSFWSI_DT_F16) hipLaunchKernelGGL((mx4_dgrad_kernel<_Float16, TO>), grid, dim3(512), 0, ST(stream), d); \
+        else hipLaunchKernelGGL((mx4_dgrad_kernel<__bf16, TO>), grid, dim3(512), 0, ST(stream), d);                    \
+    } while (0)
+    if (dx_dtype == MSFWSI_DT_BF16) MX4_DGRAD(__bf16);
+    else if (dx_dtype == MSFWSI_DT_F16) MX4_DGRAD(_Float16);
+    else MX4_DGRAD(float);
+    const int rc = msfwsi_launch_status();
+    if (rc != MSFWSI_OK || p.splits == 1) return rc;
+    MSFWSI_WITH_T(dx_dtype, hipLaunchKernelGGL(mx4_join_kernel<T>, dim3(stride_grid(M * cols)), dim3(kT), 0, ST(stream), d.sums, p.splits, M * cols, cols,
+                                               (const float*)nullptr, (T*)dx));
     return msfwsi_launch_status();
 }

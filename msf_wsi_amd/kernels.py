@@ -1755,9 +1755,12 @@ def mx4_gemm(a_codes, a_scales, b_codes, b_scales, cols: int, y, bias=None):
     if bias is not None:
         _dense(bias, "bias", torch.float32, N)
     _one_device(y, a_codes, b_codes, bias)
+    need = C.c_long()
+    _lib.check(lib.msfwsi_mx4_gemm_workspace(M, N, int(cols), C.byref(need)), "mx4_gemm_workspace")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=y.device) if need.value else None
     with torch.cuda.device(y.device):
         _lib.check(lib.msfwsi_mx4_gemm(dt_of(y), _p(a_codes), _p(a_scales), M, _p(b_codes), _p(b_scales), N, int(cols), _p(bias), _p(y),
-                                       _stream()), "mx4_gemm")
+                                       _p(ws), _stream()), "mx4_gemm")
     return y
 
 
@@ -1769,9 +1772,12 @@ def mx4_dgrad(dy, codes, scales, dx):
         raise ValueError(f"dy has {N} columns, w {codes.shape[1]} rows")
     _req(dx, "dx", numel=M * dx.shape[1])
     _one_device(dy, codes, dx)
+    need = C.c_long()
+    _lib.check(lib.msfwsi_mx4_dgrad_workspace(dt_of(dy), _p(dy), ld, M, N, dx.shape[1], C.byref(need)), "mx4_dgrad_workspace")
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dy.device) if need.value else None
     with torch.cuda.device(dy.device):
-        _lib.check(lib.msfwsi_mx4_dgrad(dt_of(dy), _p(dy), ld, M, _p(codes), _p(scales), N, dx.shape[1], dt_of(dx), _p(dx), _stream()),
-                   "mx4_dgrad")
+        _lib.check(lib.msfwsi_mx4_dgrad(dt_of(dy), _p(dy), ld, M, _p(codes), _p(scales), N, dx.shape[1], dt_of(dx), _p(dx), _p(ws),
+                                        _stream()), "mx4_dgrad")
     return dx
 
 

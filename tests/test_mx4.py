@@ -56,7 +56,7 @@ def test_c_entry_checks(hip_lib):
     assert hip_lib.msfwsi_mx4_quantize(0, None, 16, 2, 32, None, None, None) == -1     # rows overlap
     assert hip_lib.msfwsi_mx4_quantize(0, None, 32, 0, 32, None, None, None) == 0      # no rows
     assert hip_lib.msfwsi_mx4_dequantize(0, None, None, 1, 0, None, None) == -1
-    assert hip_lib.msfwsi_mx4_dgrad(0, None, 4, 1, None, None, 0, 32, 0, None, None) == -1
+    assert hip_lib.msfwsi_mx4_dgrad(0, None, 4, 1, None, None, 0, 32, 0, None, None, None) == -1
 
 
 # ---- GPU -------------------------------------------------------------------------------------------------------------
@@ -131,7 +131,7 @@ def test_quantize_slices(hip_lib, dt, offset, pitch):
 
 
 SIZES = [(1, 1, 1), (1, 256, 1000), (2, 513, 33), (5, 64, 7), (31, 255, 65), (33, 1001, 129), (64, 2048, 512), (130, 300, 257), (257, 4608, 300),
-         (300, 256, 1), (1, 18432, 40), (16, 9216, 64), (520, 2304, 391)]
+         (300, 256, 1), (1, 18432, 40), (16, 9216, 64), (520, 2304, 391), (4096, 300, 4100), (40, 18432, 70), (33, 70, 3000)]
 
 
 @pytest.mark.gpu
@@ -198,6 +198,27 @@ def test_weights_of_very_different_size(hip_lib):
         dx, = torch.autograd.grad(y, xc, dy.cuda())
         want, mass = dy.double() @ wq, dy.double().abs() @ wq.abs()
         assert bool(((dx.cpu().double() - want).abs() <= bound(3 * 48, mass, want, torch.float32)).all()), dt
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+def test_gradient_through_small_and_nan_weights(hip_lib, dt):
+    """rows of W whose size alone decides an output (zeros of dy hide the others), over all scales; blocks of NaN"""
+    from msf_wsi_amd import quant
+
+    dt = FP[dt]
+    e = torch.tensor([0, -20, -45, -70, -90, -8, 3, -60])
+    w = torch.ldexp(features(8, 96, torch.float32, 20).clamp(-30, 30), e.view(8, 1))
+    dy = torch.eye(8).to(dt) * 3
+    w[6, 40] = math.inf
+    w4 = quant.quantize_mx4(w.cuda())
+    x = torch.zeros(8, 96, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(quant.mx4_linear(x, w4, out_dtype=dt), x, dy.cuda())
+    want = 3 * to.mx4_round(w)[0]
+    assert dx[:, 32:64].isnan().all()                      # 0 * NaN: the block of the weight reaches every row
+    got = dx.cpu().double()
+    got[:, 32:64], want[:, 32:64] = 0.0, 0.0
+    assert torch.equal(got, want)                          # one term: exact
 
 
 @pytest.mark.gpu
