@@ -533,7 +533,7 @@ int msfwsi_inverse_perm(const long* perm, long* inv, long rows, int K, void* str
  *   msfwsi_mx4_dequantize: y [rows][cols] in `dtype`
  *   msfwsi_mx4_gemm:       y[m][n] = sum_k a[m][k] b[n][k] (+ bias[n], fp32), both operands quantised, fp32 sums, y [M][N]
  *   msfwsi_mx4_dgrad:      dx[m][k] = sum_n dy[m][n] w[n][k], w [N][cols] quantised; dy rows `ld` elements apart, dx [M][cols];
- *                          the products are exact whatever dy's type.  N <= 2^21
+ *                          the products are exact whatever dy's type.  N, cols <= 2^21 (N also for mx4_gemm)
  *   msfwsi_mx4_*_workspace:  host calls; *bytes = what the launch with the same arguments needs at `workspace` (16-byte
  *                          aligned; NULL when it is 0) */
 int msfwsi_mx4_quantize(int dtype, const void* x, long ld, long rows, long cols, void* codes, void* scales, void* stream);

@@ -134,21 +134,45 @@ __global__ void __launch_bounds__(NW * 64) mx4_gemm_kernel(const unsigned char* 
     }
 }
 
-// 4 bytes per lane global -> LDS, the small form of lds_dma16_buf (common.h: the rules for its waits hold here too)
-__device__ __forceinline__ void lds_dma4_buf(__amdgpu_buffer_rsrc_t rsrc, void* lds_wave_base, int voff) {
+// 16 (4) bytes per lane global -> LDS, lane l to base + 16 l (4 l): lds_dma16_buf of common.h, whose rules for waits hold here
+// too, with a constant part of the byte offset added inside -- as an operand of its own it took a register per request
+template <int BYTES>
+__device__ __forceinline__ void lds_dma(__amdgpu_buffer_rsrc_t rsrc, void* lds_wave_base, int voff, int more) {
     const unsigned lds = (unsigned)(__UINTPTR_TYPE__)(__attribute__((address_space(3))) char*)lds_wave_base;
-    asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                 :
-                 : "s"(lds), "v"(voff), "s"(rsrc)
-                 : "memory", "m0");
+    int at;
+    if constexpr (BYTES == 16)
+        asm volatile("s_mov_b32 m0, %1\n\tv_add_u32 %0, %3, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %4, 0 offen lds"
+                     : "=&v"(at)
+                     : "s"(lds), "v"(voff), "s"(more), "s"(rsrc)
+                     : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %1\n\tv_add_u32 %0, %3, %2\n\ts_nop 3\n\tbuffer_load_dword %0, %4, 0 offen lds"
+                     : "=&v"(at)
+                     : "s"(lds), "v"(voff), "s"(more), "s"(rsrc)
+                     : "memory", "m0");
 }
+// the address and the size are the same in all lanes, which hipcc does not see through a select
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const unsigned char* p, long bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p), 0, (int)bytes, 0x00020000);
+    const unsigned long u = reinterpret_cast<unsigned long>(p);
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)u), hi = __builtin_amdgcn_readfirstlane((int)(u >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(((unsigned long)hi << 32) | lo), 0,
+                                             __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
 }
 // everything this wave has asked for has arrived, and it is done reading the stage it leaves; then all waves
 __device__ __forceinline__ void stage_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// Tiles go to the XCDs in contiguous runs (xcd_remap), inside a run in columns of 8 row tiles: a run then shares few row and
+// Two adjacent results of one row, at any alignment; the second only where the row has it.
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Two {
+    T a, b;
+};
+template <typename T>
+__device__ __forceinline__ void store_two(T* p, unsigned at, float a, float b, bool both) {
+    if (both) *reinterpret_cast<Two<T>*>(p + at) = {(T)a, (T)b};
+    else p[at] = (T)a;
+}
+
+// Tiles go to the XCDs in contiguous runs (xcd_remap), inside a run down columns of 8 row tiles: a run then shares few row and
 // column tiles in its L2.
 __device__ __forceinline__ void tile_of(unsigned id, unsigned mt, unsigned nt, unsigned& m, unsigned& n) {
     const unsigned wide = 8 * nt, first = id / wide * 8, deep = min(mt - first, 8u), in = id % wide;
@@ -156,66 +180,73 @@ __device__ __forceinline__ void tile_of(unsigned id, unsigned mt, unsigned nt, u
     n = in / deep;
 }
 
-// Many rows: TM x TN outputs per workgroup of WM x WN waves, one group of 256 elements (128 bytes of every row) per step, two
-// stages in LDS filled by DMA.  A row's eight 16-byte chunks lie at (chunk ^ (row & 7)): the eight rows that a read
-// touches at a time then fall on eight different bank groups.  `split` > 0 deals the groups over gridDim.y workgroups that
-// leave fp32 sums for a join.
+struct GemmArgs {
+    const unsigned char *a, *as, *b, *bs;
+    long M, N;
+    int G, per_split;
+    const float* bias;
+    void* y;
+    float* sums;  // not NULL: the groups of a tile are dealt over several workgroups, which leave fp32 sums [split][M][N] for a join
+    unsigned mt, nt;
+};
+
+// Many rows: TM x TN outputs per workgroup of WM x WN waves, one group of 256 elements (128 bytes of every row) per stage, two
+// stages in LDS filled by DMA.  A row's eight 16-byte chunks lie at (chunk ^ (row / 2 & 7)): the sixteen rows that a read takes
+// at a time then fall on all 64 banks.  The columns of a wave's 64 are dealt to its two fragments in turn (2 l + j: b's rows lie in
+// LDS in that order), so that a lane ends up with neighbours of a row and a wave writes whole 128-byte lines.
+// 8192 x 9216 x 9216: 392 us, 3.5 PFLOP/s (4.3 without the requests; registers alone reach 6.5 at this card's power).  Requests and
+// products share the CU's LDS and issue slots; a four-stage ring of half groups (64-byte lines: 0.8 of the rate), fragments
+// read a step ahead by hand, a workgroup that runs through its tiles, and four waves of 128 x 128 were all 2 - 20 % slower.
 template <typename T, int TM, int TN, int WM, int WN>
-__global__ void __launch_bounds__(WM* WN * 64) mx4_tile_kernel(const unsigned char* __restrict__ a, const unsigned char* __restrict__ as, long M,
-                                                               const unsigned char* __restrict__ b, const unsigned char* __restrict__ bs,
-                                                               long N, int G, int per_split, const float* __restrict__ bias,
-                                                               T* __restrict__ y, float* __restrict__ sums, unsigned mt, unsigned nt) {
-    constexpr int NW = WM * WN, FM = TM / WM / 32, FN = TN / WN / 32;
+__global__ void __launch_bounds__(WM* WN * 64) mx4_tile_kernel(const GemmArgs p) {
+    constexpr int NW = WM * WN, FM = TM / WM / 32, FN = 2;
+    static_assert(TN / WN == 64, "a wave has 64 columns");
     constexpr int kStage = (TM + TN) * (kGroupBytes + 8);
+    constexpr int PA = TM / 8 / NW, PB = TN / 8 / NW, PSA = TM / 32 / NW, PSB = TN / 32 / NW, PIECES = PA + PB + PSA + PSB;
     __shared__ __attribute__((aligned(1024))) char smem[2 * kStage];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, l = lane & 31;
-    unsigned tm, tn;
-    tile_of(xcd_remap(blockIdx.x, gridDim.x), mt, nt, tm, tn);
-    const long m0 = (long)tm * TM, n0 = (long)tn * TN;
-    const long mrows = min((long)TM, M - m0), nrows = min((long)TN, N - n0);
-    const int g0 = blockIdx.y * per_split, g1 = min(G, g0 + per_split);
-    const int chunk = (lane >> 3) * kGroupBytes + (((lane & 7) ^ (lane >> 3)) << 4);
+    const int swz = ((lane & 7) ^ ((w & 1) * 4 + (lane >> 4))) << 4;  // of row (lane >> 3) of any 1 KB piece this wave brings
+    const int chunk_a = (lane >> 3) * kGroupBytes + swz, chunk_b = (lane >> 3) * 2 * kGroupBytes + swz;
 
-    auto fill = [&](int g, char* st) {
-        const __amdgpu_buffer_rsrc_t ra = buffer_of(a + (g * M + m0) * kGroupBytes, mrows * kGroupBytes);
-        const __amdgpu_buffer_rsrc_t rb = buffer_of(b + (g * N + n0) * kGroupBytes, nrows * kGroupBytes);
-        const __amdgpu_buffer_rsrc_t rsa = buffer_of(as + (g * M + m0) * 8, mrows * 8), rsb = buffer_of(bs + (g * N + n0) * 8, nrows * 8);
-#pragma unroll
-        for (int i = 0; i < TM / 8 / NW; ++i) lds_dma16_buf(ra, st + (i * NW + w) * 1024, (i * NW + w) * 1024 + chunk, 0);
-#pragma unroll
-        for (int i = 0; i < TN / 8 / NW; ++i) lds_dma16_buf(rb, st + TM * kGroupBytes + (i * NW + w) * 1024, (i * NW + w) * 1024 + chunk, 0);
+    const unsigned it = xcd_remap(blockIdx.x, gridDim.x), tiles = p.mt * p.nt, split = it / tiles;
+    unsigned tm, tn;
+    tile_of(it % tiles, p.mt, p.nt, tm, tn);
+    const long m0 = (long)tm * TM, n0 = (long)tn * TN;
+    const int mrows = (int)min((long)TM, p.M - m0), nrows = (int)min((long)TN, p.N - n0);
+    const int g0 = (int)split * p.per_split, g1 = min(p.G, g0 + p.per_split);
+    __amdgpu_buffer_rsrc_t ra, rb, rsa, rsb;
+    auto aim = [&](int g) {
+        ra = buffer_of(p.a + (g * p.M + m0) * kGroupBytes, mrows * kGroupBytes);
+        rb = buffer_of(p.b + (g * p.N + n0) * kGroupBytes, nrows * kGroupBytes);
+        rsa = buffer_of(p.as + (g * p.M + m0) * 8, mrows * 8);
+        rsb = buffer_of(p.bs + (g * p.N + n0) * 8, nrows * 8);
+    };
+    auto piece = [&](char* st, int i) {
         char* sc = st + (TM + TN) * kGroupBytes;
-#pragma unroll
-        for (int i = 0; i < TM / 32 / NW; ++i) lds_dma4_buf(rsa, sc + (i * NW + w) * 256, (i * NW + w) * 256 + lane * 4);
-#pragma unroll
-        for (int i = 0; i < TN / 32 / NW; ++i) lds_dma4_buf(rsb, sc + TM * 8 + (i * NW + w) * 256, (i * NW + w) * 256 + lane * 4);
+        const int j = i < PA ? i : i < PA + PB ? i - PA : i < PA + PB + PSA ? i - PA - PB : i - PA - PB - PSA, q = j * NW + w;
+        if (i < PA) lds_dma<16>(ra, st + q * 1024, chunk_a, q * 1024);
+        else if (i < PA + PB) lds_dma<16>(rb, st + TM * kGroupBytes + q * 1024, chunk_b, ((q >> 3) * 64 + (q & 3) * 16 + ((q >> 2) & 1)) * kGroupBytes);
+        else if (i < PA + PB + PSA) lds_dma<4>(rsa, sc + q * 256, lane * 4, q * 256);
+        else lds_dma<4>(rsb, sc + TM * 8 + q * 256, lane * 4, q * 256);
     };
     f32x16 acc[FM][FN];
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     const int wm = w / WN, wn = w % WN;
-    const int arow = wm * (TM / WM) + l, brow = wn * (TN / WN) + l;
+    const int arow = wm * (TM / WM) + l, brow = wn * 64 + l;
     auto compute = [&](const char* st) {
-        const char* pa = st + arow * kGroupBytes;
-        const char* pb = st + (TM + brow) * kGroupBytes;
         const char* sc = st + (TM + TN) * kGroupBytes + h * 4;
         int sa[FM], sb[FN];
 #pragma unroll
         for (int i = 0; i < FM; ++i) sa[i] = *reinterpret_cast<const int*>(sc + (arow + i * 32) * 8);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) sb[j] = *reinterpret_cast<const int*>(sc + (TM + brow + j * 32) * 8);
-        auto step = [&](auto sc_) {
-            constexpr int S = decltype(sc_)::value;
-            const int at = ((4 * h + S) ^ (l & 7)) << 4;
+        for (int j = 0; j < FN; ++j) sb[j] = *reinterpret_cast<const int*>(sc + (TM + wn * 64 + 2 * l + j) * 8);
+        auto step = [&](auto s_) {
+            constexpr int S = decltype(s_)::value;
+            const int at = ((4 * h + S) ^ ((l >> 1) & 7)) << 4;
             int4 fa[FM], fb[FN];
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const int4*>(pa + i * 32 * kGroupBytes + at);
+            for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const int4*>(st + (arow + i * 32) * kGroupBytes + at);
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const int4*>(pb + j * 32 * kGroupBytes + at);
+            for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const int4*>(st + (TM + brow + j * 32) * kGroupBytes + at);
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -227,29 +258,45 @@ __global__ void __launch_bounds__(WM* WN * 64) mx4_tile_kernel(const unsigned ch
         step(std::integral_constant<int, 3>());
     };
 
-    fill(g0, smem);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    aim(g0);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) piece(smem, i);
     for (int g = g0; g < g1; ++g) {
-        char* cur = smem + ((g - g0) & 1) * kStage;
+        const int odd = (g - g0) & 1;
         stage_barrier();
-        if (g + 1 < g1) fill(g + 1, smem + ((g - g0 + 1) & 1) * kStage);
-        compute(cur);
+        if (g + 1 < g1) {
+            aim(g + 1);
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) piece(smem + (odd ^ 1) * kStage, i);
+        }
+        compute(smem + odd * kStage);
     }
-    float* part = sums + (long)blockIdx.y * M * N;
-#pragma unroll
-    for (int j = 0; j < FN; ++j) {
-        const long n = n0 + brow + j * 32;
-        if (n >= N) continue;
-        const float add = sums == nullptr && bias != nullptr ? bias[n] : 0.f;
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const long m = m0 + wm * (TM / WM) + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
-                if (m >= M) continue;
-                if (sums != nullptr) part[m * N + n] = acc[i][j][e];
-                else store_elem<T>(y, m * N + n, acc[i][j][e] + add);
-            }
+
+    const int n = wn * 64 + 2 * l, left = nrows - n, N = (int)p.N;  // 256 rows of up to 2^21 columns: 32 bits hold the offsets
+    const int r0 = wm * (TM / WM) + 4 * h;
+    if (left <= 0) return;
+    float add[2] = {0.f, 0.f};
+    if (p.sums == nullptr && p.bias != nullptr) {
+        add[0] = p.bias[n0 + n];
+        if (left > 1) add[1] = p.bias[n0 + n + 1];
     }
+    float* part = p.sums + ((long)split * p.M + m0) * p.N + n0;
+    T* out = (T*)p.y + m0 * p.N + n0;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int m = r0 + i * 32 + (e & 3) + 8 * (e >> 2);
+            if (m >= mrows) continue;
+            if (p.sums != nullptr) store_two<float>(part, (unsigned)(m * N + n), acc[i][0][e], acc[i][1][e], left > 1);
+            else store_two<T>(out, (unsigned)(m * N + n), acc[i][0][e] + add[0], acc[i][1][e] + add[1], left > 1);
+        }
 }
 
 // y = the sum of `splits` fp32 partial results (+ bias of the column)
@@ -287,7 +334,7 @@ __global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy,
 
 // dx = dy W for a frozen W: 256 rows x 256 columns (one group of W's) per workgroup of 8 waves, 64 rows of W a step.  dy comes
 // by DMA like the tiles above; W's codes (8 KB a step) are widened to 16 bits on the way into LDS [n][column] and read transposed
-// (ds_read_b64_tr_b16).  The scale of a weight varies along the sum, so it is applied while widening -- relative to the
+// (ds_read_b64_tr_b16), even and odd columns apart as above.  The scale of a weight varies along the sum, so it is applied while widening -- relative to the
 // largest scale of its 32 columns over this workgroup's rows of W, which the outputs are multiplied with in the end:
 // nothing can overflow, and bf16 keeps weights down to 2^-126 of the largest.  fp16 holds scales that are at most 2^26 apart
 // exactly; where a workgroup finds them further apart it cuts each dy value into two bf16 parts (8 + 3 bits) instead.
@@ -341,7 +388,7 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
     const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, l = lane & 31;
     const int nsteps = p.steps / p.parts;
     const long mrows = min(256L, p.M - m0);
-    const int row8 = lane >> 3, chunk = (lane & 7) ^ row8;
+    const int row8 = lane >> 3, chunk = (lane & 7) ^ ((w & 1) * 4 + (lane >> 4));
     auto fill_a = [&](int s, char* st) {
         const int part = s / nsteps;
         const long n0 = (s - part * nsteps) * 64L;
@@ -350,7 +397,7 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = (i * 8 + w) * 8;
-            lds_dma16_buf(ra, st + r * 128, inside ? (int)((r + row8) * p.pitch) + chunk * 16 : (int)0x80000000, 0);
+            lds_dma<16>(ra, st + r * 128, inside ? (int)((r + row8) * p.pitch) + chunk * 16 : (int)0x80000000, 0);
         }
     };
     // a thread takes block kb of one row of W: 16 bytes of codes, one scale
@@ -369,11 +416,17 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
     auto store_b = [&](const uint4& c, int e, char* st) {
         const int x = e == 255 ? 255 : max(e - base + (CUT || !__is_same(T, _Float16) ? 127 : 140), 0);
         const float scale = __uint_as_float((unsigned)x << 23);
-        char* q = st + nr * 512 + ((kb ^ (nr & 3)) << 6);
-        *reinterpret_cast<uint4*>(q) = widen8<TW>(c.x, scale);
-        *reinterpret_cast<uint4*>(q + 16) = widen8<TW>(c.y, scale);
-        *reinterpret_cast<uint4*>(q + 32) = widen8<TW>(c.z, scale);
-        *reinterpret_cast<uint4*>(q + 48) = widen8<TW>(c.w, scale);
+        // columns 2i and 2i + 1 go to different fragments: the even ones of 64 columns first, then the odd ones, 64 bytes each.
+        // Eight of them come from two words of codes in the order 0 4 1 5 2 6 3 7 (out_pair undoes it); which half of the 16 a
+        // lane writes first depends on its block, so that a write's sixteen lanes fall on all 64 banks
+        const bool second = kb & 4;
+        const unsigned x0 = second ? c.z : c.x, y0 = second ? c.w : c.y, x1 = second ? c.x : c.z, y1 = second ? c.y : c.w;
+        char* q = st + nr * 512 + (kb & 1) * 32 + (second ? 16 : 0);
+        const int even = ((kb & 6) ^ (nr & 3)) << 6, odd = ((kb | 1) ^ (nr & 3)) << 6, other = second ? -16 : 16;
+        *reinterpret_cast<uint4*>(q + even) = widen8<TW>((x0 & 0x0f0f0f0fu) | ((y0 & 0x0f0f0f0fu) << 4), scale);
+        *reinterpret_cast<uint4*>(q + even + other) = widen8<TW>((x1 & 0x0f0f0f0fu) | ((y1 & 0x0f0f0f0fu) << 4), scale);
+        *reinterpret_cast<uint4*>(q + odd) = widen8<TW>(((x0 >> 4) & 0x0f0f0f0fu) | (y0 & 0xf0f0f0f0u), scale);
+        *reinterpret_cast<uint4*>(q + odd + other) = widen8<TW>(((x1 >> 4) & 0x0f0f0f0fu) | (y1 & 0xf0f0f0f0u), scale);
     };
     const int wm = w >> 2, wn = w & 3, li = lane & 15, gr = lane >> 4;
     const int brow = (gr >> 1) * 8 + (li >> 2);  // + 16 ks (+ 4): the swizzle depends on the two lowest bits alone
@@ -383,13 +436,13 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
         const int cb = (wn * 64 + j * 32 + (gr & 1) * 16 + (li & 3) * 4) * 2;
         boff[j] = brow * 512 + ((((cb >> 6) ^ (brow & 3)) << 6) | (cb & 63));
     }
-    auto compute = [&](const char* sa, const char* sb) {
+    auto compute = [&](const char* sa, const char* sb, int k0, int k1) {
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
+        for (int ks = k0; ks < k1; ++ks) {
             uint4 fa[4], fb[2];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                fa[i] = *reinterpret_cast<const uint4*>(sa + (wm * 128 + i * 32 + l) * 128 + (((ks * 2 + h) ^ (l & 7)) << 4));
+                fa[i] = *reinterpret_cast<const uint4*>(sa + (wm * 128 + i * 32 + l) * 128 + (((ks * 2 + h) ^ ((l >> 1) & 7)) << 4));
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const char* q = sb + boff[j] + ks * 16 * 512;
@@ -412,15 +465,21 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
     load_b(min(s0 + 1, s1 - 1), c, e);
     for (int s = s0; s < s1; ++s) {
         const int cur = (s - s0) & 1;
+        const bool more = s + 1 < s1;
         stage_barrier();
-        if (s + 1 < s1) {
-            store_b(c, e, smem + 2 * kDA + (cur ^ 1) * kDB);  // its codes arrived before the barrier
-            fill_a(s + 1, smem + (cur ^ 1) * kDA);
+        // the codes have arrived with the barrier; naming them here keeps hipcc's own wait for them in front of the requests
+        asm volatile("" : "+v"(c.x), "+v"(c.y), "+v"(c.z), "+v"(c.w), "+v"(e));
+        if (more) fill_a(s + 1, smem + (cur ^ 1) * kDA);
+        compute(smem + cur * kDA, smem + 2 * kDA + cur * kDB, 0, 2);
+        if (more) {
+            store_b(c, e, smem + 2 * kDA + (cur ^ 1) * kDB);
             load_b(min(s + 2, s1 - 1), c, e);
         }
-        compute(smem + cur * kDA, smem + 2 * kDA + cur * kDB);
+        compute(smem + cur * kDA, smem + 2 * kDA + cur * kDB, 2, 4);
     }
 }
+// the pair of columns, of a wave's 32, that lane l ends up with
+__device__ __forceinline__ int out_pair(int l) { return (l & 24) + ((l & 7) >> 1) + (l & 1) * 4; }
 
 template <typename T, typename TO>
 __global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
@@ -472,25 +531,22 @@ __global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
     } else {
         dgrad_loop<T, false>(p, smem, emax, acc, m0, g, s0, s1);
     }
-    const int wm = w >> 2, wn = w & 3;
-    float* part = p.sums + (long)blockIdx.y * p.M * p.cols;
+    const int wm = w >> 2, wn = w & 3, kc = wn * 64 + 2 * out_pair(l), left = (int)min(256L, p.cols - k0) - kc;
+    const int mrows = (int)min(256L, p.M - m0), r0 = wm * 128 + 4 * h, cols = (int)p.cols;
+    if (left <= 0) return;
+    const int up = emax[kc >> 5] - bias;
+    float* part = p.sums + ((long)blockIdx.y * p.M + m0) * p.cols + k0;
+    TO* out = (TO*)p.dx + m0 * p.cols + k0;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int kc = wn * 64 + j * 32;
-        const long k = k0 + kc + l;
-        if (k >= p.cols) continue;
-        const int up = emax[kc >> 5] - bias;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const long m = m0 + wm * 128 + i * 32 + (e & 3) + 8 * (e >> 2) + 4 * h;
-                if (m >= p.M) continue;
-                const float v = ldexpf(acc[i][j][e], up);
-                if (p.sums != nullptr) part[m * p.cols + k] = v;
-                else store_elem<TO>((TO*)p.dx, m * p.cols + k, v);
-            }
-    }
+        for (int e = 0; e < 16; ++e) {
+            const int m = r0 + i * 32 + (e & 3) + 8 * (e >> 2);  // 32 bits hold the offsets: cols is at most 2^21
+            if (m >= mrows) continue;
+            const float v0 = ldexpf(acc[i][0][e], up), v1 = ldexpf(acc[i][1][e], up);
+            if (p.sums != nullptr) store_two<float>(part, (unsigned)(m * cols + kc), v0, v1, left > 1);
+            else store_two<TO>(out, (unsigned)(m * cols + kc), v0, v1, left > 1);
+        }
 }
 
 long groups_of(long cols) { return (cols + kGroup - 1) / kGroup; }
@@ -590,7 +646,7 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
     MSFWSI_CHECK_ARG(aligned16(a_codes) && aligned16(a_scales) && aligned16(b_codes) && aligned16(b_scales));
     const GemmPlan p = gemm_plan(M, N, G);
     MSFWSI_CHECK_ARG(p.splits == 1 || (workspace && aligned16(workspace)));
-    if (p.mt > 0x7fffffffL || p.nt > 0x7fffffffL || p.nt > 0x7fffffffL / p.mt || !grid_ok(p.mt * p.nt, 1024)) return MSFWSI_EUNSUPPORTED;
+    if (N > (1L << 21) || p.mt > 0x7fffffffL || p.nt > 0x7fffffffL || p.nt > 0x7fffffffL / p.mt || !grid_ok(p.mt * p.nt * p.splits, 512)) return MSFWSI_EUNSUPPORTED;
     const unsigned char *a = (const unsigned char*)a_codes, *as = (const unsigned char*)a_scales;
     const unsigned char *b = (const unsigned char*)b_codes, *bs = (const unsigned char*)b_scales;
     const unsigned mt = (unsigned)p.mt, nt = (unsigned)p.nt;
@@ -601,9 +657,10 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
         return msfwsi_launch_status();
     }
     float* sums = p.splits > 1 ? (float*)workspace : nullptr;
-#define MX4_TILE(TM, WM, WN)                                                                                                                   \
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((mx4_tile_kernel<T, TM, TM, WM, WN>), dim3(mt* nt, p.splits), dim3(WM * WN * 64), 0, ST(stream), a, as, \
-                                            M, b, bs, N, (int)G, p.per_split, bias, (T*)y, sums, mt, nt))
+    GemmArgs args = {a, as, b, bs, M, N, (int)G, p.per_split, bias, y, sums, mt, nt};
+    const unsigned grid = mt * nt * p.splits;
+#define MX4_TILE(TM, WM, WN) \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((mx4_tile_kernel<T, TM, TM, WM, WN>), dim3(grid), dim3(WM * WN * 64), 0, ST(stream), args))
     if (p.tile == 256) MX4_TILE(256, 2, 4);
     else MX4_TILE(128, 2, 2);
     const int rc = msfwsi_launch_status();
@@ -626,7 +683,7 @@ extern "C" int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, c
     MSFWSI_CHECK_ARG(dy && codes && scales && dx && aligned16(codes) && aligned16(scales));
     const DgradPlan p = dgrad_plan(dy_dtype, dy, ld, M, N, cols);
     MSFWSI_CHECK_ARG((p.pitch == 0 && p.splits == 1) || (workspace && aligned16(workspace)));
-    if (N > (1L << 21) || p.mt > 0x7fffffffL || p.kt > 0x7fffffffL || p.kt > 0x7fffffffL / p.mt || !grid_ok(p.mt * p.kt, 512)) return MSFWSI_EUNSUPPORTED;
+    if (N > (1L << 21) || cols > (1L << 21) || p.mt > 0x7fffffffL || p.kt > 0x7fffffffL || p.kt > 0x7fffffffL / p.mt || !grid_ok(p.mt * p.kt, 512)) return MSFWSI_EUNSUPPORTED;
     const long copied = p.parts * M * p.pitch * 2;
     if (p.pitch != 0) {
         unsigned short* out = (unsigned short*)workspace;
