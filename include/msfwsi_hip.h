@@ -532,6 +532,7 @@ int msfwsi_inverse_perm(const long* perm, long* inv, long rows, int K, void* str
  *                          largest magnitude - 2, 0), 255 when it is not finite; to nearest, ties to the even code, saturating
  *   msfwsi_mx4_dequantize: y [rows][cols] in `dtype`
  *   msfwsi_mx4_gemm:       y[m][n] = sum_k a[m][k] b[n][k] (+ bias[n], fp32), both operands quantised, fp32 sums, y [M][N]
+ *   msfwsi_mx4_linear:     mx4_quantize of x [M][cols] and mx4_gemm of the result with w [N][cols], in one call
  *   msfwsi_mx4_dgrad:      dx[m][k] = sum_n dy[m][n] w[n][k], w [N][cols] quantised; dy rows `ld` elements apart, dx [M][cols];
  *                          the products are exact whatever dy's type.  N, cols <= 2^21 (N also for mx4_gemm)
  *   msfwsi_mx4_*_workspace:  host calls; *bytes = what the launch with the same arguments needs at `workspace` (16-byte
@@ -541,6 +542,9 @@ int msfwsi_mx4_dequantize(int dtype, const void* codes, const void* scales, long
 int msfwsi_mx4_gemm_workspace(long M, long N, long cols, long* bytes);
 int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_scales, long M, const void* b_codes, const void* b_scales,
                     long N, long cols, const float* bias, void* y, void* workspace, void* stream);
+int msfwsi_mx4_linear_workspace(long M, long N, long cols, long* bytes);
+int msfwsi_mx4_linear(int dtype, const void* x, long ld, long M, const void* codes, const void* scales, long N, long cols,
+                      const float* bias, int y_dtype, void* y, void* workspace, void* stream);
 int msfwsi_mx4_dgrad_workspace(int dy_dtype, const void* dy, long ld, long M, long N, long cols, long* bytes);
 int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, const void* codes, const void* scales, long N, long cols,
                      int dx_dtype, void* dx, void* workspace, void* stream);
@@ -552,17 +556,17 @@ int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, const void* 
  *                       rest = log sum over the others of exp(logit * inv_t).  workspace: msfwsi_top_logits_workspace
  *                       bytes, 16-byte aligned (a host call; NULL when it says 0)
  *   msfwsi_distill_fwd: row_loss [rows] or NULL (0 where a row does not count), stats [rows][4] (16-byte aligned) for the
- *                       backward, partials [2048][2] scratch, loss[0] = sum or mean
- *                       over the rows that count, loss[1] = the gradient's factor.  rest / mask may be NULL.
- *                       outer = 0 writes loss alone
- *   msfwsi_distill_bwd: dz [outer][classes][inner] contiguous = g * factor[1] * d loss_row / dz; g holds one value, or one per
- *                       row with g_rows; factor (NULL = 1) is the forward's loss pair */
+ *                       backward, partials [2048][2] scratch, *loss = sum or mean over the rows that count, *factor = the
+ *                       gradient's (1 / their number for the mean, else 1).  rest / mask may be NULL.  outer = 0 writes loss and
+ *                       factor alone
+ *   msfwsi_distill_bwd: dz [outer][classes][inner] contiguous = g * factor * d loss_row / dz; g holds one value, or one per
+ *                       row with g_rows; factor is the forward's (NULL = 1) */
 int msfwsi_top_logits_workspace(int dtype, long outer, int classes, long inner, int k, long* bytes);
 int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, int classes, long inner, int k, float inv_t, float* values,
                       int* indices, float* rest, void* workspace, void* stream);
 int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer, int classes, long inner, int k, const float* values,
                        const int* indices, const float* rest, const unsigned char* mask, float temperature, int mean,
-                       float* stats, float* row_loss, float* loss, double* partials, void* stream);
+                       float* stats, float* row_loss, float* loss, float* factor, double* partials, void* stream);
 int msfwsi_distill_bwd(int dtype, const void* z, long ld, long outer, int classes, long inner, int k, const float* values,
                        const int* indices, const float* rest, float temperature, const float* stats, const float* factor,
                        const float* g, int g_rows, void* dz, void* stream);

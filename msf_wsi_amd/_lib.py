@@ -115,11 +115,13 @@ SIGNATURES = {
     "msfwsi_mx4_dequantize": [_i, _vp, _vp, _l, _l, _vp, _vp],
     "msfwsi_mx4_gemm_workspace": [_l, _l, _l, _vp],
     "msfwsi_mx4_gemm": [_i, _vp, _vp, _l, _vp, _vp, _l, _l, _vp, _vp, _vp, _vp],
+    "msfwsi_mx4_linear_workspace": [_l, _l, _l, _vp],
+    "msfwsi_mx4_linear": [_i, _vp, _l, _l, _vp, _vp, _l, _l, _vp, _i, _vp, _vp, _vp],
     "msfwsi_mx4_dgrad_workspace": [_i, _vp, _l, _l, _l, _l, _vp],
     "msfwsi_mx4_dgrad": [_i, _vp, _l, _l, _vp, _vp, _l, _l, _i, _vp, _vp, _vp],
     "msfwsi_top_logits_workspace": [_i, _l, _i, _l, _i, _vp],
     "msfwsi_top_logits": [_i, _vp, _l, _l, _i, _l, _i, _f, _vp, _vp, _vp, _vp, _vp],
-    "msfwsi_distill_fwd": [_i, _vp, _l, _l, _i, _l, _i, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _vp, _vp, _vp],
+    "msfwsi_distill_fwd": [_i, _vp, _l, _l, _i, _l, _i, _vp, _vp, _vp, _vp, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp],
     "msfwsi_distill_bwd": [_i, _vp, _l, _l, _i, _l, _i, _vp, _vp, _vp, _f, _vp, _vp, _vp, _i, _vp, _vp],
     "msfwsi_set_tuning": [_i, _l],
     "msfwsi_get_tuning": [_i, _vp],

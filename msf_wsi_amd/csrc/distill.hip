@@ -403,8 +403,9 @@ __device__ __forceinline__ void leave_part(double s, double n, double* __restric
         parts[2 * blockIdx.x + 1] = n;
     }
 }
-// loss[0] = sum or mean of the rows that count, loss[1] = the factor of the gradient (1 / their number for the mean)
-__global__ void __launch_bounds__(kT) distill_finish_kernel(const double* __restrict__ parts, int n, int mean, float* __restrict__ loss) {
+// loss = sum or mean of the rows that count, factor = that of the gradient (1 / their number for the mean)
+__global__ void __launch_bounds__(kT) distill_finish_kernel(const double* __restrict__ parts, int n, int mean, float* __restrict__ loss,
+                                                            float* __restrict__ factor) {
     __shared__ double sums[kT / 64], counts[kT / 64];
     double s = 0.0, m = 0.0;
     for (int i = threadIdx.x; i < n; i += kT) s += parts[2 * i], m += parts[2 * i + 1];
@@ -415,8 +416,8 @@ __global__ void __launch_bounds__(kT) distill_finish_kernel(const double* __rest
     if (threadIdx.x == 0) {
         for (int i = 1; i < kT / 64; ++i) s += sums[i], m += counts[i];
         const double f = mean ? 1.0 / (m > 0.0 ? m : 1.0) : 1.0;
-        loss[0] = (float)(s * f);
-        loss[1] = (float)f;
+        *loss = (float)(s * f);
+        *factor = (float)f;
     }
 }
 
@@ -548,7 +549,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
     const float lv = (v - vtop) * c, lr = (r - vtop) * c;
     const float L = log2_(wave_sum(lane < k ? exp2_(lv) : 0.f) + exp2_(lr));
     const float pi = lane < k ? exp2_(lv - L) : 0.f, pr = exp2_(lr - L);
-    const float gs = g[g_rows ? row : 0] * (factor != nullptr ? factor[1] : 1.f) * temp;
+    const float gs = g[g_rows ? row : 0] * (factor != nullptr ? *factor : 1.f) * temp;
     const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - pr);
     for (int a = t * VEC; a < C; a += U * NT * VEC) {
         uint4 raw[U];
@@ -709,7 +710,7 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
     float total = exp2_(lr);
     LIST_FOR(s) total += exp2_((list.value(s) - vtop) * c);
     const float L = log2_(total);
-    const float gs = g[g_rows ? row : 0] * (factor != nullptr ? factor[1] : 1.f) * temp;
+    const float gs = g[g_rows ? row : 0] * (factor != nullptr ? *factor : 1.f) * temp;
     const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - exp2_(lr - L));
     for (int c0 = 0; c0 < C; c0 += U) {
         float f[U];
@@ -793,9 +794,9 @@ static int row_threads(long rows, int classes) { return classes <= 2048 ? 64 : r
 
 extern "C" int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer, int classes, long inner, int k, const float* values,
                                   const int* indices, const float* rest, const unsigned char* mask, float temperature, int mean, float* stats,
-                                  float* row_loss, float* loss, double* partials, void* stream) {
+                                  float* row_loss, float* loss, float* factor, double* partials, void* stream) {
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && layout_ok(outer, classes, inner, ld) && k > 0 && k <= kMaxK && temperature > 0.f);
-    MSFWSI_CHECK_ARG(loss && partials);
+    MSFWSI_CHECK_ARG(loss && factor && partials && (reinterpret_cast<uintptr_t>(partials) & 7) == 0);
     long blocks = 0;
     if (outer > 0) {
         MSFWSI_CHECK_ARG(z && values && indices && stats && (reinterpret_cast<uintptr_t>(stats) & 15) == 0);
@@ -824,7 +825,8 @@ extern "C" int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer,
         const int rc = msfwsi_launch_status();
         if (rc != MSFWSI_OK) return rc;
     }
-    hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(kT), 0, ST(stream), partials, (int)blocks, mean, loss);
+    hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(kT), 0, ST(stream), partials, (int)blocks, mean, loss,
+                       factor);
     return msfwsi_launch_status();
 }
 

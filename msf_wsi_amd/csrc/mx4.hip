@@ -28,62 +28,104 @@ __device__ __forceinline__ float scale_value(unsigned E) {
     return __uint_as_float(E == 0 ? 0x00400000u : E == 255u ? 0x7fc00000u : E << 23);
 }
 
-__device__ __forceinline__ float code_value(unsigned c) {
-    const unsigned m = c & 7u;
-    const float v = m < 4 ? 0.5f * (float)m : m == 4 ? 2.f : m == 5 ? 3.f : m == 6 ? 4.f : 6.f;
-    return (c & 8u) ? -v : v;
-}
-
+// 8 elements of a row at any alignment, zeros past its end; `left` = elements from here to the end
+struct __attribute__((packed, aligned(2))) Unaligned16 {
+    unsigned x, y, z, w;
+};
 template <typename T>
 __device__ __forceinline__ void load8(const T* __restrict__ p, long left, float* f) {
+    if (left >= 8) {
+#pragma unroll
+        for (int i = 0; i < 8 / ElemTraits<T>::VEC; ++i) {
+            const Unaligned16 u = reinterpret_cast<const Unaligned16*>(p)[i];
+            unpack16<T>(make_uint4(u.x, u.y, u.z, u.w), f + i * ElemTraits<T>::VEC);
+        }
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = e < left ? load_elem<T>(p, e) : 0.f;
 }
-
-// One half-wave (32 lanes x 8 elements) per group of a row; a block of 32 elements is 4 lanes.  The conversion's own scale
-// operand stays 1: the elements are multiplied by 2^(127 - E) first, which is exact.
 template <typename T>
-__global__ void __launch_bounds__(kT) mx4_quantize_kernel(const T* __restrict__ x, long ld, long rows, long cols,
-                                                          unsigned* __restrict__ codes, unsigned* __restrict__ scales) {
-    const int l = threadIdx.x & 31;
-    const long r = blockIdx.x * (long)(kT / 32) + (threadIdx.x >> 5), g = blockIdx.y;
-    if (r >= rows) return;  // whole half-waves leave; the shuffles below stay inside a half
-    const long c = g * kGroup + l * 8;
-    float f[8];
-    load8<T>(x + r * ld + c, cols - c, f);
-    unsigned big = 0;
+__device__ __forceinline__ void store8(T* __restrict__ p, long left, const float* f) {
+    if (left >= 8) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(f[e]) & 0x7fffffffu);  // orders like the magnitudes, NaN on top
-    big = max(big, (unsigned)__shfl_xor((int)big, 1, 64));
-    big = max(big, (unsigned)__shfl_xor((int)big, 2, 64));
-    const unsigned field = big >> 23;
-    const unsigned E = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
-    const float up = __uint_as_float((254u - (E == 255u ? 127u : E)) << 23);  // 2^(127 - E)
-    unsigned w = 0;
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0] * up, f[1] * up, 1.f, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2] * up, f[3] * up, 1.f, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4] * up, f[5] * up, 1.f, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6] * up, f[7] * up, 1.f, 3);
-    if (E == 255u) w = 0;
-    codes[(g * rows + r) * 32 + l] = w;
-    unsigned word = 0;  // lane 0 / 1 collects the scale bytes of blocks 0-3 / 4-7
-#pragma unroll
-    for (int j = 0; j < 4; ++j) word |= (unsigned)__shfl((int)E, (threadIdx.x & 32) + (l & 1) * 16 + j * 4, 64) << (8 * j);
-    if (l < 2) scales[(g * rows + r) * 2 + l] = word;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kT) mx4_dequantize_kernel(const unsigned* __restrict__ codes, const unsigned char* __restrict__ scales,
-                                                            long rows, long cols, T* __restrict__ y) {
-    const int l = threadIdx.x & 31;
-    const long r = blockIdx.x * (long)(kT / 32) + (threadIdx.x >> 5), g = blockIdx.y;
-    if (r >= rows) return;
-    const long c = g * kGroup + l * 8;
-    const unsigned w = codes[(g * rows + r) * 32 + l];
-    const float s = scale_value(scales[(g * rows + r) * 8 + (l >> 2)]);
+        for (int i = 0; i < 8 / ElemTraits<T>::VEC; ++i) {
+            const uint4 v = pack16<T>(f + i * ElemTraits<T>::VEC);
+            reinterpret_cast<Unaligned16*>(p)[i] = {v.x, v.y, v.z, v.w};
+        }
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-        if (c + e < cols) store_elem<T>(y, r * cols + c + e, code_value(w >> (4 * e)) * s);
+        if (e < left) store_elem<T>(p, e, f[e]);
+}
+
+// One half-wave (32 lanes x 8 elements) per group of a row, UG groups one after the other with their loads in flight together; a
+// block of 32 elements is 4 lanes.  The conversion's own scale operand stays 1: the elements are multiplied by 2^(127 - E) first,
+// which is exact.  Bound by memory.
+constexpr int UG = 4;
+template <typename T>
+__global__ void __launch_bounds__(kT) mx4_quantize_kernel(const T* __restrict__ x, long ld, long rows, long cols, int G,
+                                                          unsigned* __restrict__ codes, unsigned* __restrict__ scales) {
+    const int l = threadIdx.x & 31, g0 = blockIdx.y * UG;
+    const long r = blockIdx.x * (long)(kT / 32) + (threadIdx.x >> 5);
+    if (r >= rows) return;  // whole half-waves leave; the shuffles below stay inside a half
+    float f[UG][8];
+#pragma unroll
+    for (int u = 0; u < UG; ++u) {
+        const long c = (g0 + u) * (long)kGroup + l * 8;
+        load8<T>(x + r * ld + c, cols - c, f[u]);  // nothing is read of a group past the last
+    }
+#pragma unroll
+    for (int u = 0; u < UG; ++u) {
+        if (g0 + u >= G) return;
+        const long at = (long)(g0 + u) * rows + r;
+        unsigned big = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(f[u][e]) & 0x7fffffffu);  // orders like the magnitudes, NaN on top
+        big = max(big, (unsigned)__shfl_xor((int)big, 1, 64));
+        big = max(big, (unsigned)__shfl_xor((int)big, 2, 64));
+        const unsigned field = big >> 23;
+        const unsigned E = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
+        const float up = __uint_as_float((254u - (E == 255u ? 127u : E)) << 23);  // 2^(127 - E)
+        unsigned w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][0] * up, f[u][1] * up, 1.f, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][2] * up, f[u][3] * up, 1.f, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][4] * up, f[u][5] * up, 1.f, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][6] * up, f[u][7] * up, 1.f, 3);
+        codes[at * 32 + l] = E == 255u ? 0u : w;
+        unsigned word = 0;  // lane 0 / 1 collects the scale bytes of blocks 0-3 / 4-7
+#pragma unroll
+        for (int j = 0; j < 4; ++j) word |= (unsigned)__shfl((int)E, (threadIdx.x & 32) + (l & 1) * 16 + j * 4, 64) << (8 * j);
+        if (l < 2) scales[at * 2 + l] = word;
+    }
+}
+
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+template <typename T>
+__global__ void __launch_bounds__(kT) mx4_dequantize_kernel(const unsigned* __restrict__ codes, const unsigned char* __restrict__ scales,
+                                                            long rows, long cols, int G, T* __restrict__ y) {
+    const int l = threadIdx.x & 31, g0 = blockIdx.y * UG;
+    const long r = blockIdx.x * (long)(kT / 32) + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    unsigned w[UG], E[UG];
+#pragma unroll
+    for (int u = 0; u < UG; ++u) {
+        const long at = (long)min(g0 + u, G - 1) * rows + r;
+        w[u] = codes[at * 32 + l];
+        E[u] = scales[at * 8 + (l >> 2)];
+    }
+#pragma unroll
+    for (int u = 0; u < UG; ++u) {
+        if (g0 + u >= G) return;
+        const long c = (g0 + u) * (long)kGroup + l * 8;
+        const float s = scale_value(E[u]);
+        float f[8];
+        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.f, 1);
+        const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.f, 2), e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.f, 3);
+        f[0] = a.x * s, f[1] = a.y * s, f[2] = b.x * s, f[3] = b.y * s, f[4] = d.x * s, f[5] = d.y * s, f[6] = e.x * s, f[7] = e.y * s;
+        store8<T>(y + r * cols + c, cols - c, f);
+    }
 }
 
 // One 32x32x64 step takes 32 elements of row (lane & 31) of either operand from each lane.  Which 32 is free as long as both
@@ -286,17 +328,24 @@ __global__ void __launch_bounds__(WM* WN * 64) mx4_tile_kernel(const GemmArgs p)
         add[0] = p.bias[n0 + n];
         if (left > 1) add[1] = p.bias[n0 + n + 1];
     }
-    float* part = p.sums + ((long)split * p.M + m0) * p.N + n0;
-    T* out = (T*)p.y + m0 * p.N + n0;
+    auto put = [&](auto* to, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int m = r0 + i * 32 + (e & 3) + 8 * (e >> 2);
-            if (m >= mrows) continue;
-            if (p.sums != nullptr) store_two<float>(part, (unsigned)(m * N + n), acc[i][0][e], acc[i][1][e], left > 1);
-            else store_two<T>(out, (unsigned)(m * N + n), acc[i][0][e] + add[0], acc[i][1][e] + add[1], left > 1);
-        }
+            for (int e = 0; e < 16; ++e) {
+                const int m = r0 + i * 32 + (e & 3) + 8 * (e >> 2);
+                if (WHOLE || m < mrows) store_two(to, (unsigned)(m * N + n), acc[i][0][e] + add[0], acc[i][1][e] + add[1], WHOLE || left > 1);
+            }
+    };
+    const bool whole = mrows == TM && nrows == TN;
+    if (p.sums != nullptr) {
+        float* part = p.sums + ((long)split * p.M + m0) * p.N + n0;
+        whole ? put(part, std::true_type()) : put(part, std::false_type());
+    } else {
+        T* out = (T*)p.y + m0 * p.N + n0;
+        whole ? put(out, std::true_type()) : put(out, std::false_type());
+    }
 }
 
 // y = the sum of `splits` fp32 partial results (+ bias of the column)
@@ -368,6 +417,8 @@ template <typename T>
 __device__ __forceinline__ uint4 widen8(unsigned codes, float scale) {
     return make_uint4(widen2<T, 0>(codes, scale), widen2<T, 1>(codes, scale), widen2<T, 2>(codes, scale), widen2<T, 3>(codes, scale));
 }
+
+typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
 
 struct DgradArgs {
     const unsigned char *dy, *codes, *scales;
@@ -495,20 +546,33 @@ __global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
     if (t < 8) emax[t] = 0, emin[t] = 255;
     __syncthreads();
     {
-        int hi[8], lo[8];
+        // two scale bytes per word.  E + 1 and E - 1 modulo 256 leave NaN (255) out of the largest, and E = 0 -- zeros, in all but the
+        // smallest of weights -- out of the smallest
+        u16x2 hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) hi[i] = 0, lo[i] = 255;
+        for (int i = 0; i < 4; ++i) hi[i] = 0, lo[i] = 255;
         for (long n = t; n < p.N; n += 512) {
             const uint2 v = *reinterpret_cast<const uint2*>(p.scales + (g * p.N + n) * 8);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int x = ((i < 4 ? v.x : v.y) >> (8 * (i & 3))) & 255;
-                hi[i] = max(hi[i], x == 255 ? 0 : x);
-                lo[i] = min(lo[i], x == 0 ? 255 : x);  // E = 0 stands for zeros in all but the smallest of weights
+            for (int i = 0; i < 4; ++i) {
+                const unsigned x = ((i < 2 ? v.x : v.y) >> (8 * (i & 1))) & 0x00ff00ffu;
+                hi[i] = __builtin_elementwise_max(hi[i], __builtin_bit_cast(u16x2, (x + 0x00010001u) & 0x00ff00ffu));
+                lo[i] = __builtin_elementwise_min(lo[i], __builtin_bit_cast(u16x2, (x + 0x00ff00ffu) & 0x00ff00ffu));
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) atomicMax(&emax[i], hi[i]), atomicMin(&emin[i], lo[i]);
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) {
+                hi[i] = __builtin_elementwise_max(hi[i], __builtin_bit_cast(u16x2, __shfl_xor(__builtin_bit_cast(int, hi[i]), off, 64)));
+                lo[i] = __builtin_elementwise_min(lo[i], __builtin_bit_cast(u16x2, __shfl_xor(__builtin_bit_cast(int, lo[i]), off, 64)));
+            }
+            const int b = (i >> 1) * 4 + (i & 1);  // bytes b and b + 2
+            if (lane == 0) {
+                atomicMax(&emax[b], max((int)hi[i].x, 1) - 1), atomicMax(&emax[b + 2], max((int)hi[i].y, 1) - 1);
+                atomicMin(&emin[b], lo[i].x + 1), atomicMin(&emin[b + 2], lo[i].y + 1);
+            }
+        }
     }
     __syncthreads();
     f32x16 acc[4][2];
@@ -535,18 +599,25 @@ __global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
     const int mrows = (int)min(256L, p.M - m0), r0 = wm * 128 + 4 * h, cols = (int)p.cols;
     if (left <= 0) return;
     const int up = emax[kc >> 5] - bias;
-    float* part = p.sums + ((long)blockIdx.y * p.M + m0) * p.cols + k0;
-    TO* out = (TO*)p.dx + m0 * p.cols + k0;
+    auto put = [&](auto* to, auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int m = r0 + i * 32 + (e & 3) + 8 * (e >> 2);  // 32 bits hold the offsets: cols is at most 2^21
-            if (m >= mrows) continue;
-            const float v0 = ldexpf(acc[i][0][e], up), v1 = ldexpf(acc[i][1][e], up);
-            if (p.sums != nullptr) store_two<float>(part, (unsigned)(m * cols + kc), v0, v1, left > 1);
-            else store_two<TO>(out, (unsigned)(m * cols + kc), v0, v1, left > 1);
-        }
+            for (int e = 0; e < 16; ++e) {
+                const int m = r0 + i * 32 + (e & 3) + 8 * (e >> 2);  // 32 bits hold the offsets: cols is at most 2^21
+                if (WHOLE || m < mrows)
+                    store_two(to, (unsigned)(m * cols + kc), ldexpf(acc[i][0][e], up), ldexpf(acc[i][1][e], up), WHOLE || left > 1);
+            }
+    };
+    const bool whole = mrows == 256 && p.cols - k0 >= 256;
+    if (p.sums != nullptr) {
+        float* part = p.sums + ((long)blockIdx.y * p.M + m0) * p.cols + k0;
+        whole ? put(part, std::true_type()) : put(part, std::false_type());
+    } else {
+        TO* out = (TO*)p.dx + m0 * p.cols + k0;
+        whole ? put(out, std::true_type()) : put(out, std::false_type());
+    }
 }
 
 long groups_of(long cols) { return (cols + kGroup - 1) / kGroup; }
@@ -591,7 +662,7 @@ DgradPlan dgrad_plan(int dtype, const void* dy, long ld, long M, long N, long co
     const long tiles = p.mt * p.kt;
     if (tiles < kCus) {
         long s = kCus / tiles;
-        if (s > p.steps / 8) s = p.steps / 8;
+        if (s > p.steps / 2) s = p.steps / 2;
         if (s > 1) {
             p.per_split = (int)((p.steps + s - 1) / s);
             p.splits = (p.steps + p.per_split - 1) / p.per_split;
@@ -614,9 +685,9 @@ extern "C" int msfwsi_mx4_quantize(int dtype, const void* x, long ld, long rows,
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && rows >= 0 && cols > 0 && (rows <= 1 || ld >= cols));
     if (rows == 0) return MSFWSI_OK;
     const long G = groups_of(cols);
-    MSFWSI_CHECK_ARG(x && codes && scales && aligned16(codes) && aligned16(scales) && G <= 65535 && grid_ok((rows + 7) / 8));
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_quantize_kernel<T>, dim3((unsigned)((rows + 7) / 8), (unsigned)G), dim3(kT), 0, ST(stream),
-                                            (const T*)x, ld, rows, cols, (unsigned*)codes, (unsigned*)scales));
+    MSFWSI_CHECK_ARG(x && codes && scales && aligned16(codes) && aligned16(scales) && G <= 65535L * UG && grid_ok((rows + 7) / 8));
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_quantize_kernel<T>, dim3((unsigned)((rows + 7) / 8), (unsigned)((G + UG - 1) / UG)), dim3(kT), 0,
+                                            ST(stream), (const T*)x, ld, rows, cols, (int)G, (unsigned*)codes, (unsigned*)scales));
     return msfwsi_launch_status();
 }
 
@@ -624,9 +695,9 @@ extern "C" int msfwsi_mx4_dequantize(int dtype, const void* codes, const void* s
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && rows >= 0 && cols > 0);
     if (rows == 0) return MSFWSI_OK;
     const long G = groups_of(cols);
-    MSFWSI_CHECK_ARG(y && codes && scales && aligned16(codes) && aligned16(scales) && G <= 65535 && grid_ok((rows + 7) / 8));
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_dequantize_kernel<T>, dim3((unsigned)((rows + 7) / 8), (unsigned)G), dim3(kT), 0, ST(stream),
-                                            (const unsigned*)codes, (const unsigned char*)scales, rows, cols, (T*)y));
+    MSFWSI_CHECK_ARG(y && codes && scales && aligned16(codes) && aligned16(scales) && G <= 65535L * UG && grid_ok((rows + 7) / 8));
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_dequantize_kernel<T>, dim3((unsigned)((rows + 7) / 8), (unsigned)((G + UG - 1) / UG)), dim3(kT), 0,
+                                            ST(stream), (const unsigned*)codes, (const unsigned char*)scales, rows, cols, (int)G, (T*)y));
     return msfwsi_launch_status();
 }
 
@@ -667,6 +738,25 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
     if (rc != MSFWSI_OK || p.splits == 1) return rc;
     MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_join_kernel<T>, dim3(stride_grid(M * N)), dim3(kT), 0, ST(stream), sums, p.splits, M * N, N, bias, (T*)y));
     return msfwsi_launch_status();
+}
+
+// workspace of a linear call: x's codes, its scales, the partial sums
+extern "C" int msfwsi_mx4_linear_workspace(long M, long N, long cols, long* bytes) {
+    const int rc = msfwsi_mx4_gemm_workspace(M, N, cols, bytes);
+    if (rc == MSFWSI_OK) *bytes += groups_of(cols) * M * kGroupBytes + round16(groups_of(cols) * M * 8);
+    return rc;
+}
+
+extern "C" int msfwsi_mx4_linear(int dtype, const void* x, long ld, long M, const void* codes, const void* scales, long N, long cols,
+                                 const float* bias, int y_dtype, void* y, void* workspace, void* stream) {
+    MSFWSI_CHECK_ARG(msfwsi_dtype_ok(y_dtype) && M >= 0 && N > 0 && cols > 0);
+    if (M == 0) return MSFWSI_OK;
+    MSFWSI_CHECK_ARG(codes && scales && y && workspace && aligned16(workspace));
+    char* xc = (char*)workspace;
+    char* xs = xc + groups_of(cols) * M * kGroupBytes;
+    const int rc = msfwsi_mx4_quantize(dtype, x, ld, M, cols, xc, xs, stream);
+    if (rc != MSFWSI_OK) return rc;
+    return msfwsi_mx4_gemm(y_dtype, xc, xs, M, codes, scales, N, cols, bias, y, xs + round16(groups_of(cols) * M * 8), stream);
 }
 
 extern "C" int msfwsi_mx4_dgrad_workspace(int dy_dtype, const void* dy, long ld, long M, long N, long cols, long* bytes) {

@@ -1670,191 +1670,210 @@ def dice_loss(logits, target, C1: int, classes, weight: float, loss_accum, dlogi
 
 
 # ------------------------------------------------------------------------------------------------
-# frozen-teacher operators (csrc/mx4.hip, csrc/distill.hip).  Each wrapper launches on the current stream of the
-# operands' own device, whichever device is current.
+# frozen-teacher operators (csrc/mx4.hip, csrc/distill.hip).  Each wrapper launches on the current stream of its first
+# operand's device, whichever device is current; the small calls are bound by the host, so the checks are kept lean.
 MX4_GROUP = 256  # elements of a row stored together: 128 code bytes, 8 scale bytes
+TOP_LOGITS_MAX_K = 64
+_DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
 
 
-def _one_device(ref, *others):
-    for t in others:
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"operands on {ref.device} and {t.device}")
+def _call(what: str, dev: int, *args):
+    """one entry point on the current stream of device `dev`"""
+    fn = getattr(_lib.load(), "msfwsi_" + what)
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
+
+
+def _workspace(what: str, dev: torch.device, *args):
+    """scratch memory of the size that entry point `what` asks for, or None"""
+    need = C.c_long()
+    _lib.check(getattr(_lib.load(), "msfwsi_" + what)(*args, C.byref(need)), what)
+    return torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+
+
+def _gpu(t, name) -> int:
+    if not t.is_cuda:
+        raise _lib.MsfwsiHipError(f"{name}: expected a GPU tensor (no CPU path exists)")
+    return t.get_device()
+
+
+def _dense(t, name, dtype, numel, dev):
+    """contiguous on device `dev`, of any alignment (slices of a batch): what is read element by element"""
+    if t.get_device() != dev:
+        _gpu(t, name)
+        raise ValueError(f"{name}: on device {t.get_device()}, the other operands are on {dev}")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.numel() != numel:
+        raise ValueError(f"{name}: expected {numel} elements, got {t.numel()}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: must be contiguous")
+    return t.data_ptr()
+
+
+def _aligned(t, name, dtype, numel, dev):
+    ptr = _dense(t, name, dtype, numel, dev)
+    if ptr % 16 and numel:
+        raise ValueError(f"{name}: must be 16-byte aligned")
+    return ptr
+
+
+def _float(t, name) -> int:
+    code = _DT.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name}: unsupported dtype {t.dtype}")
+    return code
 
 
 def _rows2d(t, name):
     """[rows, cols] with unit column stride: the row pitch in elements (rows may be slices of a wider tensor)"""
-    if not t.is_cuda:
-        raise _lib.MsfwsiHipError(f"{name}: expected a GPU tensor (no CPU path exists)")
     if t.dim() != 2:
         raise ValueError(f"{name}: expected [rows, cols], got {tuple(t.shape)}")
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    row, col = t.stride()
+    if cols > 1 and col != 1:
         raise ValueError(f"{name}: the elements of a row must be adjacent")
-    ld = t.stride(0) if rows > 1 else cols
-    if ld < cols:
+    if rows <= 1:
+        row = cols
+    if row < cols:
         raise ValueError(f"{name}: rows overlap")
-    return rows, cols, ld
+    return rows, cols, row
 
 
-def _dense(t, name, dtype, numel):
-    """contiguous, of any alignment (slices of a batch): for operands that are read element by element"""
-    if not t.is_cuda:
-        raise _lib.MsfwsiHipError(f"{name}: expected a GPU tensor (no CPU path exists)")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: must be contiguous")
-    if t.dtype != dtype:
-        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.numel() != numel:
-        raise ValueError(f"{name}: expected {numel} elements, got {t.numel()}")
-
-
-def _mx4_shape(codes, scales, cols, name):
-    if not codes.is_cuda:
-        raise _lib.MsfwsiHipError(f"{name}: expected GPU tensors (no CPU path exists)")
-    G = (int(cols) + MX4_GROUP - 1) // MX4_GROUP
+def _mx4(codes, scales, cols: int, name, dev):
+    """checks 4-bit storage of [rows, cols]; (rows, address of the codes, of the scales)"""
+    G = (cols + MX4_GROUP - 1) // MX4_GROUP
     if cols < 1 or codes.dim() != 3 or codes.shape[0] != G or codes.shape[2] != MX4_GROUP // 2:
         raise ValueError(f"{name}: codes of {cols} columns must be [{G}, rows, 128], got {tuple(codes.shape)}")
     rows = codes.shape[1]
-    _req(codes, name + ".codes", torch.uint8, G * rows * 128)
-    _req(scales, name + ".scales", torch.uint8, G * rows * 8)
-    _one_device(codes, scales)
-    return rows
+    return (rows, _aligned(codes, name + ".codes", torch.uint8, G * rows * 128, dev),
+            _aligned(scales, name + ".scales", torch.uint8, G * rows * 8, dev))
 
 
 def mx4_quantize(x, codes, scales):
     """x [rows, cols] (any row pitch) -> 4-bit codes [G, rows, 128] and scales [G, rows, 8]"""
-    lib = _lib.load()
+    dev = _gpu(x, "x")
     rows, cols, ld = _rows2d(x, "x")
-    if _mx4_shape(codes, scales, cols, "out") != rows:
-        raise ValueError(f"out holds {codes.shape[1]} rows, x {rows}")
-    _one_device(x, codes)
-    with torch.cuda.device(x.device):
-        _lib.check(lib.msfwsi_mx4_quantize(dt_of(x), _p(x), ld, rows, cols, _p(codes), _p(scales), _stream()), "mx4_quantize")
+    held, cp, sp = _mx4(codes, scales, cols, "out", dev)
+    if held != rows:
+        raise ValueError(f"out holds {held} rows, x {rows}")
+    _call("mx4_quantize", dev, _float(x, "x"), x.data_ptr(), ld, rows, cols, cp, sp)
 
 
 def mx4_dequantize(codes, scales, y):
     """y [rows, cols] contiguous <- the values the codes stand for"""
-    lib = _lib.load()
+    dev = _gpu(y, "y")
     rows, cols = y.shape
-    if _mx4_shape(codes, scales, cols, "x") != rows:
-        raise ValueError(f"y has {rows} rows, x {codes.shape[1]}")
-    _req(y, "y")
-    _one_device(y, codes)
-    with torch.cuda.device(y.device):
-        _lib.check(lib.msfwsi_mx4_dequantize(dt_of(y), _p(codes), _p(scales), rows, cols, _p(y), _stream()), "mx4_dequantize")
+    held, cp, sp = _mx4(codes, scales, cols, "x", dev)
+    if held != rows:
+        raise ValueError(f"y has {rows} rows, x {held}")
+    _call("mx4_dequantize", dev, _float(y, "y"), cp, sp, rows, cols, _aligned(y, "y", y.dtype, rows * cols, dev))
 
 
 def mx4_gemm(a_codes, a_scales, b_codes, b_scales, cols: int, y, bias=None):
     """y [M, N] = a b^T (+ bias fp32 [N]) of two 4-bit operands with `cols` columns"""
-    lib = _lib.load()
-    M = _mx4_shape(a_codes, a_scales, cols, "a")
-    N = _mx4_shape(b_codes, b_scales, cols, "b")
+    dev = _gpu(y, "y")
+    M, ac, as_ = _mx4(a_codes, a_scales, cols, "a", dev)
+    N, bc, bs = _mx4(b_codes, b_scales, cols, "b", dev)
     if N == 0:
         raise ValueError("b has no rows")
-    _req(y, "y", numel=M * N)
-    if bias is not None:
-        _dense(bias, "bias", torch.float32, N)
-    _one_device(y, a_codes, b_codes, bias)
-    need = C.c_long()
-    _lib.check(lib.msfwsi_mx4_gemm_workspace(M, N, int(cols), C.byref(need)), "mx4_gemm_workspace")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=y.device) if need.value else None
-    with torch.cuda.device(y.device):
-        _lib.check(lib.msfwsi_mx4_gemm(dt_of(y), _p(a_codes), _p(a_scales), M, _p(b_codes), _p(b_scales), N, int(cols), _p(bias), _p(y),
-                                       _p(ws), _stream()), "mx4_gemm")
+    yp = _dense(y, "y", y.dtype, M * N, dev)
+    bp = None if bias is None else _dense(bias, "bias", torch.float32, N, dev)
+    ws = _workspace("mx4_gemm_workspace", y.device, M, N, cols)
+    _call("mx4_gemm", dev, _float(y, "y"), ac, as_, M, bc, bs, N, cols, bp, yp, _p(ws))
+    return y
+
+
+def mx4_linear(x, codes, scales, y, bias=None):
+    """y [M, N] = Q(x) w^T (+ bias fp32 [N]): x [M, cols] (any row pitch) quantised on the way in, w [N, cols] 4-bit"""
+    dev = _gpu(x, "x")
+    M, cols, ld = _rows2d(x, "x")
+    N, cp, sp = _mx4(codes, scales, cols, "w", dev)
+    if N == 0:
+        raise ValueError("w has no rows")
+    yp = _dense(y, "y", y.dtype, M * N, dev)
+    bp = None if bias is None else _dense(bias, "bias", torch.float32, N, dev)
+    ws = _workspace("mx4_linear_workspace", x.device, M, N, cols)
+    _call("mx4_linear", dev, _float(x, "x"), x.data_ptr(), ld, M, cp, sp, N, cols, bp, _float(y, "y"), yp, _p(ws))
     return y
 
 
 def mx4_dgrad(dy, codes, scales, dx):
     """dx [M, cols] contiguous = dy [M, N] (any row pitch) times a 4-bit weight [N, cols]"""
-    lib = _lib.load()
+    dev = _gpu(dy, "dy")
     M, N, ld = _rows2d(dy, "dy")
-    if _mx4_shape(codes, scales, dx.shape[1], "w") != N or N == 0:
-        raise ValueError(f"dy has {N} columns, w {codes.shape[1]} rows")
-    _req(dx, "dx", numel=M * dx.shape[1])
-    _one_device(dy, codes, dx)
-    need = C.c_long()
-    _lib.check(lib.msfwsi_mx4_dgrad_workspace(dt_of(dy), _p(dy), ld, M, N, dx.shape[1], C.byref(need)), "mx4_dgrad_workspace")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dy.device) if need.value else None
-    with torch.cuda.device(dy.device):
-        _lib.check(lib.msfwsi_mx4_dgrad(dt_of(dy), _p(dy), ld, M, _p(codes), _p(scales), N, dx.shape[1], dt_of(dx), _p(dx), _p(ws),
-                                        _stream()), "mx4_dgrad")
+    cols = dx.shape[1]
+    held, cp, sp = _mx4(codes, scales, cols, "w", dev)
+    if held != N or N == 0:
+        raise ValueError(f"dy has {N} columns, w {held} rows")
+    dt, dp = _float(dy, "dy"), dy.data_ptr()
+    xp = _dense(dx, "dx", dx.dtype, M * cols, dev)
+    ws = _workspace("mx4_dgrad_workspace", dy.device, dt, dp, ld, M, N, cols)
+    _call("mx4_dgrad", dev, dt, dp, ld, M, cp, sp, N, cols, _float(dx, "dx"), xp, _p(ws))
     return dx
-
-
-TOP_LOGITS_MAX_K = 64
 
 
 def _logit_layout(z, name):
     """[rows, C] (any row pitch) or contiguous [N, C, inner]: (outer, classes, inner, ld)"""
-    if z.dim() == 2:
+    if z.dim() != 3:
         rows, Cn, ld = _rows2d(z, name)
         return rows, Cn, 1, ld
-    if z.dim() != 3:
-        raise ValueError(f"{name}: expected [rows, classes] or [N, classes, positions], got {tuple(z.shape)}")
-    if not z.is_cuda:
-        raise _lib.MsfwsiHipError(f"{name}: expected a GPU tensor (no CPU path exists)")
     if not z.is_contiguous():
         raise ValueError(f"{name}: must be contiguous")
-    if z.shape[2] == 0:
-        return 0, z.shape[1], 1, z.shape[1]
-    return z.shape[0], z.shape[1], z.shape[2], z.shape[1] * z.shape[2]
+    N, Cn, inner = z.shape
+    return (N, Cn, inner, Cn * inner) if inner else (0, Cn, 1, Cn)
 
 
-def _top_args(values, indices, rest, outer, inner, k):
-    _dense(values, "values", torch.float32, outer * k * inner)
-    _dense(indices, "indices", torch.int32, outer * k * inner)
-    if rest is not None:
-        _dense(rest, "rest", torch.float32, outer * inner)
+def _list_args(values, indices, rest, outer, inner, k, dev):
+    return (_dense(values, "values", torch.float32, outer * k * inner, dev), _dense(indices, "indices", torch.int32, outer * k * inner, dev),
+            None if rest is None else _dense(rest, "rest", torch.float32, outer * inner, dev))
 
 
 def top_logits(x, k: int, temperature: float, values, indices, rest):
     """the k largest logits (values, indices [outer, k, inner]) and the log-sum-exp of the others (rest [outer * inner])"""
-    lib = _lib.load()
+    dev = _gpu(x, "x")
     outer, Cn, inner, ld = _logit_layout(x, "x")
-    _top_args(values, indices, rest, outer, inner, k)
-    _one_device(x, values, indices, rest)
-    need = C.c_long()
-    _lib.check(lib.msfwsi_top_logits_workspace(dt_of(x), outer, Cn, inner, int(k), C.byref(need)), "top_logits_workspace")
-    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
-    with torch.cuda.device(x.device):
-        _lib.check(lib.msfwsi_top_logits(dt_of(x), _p(x), ld, outer, Cn, inner, int(k), 1.0 / temperature, _p(values), _p(indices), _p(rest),
-                                         _p(ws), _stream()), "top_logits")
+    dt = _float(x, "x")
+    args = _list_args(values, indices, rest, outer, inner, k, dev)
+    ws = _workspace("top_logits_workspace", x.device, dt, outer, Cn, inner, k)
+    _call("top_logits", dev, dt, x.data_ptr(), ld, outer, Cn, inner, k, 1.0 / temperature, *args, _p(ws))
+
+
+_PARTS = 2048 * 2 * 8  # bytes of msfwsi_distill_fwd's partials
 
 
 def distill_fwd(z, values, indices, rest, mask, k: int, temperature: float, mean: bool, per_row: bool = True):
-    """(row_loss [rows] or None, loss fp32[2] = (sum or mean, gradient factor), stats [rows, 4] for distill_bwd)"""
-    lib = _lib.load()
+    """(row_loss [rows] or None, loss = sum or mean over the rows that count, saved: what distill_bwd needs)"""
+    dev = _gpu(z, "z")
     outer, Cn, inner, ld = _logit_layout(z, "z")
-    _top_args(values, indices, rest, outer, inner, k)
+    args = _list_args(values, indices, rest, outer, inner, k, dev)
     rows = outer * inner
-    if mask is not None:
-        _dense(mask, "mask", torch.bool, rows)
-    _one_device(z, values, indices, rest, mask)
-    stats = torch.empty(rows, 4, dtype=torch.float32, device=z.device)
+    mp = None if mask is None else _dense(mask, "mask", torch.bool, rows, dev)
+    saved = torch.empty(rows * 4 + 4 + _PARTS // 4, dtype=torch.float32, device=z.device)  # stats, the factor, scratch
     row_loss = torch.empty(rows, dtype=torch.float32, device=z.device) if per_row else None
-    loss = torch.empty(2, dtype=torch.float32, device=z.device)
-    partials = torch.empty(2, 2048, dtype=torch.float64, device=z.device)
-    with torch.cuda.device(z.device):
-        _lib.check(lib.msfwsi_distill_fwd(dt_of(z), _p(z), ld, outer, Cn, inner, int(k), _p(values), _p(indices), _p(rest), _p(mask),
-                                          float(temperature), int(bool(mean)), _p(stats), _p(row_loss), _p(loss), _p(partials), _stream()),
-                   "distill_fwd")
-    return row_loss, loss, stats
+    loss = torch.empty((), dtype=torch.float32, device=z.device)
+    sp = saved.data_ptr()
+    _call("distill_fwd", dev, _float(z, "z"), z.data_ptr(), ld, outer, Cn, inner, k, *args, mp, temperature, int(mean), sp, _p(row_loss),
+          loss.data_ptr(), sp + rows * 16, sp + rows * 16 + 16)
+    return row_loss, loss, saved
 
 
-def distill_bwd(z, values, indices, rest, k: int, temperature: float, stats, factor, g, dz):
-    """dz (contiguous, z's shape) = g (one value, or one per row) * factor[1] * d row_loss / dz"""
-    lib = _lib.load()
+def distill_bwd(z, values, indices, rest, k: int, temperature: float, saved, mean: bool, g, dz):
+    """dz (contiguous, z's shape) = g (one value, or one per row; over the number of rows that count for the mean) * d row_loss / dz"""
+    dev = _gpu(z, "z")
     outer, Cn, inner, ld = _logit_layout(z, "z")
-    _top_args(values, indices, rest, outer, inner, k)
-    rows = outer * inner
-    _req(stats, "stats", torch.float32, rows * 4)
-    _opt(factor, "factor", torch.float32, 2)
-    if g.numel() not in (1, rows):
-        raise ValueError(f"g: expected 1 or {rows} values, got {g.numel()}")
-    _dense(g, "g", torch.float32, g.numel())
-    _req(dz, "dz", z.dtype, z.numel())
-    _one_device(z, values, indices, rest, stats, factor, g, dz)
-    with torch.cuda.device(z.device):
-        _lib.check(lib.msfwsi_distill_bwd(dt_of(z), _p(z), ld, outer, Cn, inner, int(k), _p(values), _p(indices), _p(rest), float(temperature),
-                                          _p(stats), _p(factor), _p(g), int(g.numel() != 1), _p(dz), _stream()), "distill_bwd")
+    args = _list_args(values, indices, rest, outer, inner, k, dev)
+    rows, n = outer * inner, g.numel()
+    sp = _aligned(saved, "saved", torch.float32, rows * 4 + 4 + _PARTS // 4, dev)
+    if n not in (1, rows):
+        raise ValueError(f"g: expected 1 or {rows} values, got {n}")
+    gp = _dense(g, "g", torch.float32, n, dev)
+    _call("distill_bwd", dev, _float(z, "z"), z.data_ptr(), ld, outer, Cn, inner, k, *args, temperature, sp, sp + rows * 16 if mean else None,
+          gp, int(n != 1), _dense(dz, "dz", z.dtype, z.numel(), dev))
     return dz

@@ -74,31 +74,34 @@ class TopLogits(NamedTuple):
     rest: Optional[torch.Tensor] = None
 
 
-def _class_last(t: torch.Tensor, dim: int) -> torch.Tensor:
-    return t if dim == t.dim() - 1 else t.movedim(dim, -1)
-
-
-def _logit_view(logits: torch.Tensor, dim: int, what: str):
-    """(logits as [rows, C] or [N, C, positions], dim >= 0): rows where the classes are adjacent in memory (also a
-    channels-last map), maps where the positions are"""
-    if not logits.is_cuda:
-        raise _lib.MsfwsiHipError(f"{what} runs only on a HIP device (no CPU path)")
-    kn.dt_of(logits)
+def _class_dim(logits: torch.Tensor, dim: int, what: str) -> int:
+    """dim >= 0 of the classes: the last dimension, or 1"""
+    kn._gpu(logits, what)
+    kn._float(logits, what)
     nd = logits.dim()
     if nd == 0 or not -nd <= dim < nd:
         raise ValueError(f"{what}: no dimension {dim} in {tuple(logits.shape)}")
     dim = dim % nd
-    if dim not in (nd - 1, 1):
+    if dim != nd - 1 and dim != 1:
         raise ValueError(f"{what}: the class dimension must be the last one or dimension 1")
     if logits.shape[dim] == 0:
         raise ValueError(f"{what}: no classes in {tuple(logits.shape)}")
-    last = _class_last(logits, dim)
-    if dim == nd - 1 or last.is_contiguous():
+    return dim
+
+
+def _logit_view(logits: torch.Tensor, dim: int) -> torch.Tensor:
+    """[rows, C] where the classes are adjacent in memory (also a channels-last map), else [N, C, positions]"""
+    nd = logits.dim()
+    if dim == nd - 1:
+        rows = logits if nd == 2 else logits.reshape(-1, logits.shape[-1])
+    else:
+        last = logits.movedim(dim, -1)
+        if not last.is_contiguous():
+            return logits.contiguous().flatten(2)
         rows = last.reshape(-1, last.shape[-1])
-        if (rows.shape[1] > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1]):
-            rows = rows.contiguous()
-        return rows, dim
-    return logits.contiguous().flatten(2), dim
+    if not rows.is_contiguous() and ((rows.shape[1] > 1 and rows.stride(1) != 1) or (rows.shape[0] > 1 and rows.stride(0) < rows.shape[1])):
+        rows = rows.contiguous()
+    return rows
 
 
 def _temperature(t: float) -> float:
@@ -112,7 +115,8 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, dim: int 
     """The k largest logits along `dim` (the last dimension, or 1 as in segmentation maps [N, C, H, W]) of a frozen teacher:
     descending, equal ones by ascending class index, NaN above every number.  k <= 64; not differentiable.  `rest` is taken
     at `temperature`, the one the loss will run at."""
-    view, dim = _logit_view(logits.detach(), dim, "top_logits")
+    dim = _class_dim(logits, dim, "top_logits")
+    view = _logit_view(logits.detach(), dim)
     t, k = _temperature(temperature), int(k)
     if not 1 <= k <= min(kn.TOP_LOGITS_MAX_K, view.shape[1]):
         raise ValueError(f"top_logits: k = {k} outside 1 ... {min(kn.TOP_LOGITS_MAX_K, view.shape[1])}")
@@ -132,28 +136,40 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, dim: int 
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, dim, values, indices, rest, mask, k, temperature, reduction):
-        view, _ = _logit_view(logits, dim, "TopLogitDistillLoss")
-        row_loss, loss, stats = kn.distill_fwd(view, values, indices, rest, mask, k, temperature, reduction == "mean", reduction == "none")
-        ctx.save_for_backward(view, values, indices, rest, stats, loss)
-        ctx.meta = (logits.shape, dim, k, temperature, reduction)
-        if reduction == "none":
-            return row_loss.view([n for i, n in enumerate(logits.shape) if i != dim])
-        return loss[0].clone()
+    def forward(ctx, logits, values, indices, rest, mask, dim, temperature, reduction):
+        dim = _class_dim(logits, dim, "TopLogitDistillLoss")
+        shape = logits.shape
+        others = shape[:dim] + shape[dim + 1:]
+        k = values.shape[dim] if values.dim() == len(shape) else 0
+        if values.shape != indices.shape or values.shape != shape[:dim] + (k,) + shape[dim + 1:]:
+            raise ValueError(f"teacher of shapes {tuple(values.shape)}, {tuple(indices.shape)} for logits {tuple(shape)}")
+        if not 1 <= k <= kn.TOP_LOGITS_MAX_K:
+            raise ValueError(f"the teacher lists {k} classes; 1 ... {kn.TOP_LOGITS_MAX_K} are supported")
+        for name, t, dt in (("rest", rest, torch.float32), ("mask", mask, torch.bool)):
+            if t is not None and (t.shape != others or t.dtype is not dt):
+                raise ValueError(f"{name} must be {dt} of shape {tuple(others)}, got {t.dtype} {tuple(t.shape)}")
+        view = _logit_view(logits, dim)
+        if view.dim() == 2 and dim != len(shape) - 1:
+            values, indices = values.movedim(dim, -1), indices.movedim(dim, -1)
+        values, indices, rest, mask = (None if t is None else t.contiguous() for t in (values, indices, rest, mask))
+        mean = reduction == "mean"
+        row_loss, loss, saved = kn.distill_fwd(view, values, indices, rest, mask, k, temperature, mean, reduction == "none")
+        ctx.save_for_backward(view, values, indices, rest, saved)
+        ctx.meta = (shape, dim, k, temperature, mean)
+        return loss if row_loss is None else row_loss.view(others)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        view, values, indices, rest, stats, loss = ctx.saved_tensors
-        shape, dim, k, temperature, reduction = ctx.meta
+        view, values, indices, rest, saved = ctx.saved_tensors
+        shape, dim, k, temperature, mean = ctx.meta
         dz = torch.empty(view.shape, dtype=view.dtype, device=view.device)
-        kn.distill_bwd(view, values, indices, rest, k, temperature, stats, loss if reduction == "mean" else None,
-                       g.detach().float().reshape(-1).contiguous(), dz)
+        kn.distill_bwd(view, values, indices, rest, k, temperature, saved, mean, g.float().contiguous(), dz)
         if view.dim() == 2 and dim != len(shape) - 1:
-            dz = dz.view([n for i, n in enumerate(shape) if i != dim] + [shape[dim]]).movedim(-1, dim)
-        else:
+            dz = dz.view(shape[:dim] + shape[dim + 1:] + (shape[dim],)).movedim(-1, dim)
+        elif dz.shape != shape:
             dz = dz.view(shape)
-        return dz, None, None, None, None, None, None, None, None
+        return dz, None, None, None, None, None, None, None
 
 
 class TopLogitDistillLoss(torch.nn.Module):
@@ -176,22 +192,7 @@ class TopLogitDistillLoss(torch.nn.Module):
         self.temperature, self.reduction, self.dim = _temperature(temperature), reduction, int(dim)
 
     def forward(self, logits: torch.Tensor, teacher: TopLogits, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
-        view, dim = _logit_view(logits.detach(), self.dim, "TopLogitDistillLoss")
         values, indices, rest = teacher
-        others = torch.Size(n for i, n in enumerate(logits.shape) if i != dim)
-        if values.dim() != logits.dim() or values.shape != indices.shape or _class_last(values, dim).shape[:-1] != others:
-            raise ValueError(f"teacher of shapes {tuple(values.shape)}, {tuple(indices.shape)} for logits {tuple(logits.shape)}")
-        k = values.shape[dim]
-        if not 1 <= k <= kn.TOP_LOGITS_MAX_K:
-            raise ValueError(f"the teacher lists {k} classes; 1 ... {kn.TOP_LOGITS_MAX_K} are supported")
-        for name, t, dt in (("rest", rest, torch.float32), ("mask", mask, torch.bool)):
-            if t is not None and (t.shape != others or t.dtype != dt):
-                raise ValueError(f"{name} must be {dt} of shape {tuple(others)}, got {t.dtype} {tuple(t.shape)}")
-        if any(t is not None and t.requires_grad for t in (values, rest)) and torch.is_grad_enabled():
+        if (values.requires_grad or (rest is not None and rest.requires_grad)) and torch.is_grad_enabled():
             raise ValueError("the teacher is frozen: detach its values")
-        if values.dtype != torch.float32 or indices.dtype != torch.int32:
-            raise TypeError(f"teacher values must be float32 and indices int32, got {values.dtype}, {indices.dtype}")
-        if view.dim() == 2:
-            values, indices = _class_last(values, dim), _class_last(indices, dim)
-        rest, mask = (None if t is None else t.contiguous() for t in (rest, mask))
-        return _DistillFn.apply(logits, dim, values.contiguous(), indices.contiguous(), rest, mask, k, self.temperature, self.reduction)
+        return _DistillFn.apply(logits, values, indices, rest, mask, self.dim, self.temperature, self.reduction)

@@ -21,7 +21,6 @@ from typing import Optional, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _lib
 from . import kernels as kn
 
 
@@ -30,7 +29,7 @@ class MX4Tensor:
     (element 2i of a group in the low half of byte i; codes behind the last column must be zero)."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, cols: int):
-        rows = kn._mx4_shape(codes, scales, cols, "MX4Tensor")
+        rows = kn._mx4(codes, scales, int(cols), "MX4Tensor", kn._gpu(codes, "MX4Tensor"))[0]
         self.codes, self.scales, self.shape = codes, scales, torch.Size((rows, int(cols)))
 
     @property
@@ -49,13 +48,13 @@ class MX4Tensor:
 
 def _matrix(x: torch.Tensor, name: str) -> torch.Tensor:
     """[..., cols] as [rows, cols] with adjacent elements in a row, copied only where its strides need it"""
-    if not x.is_cuda:
-        raise _lib.MsfwsiHipError(f"{name}: expected a GPU tensor (no CPU path exists)")
-    kn.dt_of(x)
+    kn._gpu(x, name)
+    kn._float(x, name)
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f"{name}: expected [..., cols] with at least one column, got {tuple(x.shape)}")
-    x = x.reshape(-1, x.shape[-1])
-    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if not x.is_contiguous() and ((x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1])):
         x = x.contiguous()
     return x
 
@@ -70,17 +69,14 @@ def quantize_mx4(x: torch.Tensor) -> MX4Tensor:
     return MX4Tensor(codes, scales, x.shape[1])
 
 
-def _product(x: MX4Tensor, weight: MX4Tensor, bias, out_dtype) -> torch.Tensor:
-    y = torch.empty(x.shape[0], weight.shape[0], dtype=out_dtype, device=x.device)
-    return kn.mx4_gemm(x.codes, x.scales, weight.codes, weight.scales, x.shape[1], y, bias)
-
-
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, out_dtype):
         ctx.weight, ctx.like = weight, (x.shape, x.dtype)
-        y = _product(quantize_mx4(x), weight, bias, out_dtype)
-        return y.view(*x.shape[:-1], weight.shape[0])
+        rows = _matrix(x, "mx4_linear")
+        y = torch.empty(rows.shape[0], weight.shape[0], dtype=out_dtype, device=x.device)
+        kn.mx4_linear(rows, weight.codes, weight.scales, y, bias)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0])
 
     @staticmethod
     @once_differentiable
@@ -89,7 +85,7 @@ class _LinearFn(torch.autograd.Function):
         dy = _matrix(dy, "mx4_linear backward")
         dx = torch.empty(dy.shape[0], shape[-1], dtype=dtype, device=dy.device)
         kn.mx4_dgrad(dy, ctx.weight.codes, ctx.weight.scales, dx)
-        return dx.view(shape), None, None, None
+        return dx if len(shape) == 2 else dx.view(shape), None, None, None
 
 
 def mx4_linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optional[torch.Tensor] = None,
@@ -103,15 +99,12 @@ def mx4_linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optio
         raise ValueError(f"mx4_linear: x has shape {tuple(x.shape)}, weight {tuple(weight.shape)}")
     if weight.shape[0] == 0:
         raise ValueError("mx4_linear: weight has no rows")
-    if bias is not None:
-        if bias.requires_grad and torch.is_grad_enabled():
-            raise ValueError("mx4_linear: the layer is frozen; pass bias.detach()")
-        kn._dense(bias, "bias", torch.float32, weight.shape[0])
-    if not x.device.type == "cuda":
-        raise _lib.MsfwsiHipError("mx4_linear: expected a GPU tensor (no CPU path exists)")
-    kn._one_device(weight, x, bias)
+    if bias is not None and bias.requires_grad and torch.is_grad_enabled():
+        raise ValueError("mx4_linear: the layer is frozen; pass bias.detach()")
     if isinstance(x, MX4Tensor):
-        return _product(x, weight, bias, out_dtype or torch.float32)
+        y = torch.empty(x.shape[0], weight.shape[0], dtype=out_dtype or torch.float32, device=x.device)
+        return kn.mx4_gemm(x.codes, x.scales, weight.codes, weight.scales, x.shape[1], y, bias)
+    kn._gpu(x, "mx4_linear")
     return _LinearFn.apply(x, weight, bias, out_dtype or x.dtype)
 
 

@@ -96,7 +96,7 @@ def test_refusals_without_a_gpu(hip_lib):
     assert hip_lib.msfwsi_top_logits(0, None, 5, 1, 5, 1, 2, 1.0, None, None, None, None, None) == -1       # no memory
     assert hip_lib.msfwsi_top_logits(0, None, 4, 2, 5, 1, 2, 1.0, None, None, None, None, None) == -1       # rows overlap
     assert hip_lib.msfwsi_top_logits(0, None, 5, 0, 5, 1, 2, 1.0, None, None, None, None, None) == 0        # no rows
-    assert hip_lib.msfwsi_distill_fwd(0, None, 5, 1, 5, 1, 65, None, None, None, None, 1.0, 1, None, None, None, None, None) == -1
+    assert hip_lib.msfwsi_distill_fwd(0, None, 5, 1, 5, 1, 65, None, None, None, None, 1.0, 1, None, None, None, None, None, None) == -1
     assert hip_lib.msfwsi_distill_bwd(3, None, 5, 1, 5, 1, 2, None, None, None, 1.0, None, None, None, 0, None, None) == -1
 
 
