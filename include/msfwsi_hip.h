@@ -556,7 +556,7 @@ int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, const void* 
  *                       rest = log sum over the others of exp(logit * inv_t).  workspace: msfwsi_top_logits_workspace
  *                       bytes, 16-byte aligned (a host call; NULL when it says 0)
  *   msfwsi_distill_fwd: row_loss [rows] or NULL (0 where a row does not count), stats [rows][4] (16-byte aligned) for the
- *                       backward, partials [2048][2] scratch, *loss = sum or mean over the rows that count, *factor = the
+ *                       backward, partials [8192][2] scratch, *loss = sum or mean over the rows that count, *factor = the
  *                       gradient's (1 / their number for the mean, else 1).  rest / mask may be NULL.  outer = 0 writes loss and
  *                       factor alone
  *   msfwsi_distill_bwd: dz [outer][classes][inner] contiguous = g * factor * d loss_row / dz; g holds one value, or one per

@@ -22,12 +22,15 @@
 #include "common.h"
 #include "../../include/msfwsi_hip.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kT = 256;
 constexpr int kMaxK = 64;        // = the lanes of a wave: lane i holds entry i of a teacher's list
-constexpr int kMaxParts = 2048;  // workgroups of the forward at most; each leaves one (sum, count) pair
+constexpr int kMaxParts = 8192;  // workgroups of the forward at most; each leaves one (sum, count) pair
 constexpr int kCand = 512;       // candidates a selection ranks at once
+constexpr int kQueue = 256;      // chunks with candidates it can hold
 constexpr int kSeg = 65536;      // classes whose list membership is held as bits at a time
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -52,12 +55,14 @@ __device__ __forceinline__ int index_of(long key) { return 0x7fffffff - (int)(un
 constexpr long kNoKey = (long)0x8000000000000000L;
 
 // sum of 2^((x - m) c) over some logits x: c = log2(e) / T, m the largest of them.  Nothing: m = -inf, s = 0; a NaN among them
-// makes s NaN.  The difference is taken before the product, so logits far from zero keep their precision.
+// makes s NaN.  The difference is taken before the product, so logits far from zero keep their precision and a row of the
+// type's lowest value does not overflow.  (c x - c m in one fma was no faster.)
 struct Sum {
     float m, s;
 };
+__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
 __device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
-    const float m = fmaxf(a.m, b.m), ref = m == -INFINITY ? 0.f : m;
+    const float m = fmaxf(a.m, b.m), ref = finite_ref(m);
     return {m, a.s * exp2_((a.m - ref) * c) + b.s * exp2_((b.m - ref) * c)};
 }
 __device__ __forceinline__ Sum one(float x) { return {x, x == -INFINITY ? 0.f : 1.f}; }
@@ -95,12 +100,14 @@ struct __attribute__((packed, aligned(sizeof(T)))) Unaligned16 {
     unsigned x, y, z, w;
 };
 template <typename T>
+__device__ __forceinline__ uint4 whole_chunk(const T* __restrict__ p, int c) {
+    const Unaligned16<T> u = *reinterpret_cast<const Unaligned16<T>*>(p + c);
+    return make_uint4(u.x, u.y, u.z, u.w);
+}
+template <typename T>
 __device__ __forceinline__ uint4 load_chunk(const T* __restrict__ p, int c, int n) {
     constexpr int VEC = ElemTraits<T>::VEC;
-    if (c + VEC <= n) {
-        const Unaligned16<T> u = *reinterpret_cast<const Unaligned16<T>*>(p + c);
-        return make_uint4(u.x, u.y, u.z, u.w);
-    }
+    if (c + VEC <= n) return whole_chunk<T>(p, c);
     float f[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) f[e] = c + e < n ? load_elem<T>(p, c + e) : -INFINITY;
@@ -124,9 +131,11 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int c, int n, con
 // ---------------------------------------------------------------------------------------------------------------------
 // Selection, rows of adjacent classes.  A workgroup holds one segment of a row in registers (read once): NT threads x NCH
 // chunks of 16 bytes.  The k-th largest of the NT threads' maxima is a lower bound of the k-th largest element, found by
-// one wave bit by bit with ballots; what is not below it goes into a list -- barely more than k elements unless large
-// logits crowd into few threads or tie -- and is ranked by counting.  Everything else is summed for `rest` on the same walk.
-// A list that runs over (long ties, a masked-out segment) sends the segment through k rounds of a plain maximum instead.
+// one wave bit by bit with ballots.  Chunks that hold anything not below it -- barely more than k unless large logits crowd
+// into few threads or tie -- go to a queue, whose elements the threads then look at one by one (nearly every wave meets such a
+// chunk at nearly every step: looking at them in place cost all lanes the walk twice over, 166 us instead of SEGUS); what is
+// not below the bound goes into a list and is ranked by counting.  Everything else is summed for `rest`.
+// A queue or list that runs over (long ties, a masked-out segment) sends the segment through k rounds of a plain maximum instead.
 // Rows longer than a segment leave their segments' lists and sums to a merge.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int NT, int NCH>
@@ -135,10 +144,12 @@ __global__ void __launch_bounds__(NT) top_segment_kernel(const T* __restrict__ x
                                                          long* __restrict__ part_keys, Sum* __restrict__ part_sums) {
     constexpr int VEC = ElemTraits<T>::VEC;
     __shared__ long cand[kCand];
+    __shared__ uint4 queue[kQueue];
+    __shared__ int queue_at[kQueue];
     __shared__ int maxima[NT];
     __shared__ Sum buf[NT / 64];
     __shared__ long lbuf[NT / 64];
-    __shared__ int count, bound;
+    __shared__ int count, queued, bound;
     const int t = threadIdx.x;
     const long row = blockIdx.x / nseg;
     const int seg = (int)(blockIdx.x % nseg), c0 = seg * (NT * NCH * VEC), n = min(C - c0, NT * NCH * VEC), want = min(k, n);
@@ -148,8 +159,13 @@ __global__ void __launch_bounds__(NT) top_segment_kernel(const T* __restrict__ x
 
     uint4 raw[NCH];
     float f[VEC], top = -INFINITY;
+    if (n == NT * NCH * VEC) {
 #pragma unroll
-    for (int j = 0; j < NCH; ++j) raw[j] = load_chunk<T>(p, (j * NT + t) * VEC, n);
+        for (int j = 0; j < NCH; ++j) raw[j] = whole_chunk<T>(p, (j * NT + t) * VEC);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) raw[j] = load_chunk<T>(p, (j * NT + t) * VEC, n);
+    }
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
         unpack16<T>(raw[j], f);
@@ -157,7 +173,7 @@ __global__ void __launch_bounds__(NT) top_segment_kernel(const T* __restrict__ x
         for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[e]);
     }
     maxima[t] = order_of(top);
-    if (t == 0) count = 0;
+    if (t == 0) count = queued = 0;
     __syncthreads();
     if (t < 64) {
         int m[NT / 64];
@@ -179,39 +195,45 @@ __global__ void __launch_bounds__(NT) top_segment_kernel(const T* __restrict__ x
     const int b = bound;
     // an order below that of -inf (too few maxima, or cut-off bits) leaves nothing out
     const float lim = b <= (int)0x807fffff ? -INFINITY : value_of(b);
-    const float ref = lim == -INFINITY ? 0.f : lim;
+    const float shift = -finite_ref(lim * c);  // c x - c lim in one fma: `rest` itself has no finer step than c lim's
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
         unknown(raw[j]);
         unpack16<T>(raw[j], f);
-        float high = f[0];
+        float high = f[0], part = 0.f;
 #pragma unroll
         for (int e = 1; e < VEC; ++e) high = fmaxf(high, f[e]);
-        if (high < lim) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s += exp2_((f[e] - ref) * c);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const int at = (j * NT + t) * VEC + e;
-                if (at >= n) continue;
-                if (f[e] < lim) {
-                    s += exp2_((f[e] - ref) * c);
-                } else {
-                    const int slot = atomicAdd(&count, 1);
-                    if (slot < kCand) cand[slot] = key_of(f[e], c0 + at);
-                }
-            }
+        for (int e = 0; e < VEC; ++e) part += exp2_(fmaf(f[e], c, shift));
+        const bool queue_it = !(high < lim);
+        s += queue_it ? 0.f : part;
+        if (queue_it) {
+            const int slot = atomicAdd(&queued, 1);
+            if (slot < kQueue) queue[slot] = raw[j], queue_at[slot] = (j * NT + t) * VEC;
         }
     }
-    const Sum below = block_join<NT>({s == 0.f ? -INFINITY : ref, s}, buf, c);
+    __syncthreads();
+    const int chunks = queued;
+    if (chunks <= kQueue)
+        for (int i = t; i < chunks * VEC; i += NT) {
+            const int at = queue_at[i / VEC] + i % VEC;
+            const float v = load_elem<T>(reinterpret_cast<const T*>(queue), i);
+            if (at >= n) continue;
+            if (v < lim) {
+                s += exp2_(fmaf(v, c, shift));
+            } else {
+                const int slot = atomicAdd(&count, 1);
+                if (slot < kCand) cand[slot] = key_of(v, c0 + at);
+            }
+        }
+    const Sum below = block_join<NT>({s == 0.f ? -INFINITY : finite_ref(lim), s}, buf, c);
     __syncthreads();
     const int got = count;
     Sum left = {-INFINITY, 0.f};
     // The list decides when it holds every candidate.  The sum decides unless a NaN went by in it, or it is so small against its
     // reference that terms of it may have been flushed
-    if (got <= kCand && (got >= n || below.s >= 1e-30f)) {
+    if (chunks <= kQueue && got <= kCand && (got >= n || below.s >= 1e-30f)) {
         for (int i = t; i < got; i += NT) {
             const long key = cand[i];
             int rank = 0;
@@ -285,10 +307,42 @@ __global__ void __launch_bounds__(NT) top_segment_kernel(const T* __restrict__ x
         for (int r = want + t; r < k; r += NT) keys_out[r] = kNoKey;
 }
 
-// One wave per row: the segments' sorted lists are merged by k rounds over their heads; what is left of them joins `rest`.
-__global__ void __launch_bounds__(64) top_merge_kernel(const long* __restrict__ part_keys, const Sum* __restrict__ part_sums, int nseg, int k,
+// The segments' lists of a row become one: every entry's rank is counted (33 us as rounds over the lists' heads, 5 so, at
+// 4096 rows of 4 x 32); what is not among the k joins `rest`.
+constexpr int kMergeHeld = 2048;
+__global__ void __launch_bounds__(kT) top_merge_kernel(const long* __restrict__ part_keys, const Sum* __restrict__ part_sums, int nseg, int k,
                                                        float inv_t, float* __restrict__ values, int* __restrict__ indices,
                                                        float* __restrict__ rest) {
+    extern __shared__ long held[];
+    __shared__ Sum buf[kT / 64];
+    const int t = threadIdx.x, n = nseg * k;
+    const long row = blockIdx.x;
+    const long* keys = part_keys + row * n;
+    const float c = inv_t * kLog2e;
+    for (int i = t; i < n; i += kT) held[i] = keys[i];
+    __syncthreads();
+    Sum sum = {-INFINITY, 0.f};
+    for (int i = t; i < nseg; i += kT) sum = join(sum, part_sums[row * nseg + i], c);
+    for (int i = t; i < n; i += kT) {
+        const long key = held[i];
+        if (key == kNoKey) continue;
+        int rank = 0;
+#pragma unroll 8
+        for (int q = 0; q < n; ++q) rank += held[q] > key;
+        if (rank < k) {
+            values[row * k + rank] = value_of((int)(key >> 32));
+            indices[row * k + rank] = index_of(key);
+        } else {
+            sum = join(sum, one(value_of((int)(key >> 32))), c);
+        }
+    }
+    sum = block_join<kT>(sum, buf, c);
+    if (t == 0) rest[row] = log_of(sum, inv_t);
+}
+// The same for more entries than are worth counting: one wave per row, k rounds over the heads of the sorted lists.
+__global__ void __launch_bounds__(64) top_merge_long_kernel(const long* __restrict__ part_keys, const Sum* __restrict__ part_sums, int nseg,
+                                                            int k, float inv_t, float* __restrict__ values, int* __restrict__ indices,
+                                                            float* __restrict__ rest) {
     extern __shared__ int head[];  // entry i belongs to lane i % 64 alone
     const int l = threadIdx.x;
     const long row = blockIdx.x;
@@ -302,11 +356,11 @@ __global__ void __launch_bounds__(64) top_merge_kernel(const long* __restrict__ 
     }
     for (int r = 0; r < k; ++r) {
         long best = mine;
-        for (int off = 1; off < 64 && off < nseg; off <<= 1) {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
             const long o = __shfl_xor(best, off, 64);
             best = o > best ? o : best;
         }
-        best = __shfl(best, 0, 64);
         if (mine == best && from >= 0) {
             values[row * k + r] = value_of((int)(best >> 32));
             indices[row * k + r] = index_of(best);
@@ -334,7 +388,26 @@ __global__ void __launch_bounds__(64) top_merge_kernel(const long* __restrict__ 
 // kept sorted in registers; every class throws one value out of it (itself, a displaced one or an empty slot), which goes to
 // the running sum for `rest`, so the logits are read once.
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int KM>
+// 16-bit logits: order and index fit one int (up to 65536 classes), and a step of the insertion is a max and a min.
+template <typename T>
+__device__ __forceinline__ int order16(T x);
+template <>
+__device__ __forceinline__ int order16<__bf16>(__bf16 x) { return order_of((float)x) >> 16; }
+template <>
+__device__ __forceinline__ int order16<_Float16>(_Float16 x) {
+    if (x != x) return 0x7fff;
+    const int b = __builtin_bit_cast(short, (_Float16)(x + (_Float16)0.f));
+    return b ^ ((b >> 15) & 0x7fff);
+}
+template <typename T>
+__device__ __forceinline__ float value16(int order);
+template <>
+__device__ __forceinline__ float value16<__bf16>(int order) { return __uint_as_float((unsigned)(order ^ ((order >> 15) & 0x7fff)) << 16); }
+template <>
+__device__ __forceinline__ float value16<_Float16>(int order) {
+    return (float)__builtin_bit_cast(_Float16, (short)(order ^ ((order >> 15) & 0x7fff)));
+}
+template <typename T, int KM, bool SMALL>
 __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x, long ld, int C, long inner, long rows, int k, float inv_t,
                                                         float* __restrict__ values, int* __restrict__ indices, float* __restrict__ rest) {
     const float c = inv_t * kLog2e;
@@ -342,25 +415,42 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
     if (row >= rows) return;
     const long o = (unsigned)row / (unsigned)inner, i = row - o * inner;  // rows fit 31 bits
     const T* p = x + o * ld + i;
-    int v[KM], at[KM];
+    int v[KM], at[SMALL ? 1 : KM];
 #pragma unroll
-    for (int s = 0; s < KM; ++s) v[s] = kNothing, at[s] = 0;
+    for (int s = 0; s < KM; ++s) v[s] = kNothing;
+    if constexpr (!SMALL) {
+#pragma unroll
+        for (int s = 0; s < KM; ++s) at[s] = 0;
+    }
     Sum sum = {-INFINITY, 0.f};
 #pragma unroll 4
     for (int j = 0; j < C; ++j) {
-        int a = order_of(load_elem<T>(p, j * inner)), ai = j;
-        bool in = false;
+        float out;
+        if constexpr (SMALL) {
+            int a = order16<T>(p[j * inner]) << 16 | (0xffff - j);
 #pragma unroll
-        for (int s = 0; s < KM; ++s)
-            if (s < k) {
-                const int ov = v[s], oi = at[s];
-                in = in || a > ov;
-                v[s] = in ? a : ov;
-                at[s] = in ? ai : oi;
-                a = in ? ov : a;
-                ai = in ? oi : ai;
-            }
-        const float out = value_of(a);
+            for (int s = 0; s < KM; ++s)
+                if (s < k) {
+                    const int low = min(v[s], a);
+                    v[s] = max(v[s], a);
+                    a = low;
+                }
+            out = a == kNothing ? -INFINITY : value16<T>(a >> 16);
+        } else {
+            int a = order_of(load_elem<T>(p, j * inner)), ai = j;
+            bool in = false;
+#pragma unroll
+            for (int s = 0; s < KM; ++s)
+                if (s < k) {
+                    const int ov = v[s], oi = at[s];
+                    in = in || a > ov;
+                    v[s] = in ? a : ov;
+                    at[s] = in ? ai : oi;
+                    a = in ? ov : a;
+                    ai = in ? oi : ai;
+                }
+            out = value_of(a);
+        }
         if (out != -INFINITY) {
             const float d = out - sum.m, e = exp2_(-fabsf(d) * c);
             sum.s = d > 0.f ? fmaf(sum.s, e, 1.f) : sum.s + e;
@@ -370,20 +460,21 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
 #pragma unroll
     for (int s = 0; s < KM; ++s)
         if (s < k) {
-            values[(o * k + s) * inner + i] = value_of(v[s]);
-            indices[(o * k + s) * inner + i] = at[s];
+            if constexpr (SMALL) values[(o * k + s) * inner + i] = value16<T>(v[s] >> 16);
+            else values[(o * k + s) * inner + i] = value_of(v[s]);
+            indices[(o * k + s) * inner + i] = SMALL ? 0xffff - (v[s] & 0xffff) : at[s];
         }
     rest[row] = log_of(sum, inv_t);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// The loss.  What the backward keeps of a row, in four floats: the largest logit m and ls = log2 of sum 2^((z_j - m) c) over all
-// classes, and the same (mt, lt) over the unlisted ones.  Two maxima, because the unlisted classes may lie so far below the
+// The loss.  What the backward keeps of a row, in four floats: m and ls = log2 s of the sum over all classes (struct Sum), and the
+// same, mt and lt, over the unlisted ones.  Two maxima, because the unlisted classes may lie so far below the
 // listed ones that their sum relative to m would vanish.  A sum is at least 1, its logarithm at least 0: ls = -1 marks a row that
 // does not count.
 // ---------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float4 row_stats(Sum unlisted, Sum all) {
-    const float m = all.m == -INFINITY ? 0.f : all.m;
+    const float m = finite_ref(all.m);
     return make_float4(m, all.s == 0.f ? 0.f : log2_(all.s), unlisted.m == -INFINITY ? m : unlisted.m,
                        unlisted.s == 0.f ? 0.f : log2_(unlisted.s));
 }
@@ -404,17 +495,18 @@ __device__ __forceinline__ void leave_part(double s, double n, double* __restric
     }
 }
 // loss = sum or mean of the rows that count, factor = that of the gradient (1 / their number for the mean)
-__global__ void __launch_bounds__(kT) distill_finish_kernel(const double* __restrict__ parts, int n, int mean, float* __restrict__ loss,
+constexpr int kFinish = 1024;
+__global__ void __launch_bounds__(kFinish) distill_finish_kernel(const double* __restrict__ parts, int n, int mean, float* __restrict__ loss,
                                                             float* __restrict__ factor) {
-    __shared__ double sums[kT / 64], counts[kT / 64];
+    __shared__ double sums[kFinish / 64], counts[kFinish / 64];
     double s = 0.0, m = 0.0;
-    for (int i = threadIdx.x; i < n; i += kT) s += parts[2 * i], m += parts[2 * i + 1];
+    for (int i = threadIdx.x; i < n; i += blockDim.x) s += parts[2 * i], m += parts[2 * i + 1];
     s = wave_sum_d(s);
     m = wave_sum_d(m);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s, counts[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < kT / 64; ++i) s += sums[i], m += counts[i];
+        for (int i = 1; i < (int)blockDim.x / 64; ++i) s += sums[i], m += counts[i];
         const double f = mean ? 1.0 / (m > 0.0 ? m : 1.0) : 1.0;
         *loss = (float)(s * f);
         *factor = (float)f;
@@ -458,17 +550,14 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
             __syncthreads();
             if (here) atomicOr(&bits[(idx - s0) >> 5], 1u << ((idx - s0) & 31));
             __syncthreads();
-            for (int a = t * VEC; a < n; a += U * NT * VEC) {
-                float f[U][VEC];
+            auto add = [&](const uint4* raw, int a, auto count_) {  // chunks of this thread from `a` on
+                constexpr int N = decltype(count_)::value;
+                float f[N][VEC];
                 float top = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int at = a + u * NT * VEC;
-                    unpack16<T>(load_chunk<T>(p + s0, at, n), f[u]);  // past the row: all -inf
-                }
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int at = a + u * NT * VEC;
+                for (int u = 0; u < N; ++u) {
+                    const int at = a + (u * NT + t) * VEC;
+                    unpack16<T>(raw[u], f[u]);
                     const unsigned w = at < n ? (bits[at >> 5] >> (at & 31)) & ((1u << VEC) - 1u) : 0u;
                     if (w) {
 #pragma unroll
@@ -477,13 +566,35 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[u][e]);
                 }
-                const float m = fmaxf(sum.m, top), ref = m == -INFINITY ? 0.f : m;
+                const float m = fmaxf(sum.m, top), ref = finite_ref(m);
                 float s = sum.s * exp2_((sum.m - ref) * c);
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+                for (int u = 0; u < N; ++u)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) s += exp2_((f[u][e] - ref) * c);
                 sum = {m, s};
+            };
+            // whole turns of U chunks a thread, loaded without a test each (a load behind a branch of its own is waited for there)
+            // and one turn ahead; then the rest chunk by chunk
+            constexpr int TURN = U * NT * VEC;
+            int a = 0;
+            if (n >= TURN) {
+                uint4 raw[U], next[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) raw[u] = whole_chunk<T>(p + s0, (u * NT + t) * VEC);
+                for (; a + 2 * TURN <= n; a += TURN) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) next[u] = whole_chunk<T>(p + s0, a + TURN + (u * NT + t) * VEC);
+                    add(raw, a, std::integral_constant<int, U>());
+#pragma unroll
+                    for (int u = 0; u < U; ++u) raw[u] = next[u];
+                }
+                add(raw, a, std::integral_constant<int, U>());
+                a += TURN;
+            }
+            for (; a < n; a += NT * VEC) {
+                const uint4 raw = load_chunk<T>(p + s0, a + t * VEC, n);  // past the row: all -inf
+                add(&raw, a, std::integral_constant<int, 1>());
             }
             __syncthreads();
             if (here) bits[(idx - s0) >> 5] = 0;
@@ -497,7 +608,8 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
                 const int other = __shfl(idx, q, 64);  // by every lane: a lane that sits out cannot be read either
                 first = first && (q >= lane || other != idx);
             }
-            const Sum all = join(unlisted, wave_join(first ? one(zi) : Sum{-INFINITY, 0.f}, c), c);
+            const float m = fmaxf(unlisted.m, wave_max(zi == zi ? zi : -INFINITY)), ref = finite_ref(m);
+            const Sum all = {m, unlisted.s * exp2_((unlisted.m - ref) * c) + wave_sum(first ? exp2_((zi - ref) * c) : 0.f)};
             float4 st = row_stats(unlisted, all);
             if (bad) st.x = st.z = NAN;
             // teacher, in base-2 units relative to its largest entry
@@ -551,18 +663,26 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
     const float pi = lane < k ? exp2_(lv - L) : 0.f, pr = exp2_(lr - L);
     const float gs = g[g_rows ? row : 0] * (factor != nullptr ? *factor : 1.f) * temp;
     const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - pr);
-    for (int a = t * VEC; a < C; a += U * NT * VEC) {
+    int a = 0;
+    for (; a + U * NT * VEC <= C; a += U * NT * VEC) {
         uint4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = load_chunk<T>(p, a + u * NT * VEC, C);
+        for (int u = 0; u < U; ++u) raw[u] = whole_chunk<T>(p, a + (u * NT + t) * VEC);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             float f[VEC];
             unpack16<T>(raw[u], f);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) f[e] = outside * exp2_((f[e] - st.z) * c - st.w);
-            store_chunk<T>(d, a + u * NT * VEC, C, f);
+            store_chunk<T>(d, a + (u * NT + t) * VEC, C, f);
         }
+    }
+    for (a += t * VEC; a < C; a += NT * VEC) {
+        float f[VEC];
+        unpack16<T>(load_chunk<T>(p, a, C), f);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = outside * exp2_((f[e] - st.z) * c - st.w);
+        store_chunk<T>(d, a, C, f);
     }
     __syncthreads();
     if (t >= 64) return;
@@ -600,6 +720,12 @@ struct List {
     }
     __device__ __forceinline__ float value(int s) const { return index(s) >= 0 ? vp[s * inner] : -INFINITY; }
 };
+template <typename T, int U>
+__device__ __forceinline__ void load_classes(const T* __restrict__ p, int c0, int C, long inner, float* f) {
+#pragma unroll
+    for (int e = 0; e < U; ++e)
+        if (c0 + e < C) f[e] = load_elem<T>(p, (c0 + e) * inner);
+}
 #define LIST_FOR(S) _Pragma("clang loop unroll_count(KM > 0 ? KM : 1)") for (int S = 0; S < (KM > 0 ? KM : list.k); ++S) if (KM == 0 || S < list.k)
 
 template <typename T, int KM>
@@ -608,12 +734,14 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
                                                                 const float* __restrict__ rest, const unsigned char* __restrict__ mask,
                                                                 float temp, float inv_t, float4* __restrict__ stats,
                                                                 float* __restrict__ row_loss, double* __restrict__ parts) {
-    constexpr int U = 8;
+    constexpr int U = 32;  // classes at a time
     const float c = inv_t * kLog2e;
     double lsum = 0.0, lcount = 0.0;
     for (long row = blockIdx.x * (long)kT + threadIdx.x; row < rows; row += (long)gridDim.x * kT) {
         const long o = (unsigned)row / (unsigned)inner, i = row - o * inner;  // rows fit 31 bits
         const T* p = z + o * ld + i;
+        float f[U];
+        load_classes<T, U>(p, 0, C, inner, f);
         List<KM> list;
         list.open(values, indices, o, i, inner, k);
         const float r = rest != nullptr ? rest[row] * temp : -INFINITY;
@@ -631,30 +759,31 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
         }
         Sum un = {-INFINITY, 0.f}, in = {-INFINITY, 0.f};
         for (int c0 = 0; c0 < C; c0 += U) {
-            float f[U];
+            if (c0 > 0) load_classes<T, U>(p, c0, C, inner, f);
             unsigned w = 0;
-#pragma unroll
-            for (int e = 0; e < U; ++e) f[e] = c0 + e < C ? load_elem<T>(p, (c0 + e) * inner) : -INFINITY;
             LIST_FOR(s) {
                 const unsigned at = (unsigned)(list.index(s) - c0);
                 w |= at < U ? 1u << at : 0u;
             }
             float mu = un.m, mi = in.m;
 #pragma unroll
-            for (int e = 0; e < U; ++e) {
-                const bool listed = (w >> e) & 1u;
-                mu = fmaxf(mu, listed ? -INFINITY : f[e]);
-                mi = fmaxf(mi, listed ? f[e] : -INFINITY);
-            }
-            const float ru = mu == -INFINITY ? 0.f : mu, ri = mi == -INFINITY ? 0.f : mi;
+            for (int e = 0; e < U; ++e)
+                if (c0 + e < C) {
+                    const bool listed = (w >> e) & 1u;
+                    mu = fmaxf(mu, listed ? -INFINITY : f[e]);
+                    mi = fmaxf(mi, listed ? f[e] : -INFINITY);
+                }
+            asm volatile("" : "+v"(w));  // its bits are tested again, not kept as 2 U scalar registers
+            const float ru = finite_ref(mu), ri = finite_ref(mi);
             float su = un.s * exp2_((un.m - ru) * c), si = in.s * exp2_((in.m - ri) * c);
 #pragma unroll
-            for (int e = 0; e < U; ++e) {
-                const bool listed = (w >> e) & 1u;
-                const float x = exp2_((f[e] - (listed ? ri : ru)) * c);
-                su += listed ? 0.f : x;
-                si += listed ? x : 0.f;
-            }
+            for (int e = 0; e < U; ++e)
+                if (c0 + e < C) {
+                    const bool listed = (w >> e) & 1u;
+                    const float x = exp2_((f[e] - (listed ? ri : ru)) * c);
+                    su += listed ? 0.f : x;
+                    si += listed ? x : 0.f;
+                }
             un = {mu, su};
             in = {mi, si};
         }
@@ -686,13 +815,15 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
                                                                 const float* __restrict__ rest, float temp, float inv_t,
                                                                 const float4* __restrict__ stats, const float* __restrict__ factor,
                                                                 const float* __restrict__ g, int g_rows, T* __restrict__ dz) {
-    constexpr int U = 8;
+    constexpr int U = 32;
     const float c = inv_t * kLog2e;
     const long row = blockIdx.x * (long)kT + threadIdx.x;
     if (row >= rows) return;
     const long o = (unsigned)row / (unsigned)inner, i = row - o * inner;  // rows fit 31 bits
     const T* p = z + o * ld + i;
     T* d = dz + o * C * inner + i;
+    float f[U];
+    load_classes<T, U>(p, 0, C, inner, f);  // asked for first: the list and what follows from it come in their shadow
     const float4 st = stats[row];
     if (!row_counts(st)) {
         for (int j = 0; j < C; ++j) store_elem<T>(d, j * inner, 0.f);
@@ -710,22 +841,42 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
     float total = exp2_(lr);
     LIST_FOR(s) total += exp2_((list.value(s) - vtop) * c);
     const float L = log2_(total);
+    float pi[KM > 0 ? KM : 1];
+    if constexpr (KM > 0) {
+#pragma unroll
+        for (int s = 0; s < KM; ++s) pi[s] = s < k ? exp2_((list.value(s) - vtop) * c - L) : 0.f;
+    }
     const float gs = g[g_rows ? row : 0] * (factor != nullptr ? *factor : 1.f) * temp;
     const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - exp2_(lr - L));
     for (int c0 = 0; c0 < C; c0 += U) {
-        float f[U];
-#pragma unroll
-        for (int e = 0; e < U; ++e) f[e] = c0 + e < C ? load_elem<T>(p, (c0 + e) * inner) : 0.f;
+        unsigned w = 0;
+        if (c0 > 0) load_classes<T, U>(p, c0, C, inner, f);
+        if constexpr (KM > 0) {
+            LIST_FOR(s) {
+                const unsigned at = (unsigned)(list.index(s) - c0);
+                w |= at < U ? 1u << at : 0u;
+            }
+        }
 #pragma unroll
         for (int e = 0; e < U; ++e)
-            if (c0 + e < C) store_elem<T>(d, (c0 + e) * inner, outside * exp2_((f[e] - st.z) * c - st.w));
+            if (c0 + e < C) {
+                if constexpr (KM > 0) {
+                    const bool listed = (w >> e) & 1u;
+                    float share = 0.f;
+                    LIST_FOR(s) share += list.index(s) == c0 + e ? pi[s] : 0.f;
+                    const float x = exp2_((f[e] - (listed ? st.x : st.z)) * c - (listed ? st.y : st.w));
+                    store_elem<T>(d, (c0 + e) * inner, listed ? gs * (x - share) : outside * x);
+                } else {
+                    store_elem<T>(d, (c0 + e) * inner, outside * exp2_((f[e] - st.z) * c - st.w));
+                }
+            }
     }
-    LIST_FOR(s) {  // the same thread: these stores come after the ones above
-        const int at = list.index(s);
-        if (at >= 0 && at < C) {
-            const int self = at;
+    if constexpr (KM == 0) {
+        for (int s = 0; s < k; ++s) {  // the same thread: these stores come after the ones above
+            const int at = list.index(s);
+            if (at < 0 || at >= C) continue;
             float share = 0.f;
-            LIST_FOR(q) share += list.index(q) == self ? exp2_((list.value(q) - vtop) * c - L) : 0.f;
+            for (int q = 0; q < k; ++q) share += list.index(q) == at ? exp2_((list.value(q) - vtop) * c - L) : 0.f;
             store_elem<T>(d, at * inner, gs * (exp2_((load_elem<T>(p, at * inner) - st.x) * c - st.y) - share));
         }
     }
@@ -763,12 +914,19 @@ extern "C" int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, 
     MSFWSI_CHECK_ARG(x && values && indices && rest);
     if (by_thread(classes, inner)) {
         const long rows = outer * inner, blocks = (rows + kT - 1) / kT;
-#define TOP_THREAD(KM)                                                                                                        \
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((top_thread_kernel<T, KM>), dim3((unsigned)blocks), dim3(kT), 0, ST(stream),     \
-                                            (const T*)x, ld, classes, inner, rows, k, inv_t, values, indices, rest))
-        if (k <= 4) TOP_THREAD(4);
-        else if (k <= 16) TOP_THREAD(16);
-        else TOP_THREAD(64);
+#define TOP_THREAD(T, KM, SMALL)                                                                                                  \
+    hipLaunchKernelGGL((top_thread_kernel<T, KM, SMALL>), dim3((unsigned)blocks), dim3(kT), 0, ST(stream), (const T*)x, ld, classes, \
+                       inner, rows, k, inv_t, values, indices, rest)
+#define TOP_THREAD_K(T, SMALL)                   \
+    do {                                         \
+        if (k <= 4) TOP_THREAD(T, 4, SMALL);     \
+        else if (k <= 16) TOP_THREAD(T, 16, SMALL); \
+        else TOP_THREAD(T, 64, SMALL);           \
+    } while (0)
+        if (dtype == MSFWSI_DT_F32) TOP_THREAD_K(float, false);
+        else if (classes > 65536) MSFWSI_WITH_T(dtype, TOP_THREAD_K(T, false));
+        else if (dtype == MSFWSI_DT_BF16) TOP_THREAD_K(__bf16, true);
+        else TOP_THREAD_K(_Float16, true);
         return msfwsi_launch_status();
     }
     const int nseg = segments(dtype, classes);
@@ -783,8 +941,12 @@ extern "C" int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, 
     else TOP_ROWS(256, 8);
     const int rc = msfwsi_launch_status();
     if (rc != MSFWSI_OK || nseg == 1) return rc;
-    hipLaunchKernelGGL(top_merge_kernel, dim3((unsigned)outer), dim3(64), nseg * sizeof(int), ST(stream), keys, sums, nseg, k, inv_t, values,
-                       indices, rest);
+    if (nseg * k <= kMergeHeld)
+        hipLaunchKernelGGL(top_merge_kernel, dim3((unsigned)outer), dim3(kT), (size_t)nseg * k * 8, ST(stream), keys, sums, nseg, k, inv_t, values,
+                           indices, rest);
+    else
+        hipLaunchKernelGGL(top_merge_long_kernel, dim3((unsigned)outer), dim3(64), nseg * sizeof(int), ST(stream), keys, sums, nseg, k, inv_t,
+                           values, indices, rest);
     return msfwsi_launch_status();
 }
 
@@ -825,7 +987,7 @@ extern "C" int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer,
         const int rc = msfwsi_launch_status();
         if (rc != MSFWSI_OK) return rc;
     }
-    hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(kT), 0, ST(stream), partials, (int)blocks, mean, loss,
+    hipLaunchKernelGGL(distill_finish_kernel, dim3(1), dim3(blocks > 1024 ? kFinish : kT), 0, ST(stream), partials, (int)blocks, mean, loss,
                        factor);
     return msfwsi_launch_status();
 }

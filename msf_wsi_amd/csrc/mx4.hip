@@ -127,6 +127,35 @@ __global__ void __launch_bounds__(kT) mx4_dequantize_kernel(const unsigned* __re
         store8<T>(y + r * cols + c, cols - c, f);
     }
 }
+// fp32 results are 32 bytes a lane: here a lane takes four elements of either half of the group, so that a store covers whole lines
+__global__ void __launch_bounds__(kT) mx4_dequantize32_kernel(const unsigned short* __restrict__ codes, const unsigned char* __restrict__ scales,
+                                                              long rows, long cols, int G, float* __restrict__ y) {
+    const int l = threadIdx.x & 31, g0 = blockIdx.y * UG;
+    const long r = blockIdx.x * (long)(kT / 32) + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    unsigned w[2 * UG], E[2 * UG];
+#pragma unroll
+    for (int u = 0; u < 2 * UG; ++u) {
+        const long at = (long)min(g0 + u / 2, G - 1) * rows + r;
+        w[u] = codes[at * 64 + (u & 1) * 32 + l];
+        E[u] = scales[at * 8 + (u & 1) * 4 + (l >> 3)];
+    }
+#pragma unroll
+    for (int u = 0; u < 2 * UG; ++u) {
+        const long c = (g0 + u / 2) * (long)kGroup + (u & 1) * 128 + l * 4;
+        const float s = scale_value(E[u]);
+        const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[u], 1.f, 1);
+        const float f[4] = {a.x * s, a.y * s, b.x * s, b.y * s};
+        float* p = y + r * cols + c;
+        if (c + 4 <= cols) {
+            *reinterpret_cast<Unaligned16*>(p) = {__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (c + e < cols) p[e] = f[e];
+        }
+    }
+}
 
 // One 32x32x64 step takes 32 elements of row (lane & 31) of either operand from each lane.  Which 32 is free as long as both
 // operands agree: half h of the wave takes block 4h + S of a group in step S, so its four scales are one aligned dword, of which
@@ -696,8 +725,14 @@ extern "C" int msfwsi_mx4_dequantize(int dtype, const void* codes, const void* s
     if (rows == 0) return MSFWSI_OK;
     const long G = groups_of(cols);
     MSFWSI_CHECK_ARG(y && codes && scales && aligned16(codes) && aligned16(scales) && G <= 65535L * UG && grid_ok((rows + 7) / 8));
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL(mx4_dequantize_kernel<T>, dim3((unsigned)((rows + 7) / 8), (unsigned)((G + UG - 1) / UG)), dim3(kT), 0,
-                                            ST(stream), (const unsigned*)codes, (const unsigned char*)scales, rows, cols, (int)G, (T*)y));
+    const dim3 grid((unsigned)((rows + 7) / 8), (unsigned)((G + UG - 1) / UG));
+#define MX4_WIDEN(T) \
+    hipLaunchKernelGGL(mx4_dequantize_kernel<T>, grid, dim3(kT), 0, ST(stream), (const unsigned*)codes, (const unsigned char*)scales, rows, cols, (int)G, (T*)y)
+    if (dtype == MSFWSI_DT_F32)
+        hipLaunchKernelGGL(mx4_dequantize32_kernel, grid, dim3(kT), 0, ST(stream), (const unsigned short*)codes, (const unsigned char*)scales, rows, cols,
+                           (int)G, (float*)y);
+    else if (dtype == MSFWSI_DT_BF16) MX4_WIDEN(__bf16);
+    else MX4_WIDEN(_Float16);
     return msfwsi_launch_status();
 }
 

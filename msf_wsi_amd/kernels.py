@@ -1845,7 +1845,7 @@ def top_logits(x, k: int, temperature: float, values, indices, rest):
     _call("top_logits", dev, dt, x.data_ptr(), ld, outer, Cn, inner, k, 1.0 / temperature, *args, _p(ws))
 
 
-_PARTS = 2048 * 2 * 8  # bytes of msfwsi_distill_fwd's partials
+_PARTS = 8192 * 2 * 8  # bytes of msfwsi_distill_fwd's partials
 
 
 def distill_fwd(z, values, indices, rest, mask, k: int, temperature: float, mean: bool, per_row: bool = True):
