@@ -104,6 +104,13 @@ __device__ __forceinline__ uint4 whole_chunk(const T* __restrict__ p, int c) {
     const Unaligned16<T> u = *reinterpret_cast<const Unaligned16<T>*>(p + c);
     return make_uint4(u.x, u.y, u.z, u.w);
 }
+// the same for a row that is read once: not kept in the caches (155 -> 149 us at 4096 x 65536)
+template <typename T>
+__device__ __forceinline__ uint4 passing_chunk(const T* __restrict__ p, int c) {
+    typedef __attribute__((ext_vector_type(4), aligned(2))) unsigned u32x4_any;
+    const u32x4_any u = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p + c));
+    return make_uint4(u.x, u.y, u.z, u.w);
+}
 template <typename T>
 __device__ __forceinline__ uint4 load_chunk(const T* __restrict__ p, int c, int n) {
     constexpr int VEC = ElemTraits<T>::VEC;
@@ -133,13 +140,13 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int c, int n, con
 // chunks of 16 bytes.  The k-th largest of the NT threads' maxima is a lower bound of the k-th largest element, found by
 // one wave bit by bit with ballots.  Chunks that hold anything not below it -- barely more than k unless large logits crowd
 // into few threads or tie -- go to a queue, whose elements the threads then look at one by one (nearly every wave meets such a
-// chunk at nearly every step: looking at them in place cost all lanes the walk twice over, 166 us instead of SEGUS); what is
+// chunk at nearly every step: looking at them in place cost all lanes the walk twice over, 166 us instead of 149); what is
 // not below the bound goes into a list and is ranked by counting.  Everything else is summed for `rest`.
 // A queue or list that runs over (long ties, a masked-out segment) sends the segment through k rounds of a plain maximum instead.
 // Rows longer than a segment leave their segments' lists and sums to a merge.
 // ---------------------------------------------------------------------------------------------------------------------
 template <typename T, int NT, int NCH>
-__global__ void __launch_bounds__(NT) top_segment_kernel(const T* __restrict__ x, long ld, int C, int nseg, int k, float inv_t,
+__global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(const T* __restrict__ x, long ld, int C, int nseg, int k, float inv_t,
                                                          float* __restrict__ values, int* __restrict__ indices, float* __restrict__ rest,
                                                          long* __restrict__ part_keys, Sum* __restrict__ part_sums) {
     constexpr int VEC = ElemTraits<T>::VEC;
@@ -161,7 +168,7 @@ __global__ void __launch_bounds__(NT) top_segment_kernel(const T* __restrict__ x
     float f[VEC], top = -INFINITY;
     if (n == NT * NCH * VEC) {
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) raw[j] = whole_chunk<T>(p, (j * NT + t) * VEC);
+        for (int j = 0; j < NCH; ++j) raw[j] = passing_chunk<T>(p, (j * NT + t) * VEC);
     } else {
 #pragma unroll
         for (int j = 0; j < NCH; ++j) raw[j] = load_chunk<T>(p, (j * NT + t) * VEC, n);

@@ -60,6 +60,13 @@ __device__ __forceinline__ void store8(T* __restrict__ p, long left, const float
         if (e < left) store_elem<T>(p, e, f[e]);
 }
 
+// the scale code of a block whose largest magnitude has the bits `big`, and 2^(127 - E)
+__device__ __forceinline__ float block_scale(unsigned big, unsigned& E) {
+    const unsigned field = big >> 23;
+    E = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
+    return __uint_as_float((254u - (E == 255u ? 127u : E)) << 23);
+}
+
 // One half-wave (32 lanes x 8 elements) per group of a row, UG groups one after the other with their loads in flight together; a
 // block of 32 elements is 4 lanes.  The conversion's own scale operand stays 1: the elements are multiplied by 2^(127 - E) first,
 // which is exact.  Bound by memory.
@@ -85,9 +92,8 @@ __global__ void __launch_bounds__(kT) mx4_quantize_kernel(const T* __restrict__ 
         for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(f[u][e]) & 0x7fffffffu);  // orders like the magnitudes, NaN on top
         big = max(big, (unsigned)__shfl_xor((int)big, 1, 64));
         big = max(big, (unsigned)__shfl_xor((int)big, 2, 64));
-        const unsigned field = big >> 23;
-        const unsigned E = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
-        const float up = __uint_as_float((254u - (E == 255u ? 127u : E)) << 23);  // 2^(127 - E)
+        unsigned E;
+        const float up = block_scale(big, E);
         unsigned w = 0;
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][0] * up, f[u][1] * up, 1.f, 0);
         w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][2] * up, f[u][3] * up, 1.f, 1);
@@ -167,34 +173,80 @@ __device__ __forceinline__ void mx4_step(f32x16& acc, const int4& a, int sa, con
 }
 
 // Few rows: 32 x 32 outputs per workgroup straight from memory, the groups dealt over its NW waves and joined in LDS.  Bound
-// by reading b once; nothing is shared between workgroups, so nothing is staged.
-template <typename T, int NW>
-__global__ void __launch_bounds__(NW * 64) mx4_gemm_kernel(const unsigned char* __restrict__ a, const unsigned char* __restrict__ as, long M,
+// by reading b once (18432 x 18432 at one row: FEWUS); nothing is shared between workgroups, so nothing is staged.  The next
+// group's loads are on their way while one is multiplied.
+// ROW: a single row, which comes as it is (TX) and is quantised by the wave that needs it, so that one launch does it all: 4
+// elements a lane, a block of 32 is 8 lanes; the codes pass through 128 bytes of LDS into the operand's order.
+template <typename T, typename TX, bool ROW, int NW>
+__global__ void __launch_bounds__(NW * 64) mx4_gemm_kernel(const void* __restrict__ a, const unsigned char* __restrict__ as, long M, long cols,
                                                            const unsigned char* __restrict__ b, const unsigned char* __restrict__ bs, long N,
                                                            int G, const float* __restrict__ bias, T* __restrict__ y, unsigned nt) {
-    __shared__ float part[NW][32 * 33];
+    __shared__ float part[NW][ROW ? 32 : 32 * 33];
+    __shared__ __attribute__((aligned(16))) unsigned char own[NW][kGroupBytes + 16];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
-    const long m0 = (long)(blockIdx.x / nt) * 32, n0 = (long)(blockIdx.x % nt) * 32;
+    const long m0 = ROW ? 0 : (long)(blockIdx.x / nt) * 32, n0 = (long)(ROW ? blockIdx.x : blockIdx.x % nt) * 32;
     const long m = min(m0 + (lane & 31), M - 1), n = min(n0 + (lane & 31), N - 1);
-    f32x16 acc = {0.f};
-    for (int g = w; g < G; g += NW) {
-        const long ra = g * M + m, rb = g * N + n;
-        const int sa = *reinterpret_cast<const int*>(as + ra * 8 + h * 4), sb = *reinterpret_cast<const int*>(bs + rb * 8 + h * 4);
-        int4 fa[4], fb[4];
+    struct Operands {
+        int4 a[4], b[4];
+        int sa, sb;
+        float x[4];
+    } cur, nxt;
+    auto load = [&](int g, Operands& o) {
+        const long rb = g * N + n;
+        o.sb = *reinterpret_cast<const int*>(bs + rb * 8 + h * 4);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            fa[s] = *reinterpret_cast<const int4*>(a + ra * kGroupBytes + (4 * h + s) * 16);
-            fb[s] = *reinterpret_cast<const int4*>(b + rb * kGroupBytes + (4 * h + s) * 16);
+        for (int s = 0; s < 4; ++s) o.b[s] = *reinterpret_cast<const int4*>(b + rb * kGroupBytes + (4 * h + s) * 16);
+        if constexpr (ROW) {
+            const long c = g * (long)kGroup + lane * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o.x[e] = c + e < cols ? load_elem<TX>(reinterpret_cast<const TX*>(a), c + e) : 0.f;
+        } else {
+            const long ra = g * M + m;
+            o.sa = *reinterpret_cast<const int*>(as + ra * 8 + h * 4);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+                o.a[s] = *reinterpret_cast<const int4*>(reinterpret_cast<const unsigned char*>(a) + ra * kGroupBytes + (4 * h + s) * 16);
         }
-        mx4_step<0>(acc, fa[0], sa, fb[0], sb);
-        mx4_step<1>(acc, fa[1], sa, fb[1], sb);
-        mx4_step<2>(acc, fa[2], sa, fb[2], sb);
-        mx4_step<3>(acc, fa[3], sa, fb[3], sb);
-    }
+    };
+    auto quantize = [&](Operands& o) {
+        unsigned big = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) part[w][((i & 3) + 8 * (i >> 2) + 4 * h) * 33 + (lane & 31)] = acc[i];
+        for (int e = 0; e < 4; ++e) big = max(big, __float_as_uint(o.x[e]) & 0x7fffffffu);
+#pragma unroll
+        for (int off = 1; off < 8; off <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, off, 64));
+        unsigned E;
+        const float up = block_scale(big, E);
+        unsigned c = 0;
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, o.x[0] * up, o.x[1] * up, 1.f, 0);
+        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, o.x[2] * up, o.x[3] * up, 1.f, 1);
+        // a wave's LDS instructions run in order: no barrier, but hipcc has to keep them so too
+        *reinterpret_cast<unsigned short*>(&own[w][lane * 2]) = (unsigned short)(E == 255u ? 0u : c);
+        if ((lane & 7) == 0) own[w][kGroupBytes + (lane >> 3)] = (unsigned char)E;
+        asm volatile("" ::: "memory");
+        o.sa = *reinterpret_cast<const int*>(&own[w][kGroupBytes + h * 4]);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) o.a[s] = *reinterpret_cast<const int4*>(&own[w][(4 * h + s) * 16]);
+        asm volatile("" ::: "memory");
+    };
+    f32x16 acc = {0.f};
+    if (w < G) load(w, cur);
+    for (int g = w; g < G; g += NW) {
+        load(min(g + NW, G - 1), nxt);
+        if constexpr (ROW) quantize(cur);
+        mx4_step<0>(acc, cur.a[0], cur.sa, cur.b[0], cur.sb);
+        mx4_step<1>(acc, cur.a[1], cur.sa, cur.b[1], cur.sb);
+        mx4_step<2>(acc, cur.a[2], cur.sa, cur.b[2], cur.sb);
+        mx4_step<3>(acc, cur.a[3], cur.sa, cur.b[3], cur.sb);
+        cur = nxt;
+    }
+    if constexpr (ROW) {  // all 32 rows of the operand are this one
+        if (lane < 32) part[w][lane] = acc[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) part[w][((i & 3) + 8 * (i >> 2) + 4 * h) * 33 + (lane & 31)] = acc[i];
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < 1024; i += NW * 64) {
+    for (int i = threadIdx.x; i < (ROW ? 32 : 1024); i += NW * 64) {
         const int r = i >> 5, c = i & 31;
         if (m0 + r >= M || n0 + c >= N) continue;
         float v = 0.f;
@@ -757,9 +809,8 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
     const unsigned char *b = (const unsigned char*)b_codes, *bs = (const unsigned char*)b_scales;
     const unsigned mt = (unsigned)p.mt, nt = (unsigned)p.nt;
     if (p.tile == 0) {
-#define MX4_ROWS(NW) \
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((mx4_gemm_kernel<T, NW>), dim3(mt* nt), dim3(NW * 64), 0, ST(stream), a, as, M, b, bs, N, (int)G, bias, (T*)y, nt))
-        MX4_ROWS(4);
+        MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((mx4_gemm_kernel<T, float, false, 4>), dim3(mt* nt), dim3(256), 0, ST(stream), a, as, M, cols, b, bs, N,
+                                                (int)G, bias, (T*)y, nt));
         return msfwsi_launch_status();
     }
     float* sums = p.splits > 1 ? (float*)workspace : nullptr;
@@ -775,18 +826,34 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
     return msfwsi_launch_status();
 }
 
-// workspace of a linear call: x's codes, its scales, the partial sums
+// workspace of a linear call: x's codes, its scales, the partial sums; a single row needs none
 extern "C" int msfwsi_mx4_linear_workspace(long M, long N, long cols, long* bytes) {
     const int rc = msfwsi_mx4_gemm_workspace(M, N, cols, bytes);
-    if (rc == MSFWSI_OK) *bytes += groups_of(cols) * M * kGroupBytes + round16(groups_of(cols) * M * 8);
+    if (rc == MSFWSI_OK) *bytes = M == 1 ? 0 : *bytes + groups_of(cols) * M * kGroupBytes + round16(groups_of(cols) * M * 8);
     return rc;
+}
+
+template <typename TX>
+static void launch_row(int y_dtype, const void* x, const void* codes, const void* scales, long N, long cols, const float* bias, void* y, void* stream) {
+    const unsigned nt = (unsigned)((N + 31) / 32);
+    MSFWSI_WITH_T(y_dtype, hipLaunchKernelGGL((mx4_gemm_kernel<T, TX, true, 4>), dim3(nt), dim3(256), 0, ST(stream), x, (const unsigned char*)nullptr, 1L, cols,
+                                              (const unsigned char*)codes, (const unsigned char*)scales, N, (int)groups_of(cols), bias, (T*)y, nt));
 }
 
 extern "C" int msfwsi_mx4_linear(int dtype, const void* x, long ld, long M, const void* codes, const void* scales, long N, long cols,
                                  const float* bias, int y_dtype, void* y, void* workspace, void* stream) {
-    MSFWSI_CHECK_ARG(msfwsi_dtype_ok(y_dtype) && M >= 0 && N > 0 && cols > 0);
+    MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && msfwsi_dtype_ok(y_dtype) && M >= 0 && N > 0 && cols > 0);
     if (M == 0) return MSFWSI_OK;
-    MSFWSI_CHECK_ARG(codes && scales && y && workspace && aligned16(workspace));
+    MSFWSI_CHECK_ARG(codes && scales && y);
+    if (M == 1) {
+        MSFWSI_CHECK_ARG(x && aligned16(codes) && aligned16(scales));
+        if (N > (1L << 21) || groups_of(cols) > 0x7fffffffL) return MSFWSI_EUNSUPPORTED;
+        if (dtype == MSFWSI_DT_BF16) launch_row<__bf16>(y_dtype, x, codes, scales, N, cols, bias, y, stream);
+        else if (dtype == MSFWSI_DT_F16) launch_row<_Float16>(y_dtype, x, codes, scales, N, cols, bias, y, stream);
+        else launch_row<float>(y_dtype, x, codes, scales, N, cols, bias, y, stream);
+        return msfwsi_launch_status();
+    }
+    MSFWSI_CHECK_ARG(workspace && aligned16(workspace));
     char* xc = (char*)workspace;
     char* xs = xc + groups_of(cols) * M * kGroupBytes;
     const int rc = msfwsi_mx4_quantize(dtype, x, ld, M, cols, xc, xs, stream);

@@ -177,6 +177,25 @@ def test_linear_of_quantized_input_and_other_output_type(hip_lib, out):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("K,N", [(1, 1), (31, 5), (257, 33), (1001, 1537), (4608, 64)])
+def test_one_row_is_a_row_of_many(hip_lib, dt, K, N):
+    """a single row takes a path of its own: the same 4-bit values as the same row among others, NaN blocks included"""
+    from msf_wsi_amd import quant
+
+    x = features(3, K, FP[dt], K + N).cuda()
+    w4 = quant.quantize_mx4(features(N, K, torch.float32, 5).cuda())
+    many = quant.mx4_linear(x, w4, out_dtype=torch.float32)
+    one = quant.mx4_linear(x[1:2], w4, out_dtype=torch.float32)
+    mass = quant.quantize_mx4(x).dequantize().double().abs() @ w4.dequantize().double().abs().t()
+    assert bool(((one.double() - many[1:2].double()).abs() <= 2 * (K + 8) * 2.0 ** -23 * mass[1:2]).all())
+    assert torch.equal(quant.mx4_linear(x[1], w4, out_dtype=torch.float32), one[0])
+    bad = x[1:2].clone()
+    bad[0, K // 2] = math.inf
+    assert quant.mx4_linear(bad, w4).isnan().all()
+
+
+@pytest.mark.gpu
 def test_weights_of_very_different_size(hip_lib):
     """scales up to 2^100 apart, in both operands' directions: every block's own scale counts"""
     from msf_wsi_amd import quant
