@@ -60,16 +60,27 @@ __device__ __forceinline__ void store8(T* __restrict__ p, long left, const float
         if (e < left) store_elem<T>(p, e, f[e]);
 }
 
-// the scale code of a block whose largest magnitude has the bits `big`, and 2^(127 - E)
-__device__ __forceinline__ float block_scale(unsigned big, unsigned& E) {
+// 8 elements of a block whose other 24 are in the neighbouring lanes (4 lanes from a multiple of 4): their codes, the block's E.
+// The conversion's own scale operand stays 1: the elements are multiplied by 2^(127 - E) first, which is exact.
+__device__ __forceinline__ unsigned quantize8(const float* f, unsigned& E) {
+    unsigned big = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(f[e]) & 0x7fffffffu);  // orders like the magnitudes, NaN on top
+    big = max(big, (unsigned)__shfl_xor((int)big, 1, 64));
+    big = max(big, (unsigned)__shfl_xor((int)big, 2, 64));
     const unsigned field = big >> 23;
     E = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
-    return __uint_as_float((254u - (E == 255u ? 127u : E)) << 23);
+    const float up = __uint_as_float((254u - (E == 255u ? 127u : E)) << 23);  // 2^(127 - E)
+    unsigned w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0] * up, f[1] * up, 1.f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2] * up, f[3] * up, 1.f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4] * up, f[5] * up, 1.f, 2);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6] * up, f[7] * up, 1.f, 3);
+    return E == 255u ? 0u : w;
 }
 
-// One half-wave (32 lanes x 8 elements) per group of a row, UG groups one after the other with their loads in flight together; a
-// block of 32 elements is 4 lanes.  The conversion's own scale operand stays 1: the elements are multiplied by 2^(127 - E) first,
-// which is exact.  Bound by memory.
+// One half-wave (32 lanes x 8 elements) per group of a row, UG groups one after the other with their loads in flight together.
+// Bound by memory.
 constexpr int UG = 4;
 template <typename T>
 __global__ void __launch_bounds__(kT) mx4_quantize_kernel(const T* __restrict__ x, long ld, long rows, long cols, int G,
@@ -87,19 +98,8 @@ __global__ void __launch_bounds__(kT) mx4_quantize_kernel(const T* __restrict__ 
     for (int u = 0; u < UG; ++u) {
         if (g0 + u >= G) return;
         const long at = (long)(g0 + u) * rows + r;
-        unsigned big = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(f[u][e]) & 0x7fffffffu);  // orders like the magnitudes, NaN on top
-        big = max(big, (unsigned)__shfl_xor((int)big, 1, 64));
-        big = max(big, (unsigned)__shfl_xor((int)big, 2, 64));
         unsigned E;
-        const float up = block_scale(big, E);
-        unsigned w = 0;
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][0] * up, f[u][1] * up, 1.f, 0);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][2] * up, f[u][3] * up, 1.f, 1);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][4] * up, f[u][5] * up, 1.f, 2);
-        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[u][6] * up, f[u][7] * up, 1.f, 3);
-        codes[at * 32 + l] = E == 255u ? 0u : w;
+        codes[at * 32 + l] = quantize8(f[u], E);
         unsigned word = 0;  // lane 0 / 1 collects the scale bytes of blocks 0-3 / 4-7
 #pragma unroll
         for (int j = 0; j < 4; ++j) word |= (unsigned)__shfl((int)E, (threadIdx.x & 32) + (l & 1) * 16 + j * 4, 64) << (8 * j);
@@ -172,88 +172,113 @@ __device__ __forceinline__ void mx4_step(f32x16& acc, const int4& a, int sa, con
                                                           acc, 4, 4, S, sa, S, sb);
 }
 
-// Few rows: 32 x 32 outputs per workgroup straight from memory, the groups dealt over its NW waves and joined in LDS.  Bound
-// by reading b once (18432 x 18432 at one row: FEWUS); nothing is shared between workgroups, so nothing is staged.  The next
-// group's loads are on their way while one is multiplied.
-// ROW: a single row, which comes as it is (TX) and is quantised by the wave that needs it, so that one launch does it all: 4
-// elements a lane, a block of 32 is 8 lanes; the codes pass through 128 bytes of LDS into the operand's order.
-template <typename T, typename TX, bool ROW, int NW>
+// Few rows (up to 16 FA): 16 columns per workgroup straight from memory, the groups dealt over its NW waves and joined in LDS.
+// Bound by reading b once; nothing is shared between workgroups, so nothing is staged, and the next group's loads are on their
+// way while one is multiplied.  16 columns, because a CU's share is a whole number of workgroups: 576 of 32 columns on 256 CUs
+// (18432 rows of b) took 51 us, 1152 of 16 take 40.
+// A 16x16x128 step takes 32 elements from each lane; quarter q of the wave takes blocks 2q, 2q + 1 of a group in its two steps.
+// ROW: a single row of up to kRowGroups groups, which comes as it is (TX) and is quantised by every workgroup for itself, so that one
+// launch does it all; the codes wait in LDS.  (One group after the other, with its loads waited for, this took 13 us.)
+constexpr int kRowGroups = 128;
+template <int S>
+__device__ __forceinline__ void mx4_step16(f32x4& acc, const int4& a, int sa, const int4& b, int sb) {
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4((i32x8){a.x, a.y, a.z, a.w, 0, 0, 0, 0}, (i32x8){b.x, b.y, b.z, b.w, 0, 0, 0, 0},
+                                                           acc, 4, 4, S, sa, S, sb);
+}
+template <typename T, typename TX, bool ROW, int FA, int NW>
 __global__ void __launch_bounds__(NW * 64) mx4_gemm_kernel(const void* __restrict__ a, const unsigned char* __restrict__ as, long M, long cols,
                                                            const unsigned char* __restrict__ b, const unsigned char* __restrict__ bs, long N,
-                                                           int G, const float* __restrict__ bias, T* __restrict__ y, unsigned nt) {
-    __shared__ float part[NW][ROW ? 32 : 32 * 33];
-    __shared__ __attribute__((aligned(16))) unsigned char own[NW][kGroupBytes + 16];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, h = lane >> 5;
-    const long m0 = ROW ? 0 : (long)(blockIdx.x / nt) * 32, n0 = (long)(ROW ? blockIdx.x : blockIdx.x % nt) * 32;
-    const long m = min(m0 + (lane & 31), M - 1), n = min(n0 + (lane & 31), N - 1);
+                                                           int G, const float* __restrict__ bias, T* __restrict__ y) {
+    __shared__ float part[NW][ROW ? 16 : FA * 16 * 17];
+    __shared__ __attribute__((aligned(16))) unsigned char own[ROW ? kRowGroups * (kGroupBytes + 16) : 16];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, l = lane & 15;
+    const long n0 = blockIdx.x * 16L, n = min(n0 + l, N - 1);
     struct Operands {
-        int4 a[4], b[4];
-        int sa, sb;
-        float x[4];
-    } cur, nxt;
+        int4 a[FA][2], b[2];
+        int sa[FA], sb;
+    } first, second;
     auto load = [&](int g, Operands& o) {
+        if constexpr (!ROW) {
+#pragma unroll
+            for (int i = 0; i < FA; ++i) {
+                const long ra = g * M + min(i * 16L + l, M - 1);
+                o.sa[i] = *reinterpret_cast<const unsigned short*>(as + ra * 8 + q * 2);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+                    o.a[i][s] = *reinterpret_cast<const int4*>(reinterpret_cast<const unsigned char*>(a) + ra * kGroupBytes + (2 * q + s) * 16);
+            }
+        }
         const long rb = g * N + n;
-        o.sb = *reinterpret_cast<const int*>(bs + rb * 8 + h * 4);
+        o.sb = *reinterpret_cast<const unsigned short*>(bs + rb * 8 + q * 2);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) o.b[s] = *reinterpret_cast<const int4*>(b + rb * kGroupBytes + (4 * h + s) * 16);
+        for (int s = 0; s < 2; ++s) o.b[s] = *reinterpret_cast<const int4*>(b + rb * kGroupBytes + (2 * q + s) * 16);
+    };
+    f32x4 acc[FA];
+#pragma unroll
+    for (int i = 0; i < FA; ++i) acc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](int g, Operands& o) {
         if constexpr (ROW) {
-            const long c = g * (long)kGroup + lane * 4;
+            const unsigned char* x = own + g * (kGroupBytes + 16);
+            o.sa[0] = *reinterpret_cast<const unsigned short*>(x + kGroupBytes + q * 2);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o.x[e] = c + e < cols ? load_elem<TX>(reinterpret_cast<const TX*>(a), c + e) : 0.f;
-        } else {
-            const long ra = g * M + m;
-            o.sa = *reinterpret_cast<const int*>(as + ra * 8 + h * 4);
+            for (int s = 0; s < 2; ++s) o.a[0][s] = *reinterpret_cast<const int4*>(x + (2 * q + s) * 16);
+        }
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
-                o.a[s] = *reinterpret_cast<const int4*>(reinterpret_cast<const unsigned char*>(a) + ra * kGroupBytes + (4 * h + s) * 16);
+        for (int i = 0; i < FA; ++i) {
+            mx4_step16<0>(acc[i], o.a[i][0], o.sa[i], o.b[0], o.sb);
+            mx4_step16<1>(acc[i], o.a[i][1], o.sa[i], o.b[1], o.sb);
         }
     };
-    auto quantize = [&](Operands& o) {
-        unsigned big = 0;
+    load(min(w, G - 1), first);
+    if constexpr (ROW) {  // half a wave per group, 8 elements a lane (mx4_quantize_kernel), all loads of five groups in flight
+        constexpr int H = 2 * NW, U = 5;
+        const int hl = threadIdx.x & 31;
+        for (int g = threadIdx.x >> 5; g < G; g += H * U) {
+            float f[U][8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) big = max(big, __float_as_uint(o.x[e]) & 0x7fffffffu);
+            for (int u = 0; u < U; ++u) {
+                const long c = (g + u * H) * (long)kGroup + hl * 8;
+                load8<TX>(reinterpret_cast<const TX*>(a) + c, cols - c, f[u]);
+            }
 #pragma unroll
-        for (int off = 1; off < 8; off <<= 1) big = max(big, (unsigned)__shfl_xor((int)big, off, 64));
-        unsigned E;
-        const float up = block_scale(big, E);
-        unsigned c = 0;
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, o.x[0] * up, o.x[1] * up, 1.f, 0);
-        c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, o.x[2] * up, o.x[3] * up, 1.f, 1);
-        // a wave's LDS instructions run in order: no barrier, but hipcc has to keep them so too
-        *reinterpret_cast<unsigned short*>(&own[w][lane * 2]) = (unsigned short)(E == 255u ? 0u : c);
-        if ((lane & 7) == 0) own[w][kGroupBytes + (lane >> 3)] = (unsigned char)E;
-        asm volatile("" ::: "memory");
-        o.sa = *reinterpret_cast<const int*>(&own[w][kGroupBytes + h * 4]);
-#pragma unroll
-        for (int s = 0; s < 4; ++s) o.a[s] = *reinterpret_cast<const int4*>(&own[w][(4 * h + s) * 16]);
-        asm volatile("" ::: "memory");
-    };
-    f32x16 acc = {0.f};
-    if (w < G) load(w, cur);
-    for (int g = w; g < G; g += NW) {
-        load(min(g + NW, G - 1), nxt);
-        if constexpr (ROW) quantize(cur);
-        mx4_step<0>(acc, cur.a[0], cur.sa, cur.b[0], cur.sb);
-        mx4_step<1>(acc, cur.a[1], cur.sa, cur.b[1], cur.sb);
-        mx4_step<2>(acc, cur.a[2], cur.sa, cur.b[2], cur.sb);
-        mx4_step<3>(acc, cur.a[3], cur.sa, cur.b[3], cur.sb);
-        cur = nxt;
+            for (int u = 0; u < U; ++u) {
+                if (g + u * H >= G) break;
+                unsigned E;
+                const unsigned code = quantize8(f[u], E);
+                unsigned char* x = own + (g + u * H) * (kGroupBytes + 16);
+                *reinterpret_cast<unsigned*>(x + hl * 4) = code;
+                if ((hl & 3) == 0) x[kGroupBytes + (hl >> 2)] = (unsigned char)E;
+            }
+        }
+        __syncthreads();
     }
-    if constexpr (ROW) {  // all 32 rows of the operand are this one
-        if (lane < 32) part[w][lane] = acc[0];
+    int g = w;
+    for (; g + NW < G; g += 2 * NW) {  // two sets of registers in turn: a copy from one to the other would wait for its loads
+        load(g + NW, second);
+        __builtin_amdgcn_sched_barrier(0);  // and neither set's loads move behind the other's products
+        multiply(g, first);
+        load(min(g + 2 * NW, G - 1), first);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(g + NW, second);
+    }
+    if (g < G) multiply(g, first);
+    if constexpr (ROW) {  // all 16 rows of the operand are this one
+        if (lane < 16) part[w][lane] = acc[0][0];
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) part[w][((i & 3) + 8 * (i >> 2) + 4 * h) * 33 + (lane & 31)] = acc[i];
+        for (int i = 0; i < FA; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[w][(i * 16 + q * 4 + e) * 17 + l] = acc[i][e];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < (ROW ? 32 : 1024); i += NW * 64) {
-        const int r = i >> 5, c = i & 31;
-        if (m0 + r >= M || n0 + c >= N) continue;
+    for (int i = threadIdx.x; i < (ROW ? 16 : FA * 256); i += NW * 64) {
+        const int r = i >> 4, c = i & 15;
+        if (r >= M || n0 + c >= N) continue;
         float v = 0.f;
 #pragma unroll
-        for (int q = 0; q < NW; ++q) v += part[q][r * 33 + c];
+        for (int p = 0; p < NW; ++p) v += part[p][r * 17 + c];
         if (bias != nullptr) v += bias[n0 + c];
-        store_elem<T>(y, (m0 + r) * N + n0 + c, v);
+        store_elem<T>(y, r * N + n0 + c, v);
     }
 }
 
@@ -711,8 +736,9 @@ struct GemmPlan {
     int splits, per_split;
 };
 constexpr long kCus = 256;
+constexpr int NWR = 8;  // waves that share 16 columns of few rows
 GemmPlan gemm_plan(long M, long N, long G) {
-    GemmPlan p = {0, (M + 31) / 32, (N + 31) / 32, 1, (int)G};
+    GemmPlan p = {0, 1, (N + 15) / 16, 1, (int)G};
     if (M <= 32) return p;
     const long big = ((M + 255) / 256) * ((N + 255) / 256);
     p.tile = big >= kCus ? 256 : 128;
@@ -809,8 +835,11 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
     const unsigned char *b = (const unsigned char*)b_codes, *bs = (const unsigned char*)b_scales;
     const unsigned mt = (unsigned)p.mt, nt = (unsigned)p.nt;
     if (p.tile == 0) {
-        MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((mx4_gemm_kernel<T, float, false, 4>), dim3(mt* nt), dim3(256), 0, ST(stream), a, as, M, cols, b, bs, N,
-                                                (int)G, bias, (T*)y, nt));
+#define MX4_ROWS(FA)                                                                                                                           \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((mx4_gemm_kernel<T, float, false, FA, NWR>), dim3(nt), dim3(NWR * 64), 0, ST(stream), a, as, M, cols, b, \
+                                            bs, N, (int)G, bias, (T*)y))
+        if (M <= 16) MX4_ROWS(1);
+        else MX4_ROWS(2);
         return msfwsi_launch_status();
     }
     float* sums = p.splits > 1 ? (float*)workspace : nullptr;
@@ -829,15 +858,15 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
 // workspace of a linear call: x's codes, its scales, the partial sums; a single row needs none
 extern "C" int msfwsi_mx4_linear_workspace(long M, long N, long cols, long* bytes) {
     const int rc = msfwsi_mx4_gemm_workspace(M, N, cols, bytes);
-    if (rc == MSFWSI_OK) *bytes = M == 1 ? 0 : *bytes + groups_of(cols) * M * kGroupBytes + round16(groups_of(cols) * M * 8);
+    if (rc == MSFWSI_OK) *bytes = M == 1 && groups_of(cols) <= kRowGroups ? 0 : *bytes + groups_of(cols) * M * kGroupBytes + round16(groups_of(cols) * M * 8);
     return rc;
 }
 
 template <typename TX>
 static void launch_row(int y_dtype, const void* x, const void* codes, const void* scales, long N, long cols, const float* bias, void* y, void* stream) {
-    const unsigned nt = (unsigned)((N + 31) / 32);
-    MSFWSI_WITH_T(y_dtype, hipLaunchKernelGGL((mx4_gemm_kernel<T, TX, true, 4>), dim3(nt), dim3(256), 0, ST(stream), x, (const unsigned char*)nullptr, 1L, cols,
-                                              (const unsigned char*)codes, (const unsigned char*)scales, N, (int)groups_of(cols), bias, (T*)y, nt));
+    MSFWSI_WITH_T(y_dtype, hipLaunchKernelGGL((mx4_gemm_kernel<T, TX, true, 1, NWR>), dim3((unsigned)((N + 15) / 16)), dim3(NWR * 64), 0, ST(stream), x,
+                                              (const unsigned char*)nullptr, 1L, cols, (const unsigned char*)codes, (const unsigned char*)scales, N,
+                                              (int)groups_of(cols), bias, (T*)y));
 }
 
 extern "C" int msfwsi_mx4_linear(int dtype, const void* x, long ld, long M, const void* codes, const void* scales, long N, long cols,
@@ -845,9 +874,9 @@ extern "C" int msfwsi_mx4_linear(int dtype, const void* x, long ld, long M, cons
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && msfwsi_dtype_ok(y_dtype) && M >= 0 && N > 0 && cols > 0);
     if (M == 0) return MSFWSI_OK;
     MSFWSI_CHECK_ARG(codes && scales && y);
-    if (M == 1) {
+    if (M == 1 && groups_of(cols) <= kRowGroups) {
         MSFWSI_CHECK_ARG(x && aligned16(codes) && aligned16(scales));
-        if (N > (1L << 21) || groups_of(cols) > 0x7fffffffL) return MSFWSI_EUNSUPPORTED;
+        if (N > (1L << 21)) return MSFWSI_EUNSUPPORTED;
         if (dtype == MSFWSI_DT_BF16) launch_row<__bf16>(y_dtype, x, codes, scales, N, cols, bias, y, stream);
         else if (dtype == MSFWSI_DT_F16) launch_row<_Float16>(y_dtype, x, codes, scales, N, cols, bias, y, stream);
         else launch_row<float>(y_dtype, x, codes, scales, N, cols, bias, y, stream);
