@@ -31,6 +31,7 @@ constexpr int kMaxK = 64;        // = the lanes of a wave: lane i holds entry i 
 constexpr int kMaxParts = 8192;  // workgroups of the forward at most; each leaves one (sum, count) pair
 constexpr int kCand = 512;       // candidates a selection ranks at once
 constexpr int kQueue = 256;      // chunks with candidates it can hold
+static_assert(kCand * sizeof(long) <= kQueue * sizeof(uint4), "the sorted candidates take the queue's place");
 constexpr int kSeg = 65536;      // classes whose list membership is held as bits at a time
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -141,7 +142,8 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int c, int n, con
 // one wave bit by bit with ballots.  Chunks that hold anything not below it -- barely more than k unless large logits crowd
 // into few threads or tie -- go to a queue, whose elements the threads then look at one by one (nearly every wave meets such a
 // chunk at nearly every step: looking at them in place cost all lanes the walk twice over, 166 us instead of 149); what is
-// not below the bound goes into a list and is ranked by counting.  Everything else is summed for `rest`.
+// not below the bound goes into a list and is ranked by counting.  Everything else is summed for `rest`, each thread its own and the
+// list's surplus once it is in order: the lists fill in any order, no sum depends on it.
 // A queue or list that runs over (long ties, a masked-out segment) sends the segment through k rounds of a plain maximum instead.
 // Rows longer than a segment leave their segments' lists and sums to a merge.
 // ---------------------------------------------------------------------------------------------------------------------
@@ -212,9 +214,12 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(cons
 #pragma unroll
         for (int e = 1; e < VEC; ++e) high = fmaxf(high, f[e]);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) part += exp2_(fmaf(f[e], c, shift));
+        for (int e = 0; e < VEC; ++e) {
+            const float x2 = exp2_(fmaf(f[e], c, shift));
+            part += f[e] >= lim ? 0.f : x2;
+        }
         const bool queue_it = !(high < lim);
-        s += queue_it ? 0.f : part;
+        s += part;
         if (queue_it) {
             const int slot = atomicAdd(&queued, 1);
             if (slot < kQueue) queue[slot] = raw[j], queue_at[slot] = (j * NT + t) * VEC;
@@ -227,9 +232,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(cons
             const int at = queue_at[i / VEC] + i % VEC;
             const float v = load_elem<T>(reinterpret_cast<const T*>(queue), i);
             if (at >= n) continue;
-            if (v < lim) {
-                s += exp2_(fmaf(v, c, shift));
-            } else {
+            if (!(v < lim)) {
                 const int slot = atomicAdd(&count, 1);
                 if (slot < kCand) cand[slot] = key_of(v, c0 + at);
             }
@@ -241,20 +244,27 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(cons
     // The list decides when it holds every candidate.  The sum decides unless a NaN went by in it, or it is so small against its
     // reference that terms of it may have been flushed
     if (chunks <= kQueue && got <= kCand && (got >= n || below.s >= 1e-30f)) {
+        long* sorted = reinterpret_cast<long*>(queue);  // which has been read
         for (int i = t; i < got; i += NT) {
             const long key = cand[i];
             int rank = 0;
             for (int q = 0; q < got; ++q) rank += cand[q] > key;
-            if (rank >= want) {
+            sorted[rank] = key;
+        }
+        __syncthreads();
+        for (int i = t; i < got; i += NT) {
+            const long key = sorted[i];
+            if (i >= want) {
                 left = join(left, one(value_of((int)(key >> 32))), c);
             } else if (nseg == 1) {
-                values[row * k + rank] = value_of((int)(key >> 32));
-                indices[row * k + rank] = index_of(key);
+                values[row * k + i] = value_of((int)(key >> 32));
+                indices[row * k + i] = index_of(key);
             } else {
-                keys_out[rank] = key;
+                keys_out[i] = key;
             }
         }
-        left = join(below, block_join<NT>(left, buf, c), c);
+        left = block_join<NT>(left, buf, c);
+        if (got < n) left = join(below, left, c);  // else there is nothing below, and a NaN in that sum is a candidate
     } else {
         long last = 0x7fffffffffffffffL;
         for (int r = 0; r < want; ++r) {
@@ -314,7 +324,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(cons
         for (int r = want + t; r < k; r += NT) keys_out[r] = kNoKey;
 }
 
-// The segments' lists of a row become one: every entry's rank is counted (33 us as rounds over the lists' heads, 5 so, at
+// The segments' lists of a row become one: every entry's rank is counted (33 us as rounds over the lists' heads, 15 so, at
 // 4096 rows of 4 x 32); what is not among the k joins `rest`.
 constexpr int kMergeHeld = 2048;
 __global__ void __launch_bounds__(kT) top_merge_kernel(const long* __restrict__ part_keys, const Sum* __restrict__ part_sums, int nseg, int k,

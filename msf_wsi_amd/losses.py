@@ -106,8 +106,8 @@ def _logit_view(logits: torch.Tensor, dim: int) -> torch.Tensor:
 
 def _temperature(t: float) -> float:
     t = float(t)
-    if not (0.0 < t < float("inf")):
-        raise ValueError(f"temperature must be positive and finite, got {t}")
+    if not 1e-6 <= t <= 1e6:  # so that 1 / T and T^2 stay far inside float32
+        raise ValueError(f"temperature must lie within 1e-6 ... 1e6, got {t}")
     return t
 
 

@@ -174,6 +174,72 @@ def test_top_logits_maps(hip_lib, dt, shape, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+def test_top_logits_repeat_bit_for_bit(hip_lib, dt):
+    """also where many candidates compete for places (coarse values: ties everywhere)"""
+    from msf_wsi_amd import losses
+
+    x = torch.cat([logits_of(40, 30011, FP[dt], 5), (logits_of(40, 30011, torch.float32, 6) * 4).round().to(FP[dt])]).cuda()
+    first = losses.top_logits(x, 48, 2.0)
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(first, losses.top_logits(x, 48, 2.0)))
+
+
+@pytest.mark.gpu
+def test_masks_of_the_lowest_value(hip_lib):
+    """logits masked with the type's lowest number instead of -inf: as -inf beside others, uniform where nothing else is left"""
+    from msf_wsi_amd import losses
+
+    for dt in FP.values():
+        low = torch.finfo(dt).min
+        z = torch.full((3, 900), low, dtype=dt)
+        z[0, 3:9], z[1] = 0.5, -math.inf
+        z[1, 7] = 1.0
+        top = losses.top_logits(z.cuda(), 4, 2.0)
+        assert top.indices.tolist() == [[3, 4, 5, 6], [7, 0, 1, 2], [0, 1, 2, 3]]
+        assert abs(float(top.rest[0]) - (0.25 + math.log(2))) < 1e-6 and float(top.rest[1]) == -math.inf
+        teacher = losses.TopLogits(torch.zeros(3, 2, device="cuda"), torch.tensor([[3, 4]] * 3, dtype=torch.int32, device="cuda"))
+        zc = z[[0, 2]].cuda().requires_grad_()
+        crit = losses.TopLogitDistillLoss(2.0, "none")
+        row = crit(zc, losses.TopLogits(*(t[:2] for t in teacher[:2])))
+        want = [4.0 * math.log(6 / 2), 4.0 * math.log(900 / 2)]      # T^2 (log 1/2 - log q) with q = 1/6, 1/900
+        assert all(abs(a - b) < 1e-4 for a, b in zip(row.tolist(), want))
+        g, = torch.autograd.grad(row, zc, torch.ones(2, device="cuda"))
+        # A probability is a product of two powers of 2 whose exponents hold log2(s), s up to 900: at most 1.5 steps of 2^-20 off (one
+        # of the logarithm, half of its rounding), so 1.5 ln 2 2^-20; the two powers, a step of 2^-23 each, and four roundings of
+        # 2^-24 follow.  Together under 13 2^-23 of the value.  The teacher's 1/2 has log2(2) in its exponent: under 4 2^-23.
+        half, f32 = torch.finfo(dt).eps / 2, 2.0 ** -23
+        assert abs(float(g[1, 10]) - 2.0 / 900) <= (half + 13 * f32) * 2.0 / 900
+        assert abs(float(g[1, 3]) - 2.0 * (1 / 900 - 0.5)) <= half + 4 * f32
+        assert float(g[0, 10]) == 0.0 and abs(float(g[0, 8]) - 2.0 / 6) <= (half + 13 * f32) / 3
+
+
+@pytest.mark.gpu
+def test_offsets_past_31_bits(hip_lib):
+    """33000 x 65600 bf16 logits (4.3 GB): the last rows, and the rows either side of 2^31 elements, as in a small tensor"""
+    from msf_wsi_amd import losses
+
+    rows, C = 33000, 65600
+    z = torch.zeros(rows, C, dtype=torch.bfloat16, device="cuda")
+    pick = [0, 32734, 32735, 32736, rows - 1]
+    z[pick] = logits_of(5, C, torch.bfloat16, 77).cuda()
+    small = z[pick].clone()
+    big, few = losses.top_logits(z, 6, 2.0), losses.top_logits(small, 6, 2.0)
+    assert all(torch.equal(a[pick], b) for a, b in zip(big, few))
+    del big
+    teacher = losses.TopLogits(few.values.new_zeros(rows, 6), few.indices.new_zeros(rows, 6), None)
+    teacher.values[pick], teacher.indices[pick] = few.values, few.indices
+    mask = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    mask[pick] = True
+    crit = losses.TopLogitDistillLoss(2.0, "sum")
+    zr, sr = z.requires_grad_(), small.requires_grad_()
+    a, b = crit(zr, teacher, mask), crit(sr, losses.TopLogits(few.values, few.indices))
+    assert abs(a.item() - b.item()) <= 4 * U * abs(b.item())
+    ga, gb = torch.autograd.grad(a, zr)[0], torch.autograd.grad(b, sr)[0]
+    assert torch.equal(ga[pick], gb) and float(ga[1].abs().max()) == 0.0
+
+
+@pytest.mark.gpu
 def test_top_logits_slices_and_refusals(hip_lib):
     from msf_wsi_amd import losses
 
