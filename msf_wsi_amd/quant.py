@@ -72,7 +72,8 @@ def quantize_mx4(x: torch.Tensor) -> MX4Tensor:
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, out_dtype):
-        ctx.weight, ctx.like = weight, (x.shape, x.dtype)
+        ctx.save_for_backward(weight.codes, weight.scales)
+        ctx.like = (x.shape, x.dtype)
         rows = _matrix(x, "mx4_linear")
         y = torch.empty(rows.shape[0], weight.shape[0], dtype=out_dtype, device=x.device)
         kn.mx4_linear(rows, weight.codes, weight.scales, y, bias)
@@ -81,10 +82,11 @@ class _LinearFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        codes, scales = ctx.saved_tensors
         shape, dtype = ctx.like
         dy = _matrix(dy, "mx4_linear backward")
         dx = torch.empty(dy.shape[0], shape[-1], dtype=dtype, device=dy.device)
-        kn.mx4_dgrad(dy, ctx.weight.codes, ctx.weight.scales, dx)
+        kn.mx4_dgrad(dy, codes, scales, dx)
         return dx if len(shape) == 2 else dx.view(shape), None, None, None
 
 

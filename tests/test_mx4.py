@@ -348,6 +348,43 @@ def test_refusals(hip_lib):
 
 
 @pytest.mark.gpu
+def test_offsets_past_31_bits(hip_lib):
+    """70000 x 32000 bf16 (4.5 GB): quantised, widened and multiplied, the last rows as in a small tensor"""
+    from msf_wsi_amd import quant
+
+    x = torch.zeros(70000, 32000, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = features(3, 32000, torch.bfloat16, 1).cuda()
+    q, few = quant.quantize_mx4(x), quant.quantize_mx4(x[-3:].clone())
+    assert torch.equal(q.codes[:, -3:], few.codes) and torch.equal(q.scales[:, -3:], few.scales)
+    assert torch.equal(q.dequantize(torch.bfloat16)[-3:], few.dequantize(torch.bfloat16))
+    w4 = quant.quantize_mx4(features(40, 32000, torch.float32, 2).cuda() / 200)
+    y, want = quant.mx4_linear(q, w4)[-3:].double(), quant.mx4_linear(few, w4).double()
+    mass = few.dequantize().double().abs() @ w4.dequantize().double().abs().t()
+    assert bool(((y - want).abs() <= 2 * 32008 * 2.0 ** -23 * mass).all())
+    del x, q
+    dy = torch.zeros(70000, 40, dtype=torch.bfloat16, device="cuda")
+    dy[-3:] = 1.0
+    w = quant.MX4Tensor(w4.codes, w4.scales, 32000)
+    xr = torch.zeros(70000, 32000, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    dx, = torch.autograd.grad(quant.mx4_linear(xr, w), xr, dy)
+    small, = torch.autograd.grad(quant.mx4_linear(xr[-3:], w), xr, torch.ones(3, 40, dtype=torch.bfloat16, device="cuda"))
+    assert torch.equal(dx[-3:], small[-3:]) and float(dx[0].abs().max()) == 0.0
+
+
+@pytest.mark.gpu
+def test_changed_weights_are_noticed(hip_lib):
+    """the gradient of a weight that was overwritten after the forward is refused, not computed from the new values"""
+    from msf_wsi_amd import quant
+
+    w4 = quant.quantize_mx4(torch.ones(8, 64, device="cuda"))
+    x = torch.ones(2, 64, device="cuda", requires_grad=True)
+    y = quant.mx4_linear(x, w4)
+    w4.codes.zero_()
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+
+
+@pytest.mark.gpu
 def test_module_and_state(hip_lib):
     from msf_wsi_amd import quant
 
