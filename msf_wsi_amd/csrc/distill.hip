@@ -947,14 +947,16 @@ extern "C" int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, 
         return msfwsi_launch_status();
     }
     const int nseg = segments(dtype, classes);
-    if (nseg > 4096 || outer > 0xffffffL / nseg) return MSFWSI_EUNSUPPORTED;  // heads of a merge in LDS; a grid holds < 2^32 threads
+    const bool narrow = classes <= 64 * 4 * msfwsi_vec_of(dtype);
+    // heads of a merge in LDS; a grid holds < 2^32 threads
+    if (nseg > 4096 || outer > 0xffffffffL / ((narrow ? 64 : 256) * (long)nseg)) return MSFWSI_EUNSUPPORTED;
     MSFWSI_CHECK_ARG(nseg == 1 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0));
     long* keys = (long*)workspace;
     Sum* sums = (Sum*)(keys + outer * nseg * (long)k);
 #define TOP_ROWS(NT, NCH)                                                                                                            \
     MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((top_segment_kernel<T, NT, NCH>), dim3((unsigned)(outer * nseg)), dim3(NT), 0, ST(stream), \
                                             (const T*)x, ld, classes, nseg, k, inv_t, values, indices, rest, keys, sums))
-    if (classes <= 64 * 4 * msfwsi_vec_of(dtype)) TOP_ROWS(64, 4);
+    if (narrow) TOP_ROWS(64, 4);
     else TOP_ROWS(256, 8);
     const int rc = msfwsi_launch_status();
     if (rc != MSFWSI_OK || nseg == 1) return rc;

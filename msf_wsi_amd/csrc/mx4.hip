@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy,
 // by DMA like the tiles above; W's codes (8 KB a step) are widened to 16 bits on the way into LDS [n][column] and read transposed
 // (ds_read_b64_tr_b16), even and odd columns apart as above.  The scale of a weight varies along the sum, so it is applied while widening -- relative to the
 // largest scale of its 32 columns over this workgroup's rows of W, which the outputs are multiplied with in the end:
-// nothing can overflow, and bf16 keeps weights down to 2^-126 of the largest.  fp16 holds scales that are at most 2^26 apart
+// no weight can overflow, and bf16 keeps weights down to 2^-126 of the largest.  fp16 holds scales that are at most 2^26 apart
 // exactly; where a workgroup finds them further apart it cuts each dy value into two bf16 parts (8 + 3 bits) instead.
 template <typename T, bool CUT>
 __device__ __forceinline__ void dgrad_mma(f32x16& acc, const uint4& a, const uint4& b) {
@@ -572,7 +572,7 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
     const int base = emax[kb];
     auto store_b = [&](const uint4& c, int e, char* st) {
         const int x = e == 255 ? 255 : max(e - base + (CUT || !__is_same(T, _Float16) ? 127 : 140), 0);
-        const float scale = __uint_as_float((unsigned)x << 23);
+        const float scale = __uint_as_float(x == 255 ? 0x7fc00000u : (unsigned)x << 23);  // NaN whatever the codes
         // columns 2i and 2i + 1 go to different fragments: the even ones of 64 columns first, then the odd ones, 64 bytes each.
         // Eight of them come from two words of codes in the order 0 4 1 5 2 6 3 7 (out_pair undoes it); which half of the 16 a
         // lane writes first depends on its block, so that a write's sixteen lanes fall on all 64 banks
@@ -763,7 +763,7 @@ struct DgradPlan {
 DgradPlan dgrad_plan(int dtype, const void* dy, long ld, long M, long N, long cols) {
     DgradPlan p = {(M + 255) / 256, groups_of(cols), 0, dtype == MSFWSI_DT_F32 ? 3 : 1, 0, 1, 0};
     // DMA takes 16-byte chunks of rows, and a tile's rows lie within 2 GB
-    if (dtype == MSFWSI_DT_F32 || N % 8 != 0 || (M > 1 && ld % 8 != 0) || ld > (1L << 21) || (reinterpret_cast<uintptr_t>(dy) & 15)) p.pitch = (N + 7) / 8 * 8;
+    if (dtype == MSFWSI_DT_F32 || N % 8 != 0 || ld % 8 != 0 || ld > (1L << 21) || (reinterpret_cast<uintptr_t>(dy) & 15)) p.pitch = (N + 7) / 8 * 8;
     p.steps = p.parts * (int)((N + 63) / 64);
     p.per_split = p.steps;
     const long tiles = p.mt * p.kt;
@@ -892,7 +892,7 @@ extern "C" int msfwsi_mx4_linear(int dtype, const void* x, long ld, long M, cons
 
 extern "C" int msfwsi_mx4_dgrad_workspace(int dy_dtype, const void* dy, long ld, long M, long N, long cols, long* bytes) {
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dy_dtype) && bytes && M >= 0 && N > 0 && cols > 0);
-    const DgradPlan p = dgrad_plan(dy_dtype, dy, ld, M > 0 ? M : 1, N, cols);
+    const DgradPlan p = dgrad_plan(dy_dtype, dy, M > 1 ? ld : N, M > 0 ? M : 1, N, cols);
     *bytes = round16(p.parts * M * p.pitch * 2) + (p.splits > 1 ? p.splits * M * cols * 4 : 0);
     return MSFWSI_OK;
 }
@@ -902,6 +902,7 @@ extern "C" int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, c
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dy_dtype) && msfwsi_dtype_ok(dx_dtype) && M >= 0 && N > 0 && cols > 0 && (M <= 1 || ld >= N));
     if (M == 0) return MSFWSI_OK;
     MSFWSI_CHECK_ARG(dy && codes && scales && dx && aligned16(codes) && aligned16(scales));
+    if (M == 1) ld = N;  // a single row's pitch means nothing
     const DgradPlan p = dgrad_plan(dy_dtype, dy, ld, M, N, cols);
     MSFWSI_CHECK_ARG((p.pitch == 0 && p.splits == 1) || (workspace && aligned16(workspace)));
     if (N > (1L << 21) || cols > (1L << 21) || p.mt > 0x7fffffffL || p.kt > 0x7fffffffL || p.kt > 0x7fffffffL / p.mt || !grid_ok(p.mt * p.kt, 512)) return MSFWSI_EUNSUPPORTED;

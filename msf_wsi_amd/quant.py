@@ -126,7 +126,8 @@ class MX4Linear(torch.nn.Module):
         return cls(quantize_mx4(linear.weight), b)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        return mx4_linear(x, MX4Tensor(self.codes, self.scales, self.in_features), self.bias)
+        bias = None if self.bias is None else self.bias.float()  # a module cast to 16 bits takes its buffers along
+        return mx4_linear(x, MX4Tensor(self.codes, self.scales, self.in_features), bias)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"

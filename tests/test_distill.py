@@ -174,6 +174,37 @@ def test_top_logits_maps(hip_lib, dt, shape, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,C", [("fp32", 300001), ("bf16", 540003)])
+def test_top_logits_many_segments(hip_lib, dt, C):
+    """more list entries than a merge holds at once"""
+    test_top_logits_rows(hip_lib, dt, 2, C, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+def test_maps_of_many_classes(hip_lib, dt):
+    """maps whose class index takes more than 16 bits, lists of every length class"""
+    for k in (3, 9, 40):
+        test_top_logits_maps(hip_lib, dt, (1, 70001, 3), k)
+        test_loss_maps(hip_lib, dt, (1, 70001, 3), k)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_2_to_the_24(hip_lib):
+    from msf_wsi_amd import losses
+
+    z = torch.zeros(2 ** 24 + 77, 40, dtype=torch.bfloat16, device="cuda")
+    pick = [0, 2 ** 24 - 2, 2 ** 24 - 1, 2 ** 24, 2 ** 24 + 76]
+    z[pick] = logits_of(5, 40, torch.bfloat16, 3).cuda()
+    small = z[pick].clone()
+    big, few = losses.top_logits(z, 2), losses.top_logits(small, 2)
+    assert all(torch.equal(a[pick], b) for a, b in zip(big, few))
+    crit = losses.TopLogitDistillLoss(reduction="none")
+    a, b = crit(z, big), crit(small, few)
+    assert torch.equal(a[pick], b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", list(FP))
 def test_top_logits_repeat_bit_for_bit(hip_lib, dt):
     """also where many candidates compete for places (coarse values: ties everywhere)"""

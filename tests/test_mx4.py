@@ -164,6 +164,60 @@ def test_linear_forward_and_gradient(hip_lib, dt, M, K, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("M,K,N", [(1, 33000, 40), (3, 33100, 20), (100, 4096, 512), (700, 1100, 1300), (1, 300, 70000), (32, 8, 9)])
+def test_linear_long_sums_and_split_ones(hip_lib, dt, M, K, N):
+    test_linear_forward_and_gradient(hip_lib, dt, M, K, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+def test_nan_scale_counts_whatever_the_codes(hip_lib, dt):
+    from msf_wsi_amd import quant
+
+    g = torch.Generator().manual_seed(4)
+    q = quant.quantize_mx4(torch.randn(40, 600, generator=g).cuda())
+    q.scales[1, 7, 2] = 255                                  # columns 320 ... 351 of row 7; the codes stay
+    w = quant.MX4Tensor(q.codes, q.scales, 600)
+    bad = torch.zeros(40, 600, dtype=torch.bool)
+    bad[7, 320:352] = True
+    assert torch.equal(w.dequantize(FP[dt]).isnan().cpu(), bad)
+    for M in (1, 5, 40, 300):
+        x = torch.randn(M, 600, generator=g).to(FP[dt]).cuda().requires_grad_()
+        y = quant.mx4_linear(x, w)
+        assert torch.equal(y.isnan().cpu(), bad.any(1).expand(M, 40))
+        dx, = torch.autograd.grad(y, x, torch.randn(M, 40, generator=g).to(FP[dt]).cuda())
+        assert torch.equal(dx.isnan().cpu(), bad.any(0).expand(M, 600))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(hip_lib):
+    """products that split their sums and share nothing but the weight, in flight on two streams together"""
+    from msf_wsi_amd import quant
+
+    w4 = quant.quantize_mx4(features(512, 4096, torch.float32, 8).cuda() / 30)
+    xs = [features(M, 4096, torch.bfloat16, M).cuda().requires_grad_() for M in (100, 90)]
+    dys = [features(x.shape[0], 512, torch.bfloat16, 3).cuda() for x in xs]
+
+    def both(x, dy):
+        y = quant.mx4_linear(x, w4)
+        return y.detach(), torch.autograd.grad(y, x, dy)[0]
+
+    want = [both(x, dy) for x, dy in zip(xs, dys)]
+    streams = [torch.cuda.Stream() for _ in xs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(both(xs[i], dys[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for pair in got[i] for a, b in zip(pair, want[i]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("out", list(FP))
 def test_linear_of_quantized_input_and_other_output_type(hip_lib, out):
     from msf_wsi_amd import quant
@@ -317,6 +371,11 @@ def test_captured_forward_and_backward(hip_lib, M, K, N):
 
 
 @pytest.mark.gpu
+def test_captured_split_sums(hip_lib):
+    test_captured_forward_and_backward(hip_lib, 100, 4096, 512)
+
+
+@pytest.mark.gpu
 def test_refusals(hip_lib):
     from msf_wsi_amd import _lib, quant
 
@@ -397,3 +456,13 @@ def test_module_and_state(hip_lib):
     other = quant.MX4Linear.from_linear(torch.nn.Linear(200, 70).cuda())
     other.load_state_dict(layer.state_dict())
     assert torch.equal(other(x), want) and not list(layer.parameters())
+
+
+@pytest.mark.gpu
+def test_module_cast_to_16_bits(hip_lib):
+    from msf_wsi_amd import quant
+
+    layer = quant.MX4Linear.from_linear(torch.nn.Linear(70, 30).cuda())
+    x = features(5, 70, torch.bfloat16, 1).cuda()
+    want = quant.mx4_linear(x, quant.MX4Tensor(layer.codes, layer.scales, 70), layer.bias.bfloat16().float())
+    assert torch.equal(layer.bfloat16()(x), want)
