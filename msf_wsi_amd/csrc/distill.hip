@@ -29,9 +29,6 @@ namespace {
 constexpr int kT = 256;
 constexpr int kMaxK = 64;        // = the lanes of a wave: lane i holds entry i of a teacher's list
 constexpr int kMaxParts = 8192;  // workgroups of the forward at most; each leaves one (sum, count) pair
-constexpr int kCand = 512;       // candidates a selection ranks at once
-constexpr int kQueue = 256;      // chunks with candidates it can hold
-static_assert(kCand * sizeof(long) <= kQueue * sizeof(uint4), "the sorted candidates take the queue's place");
 constexpr int kSeg = 65536;      // classes whose list membership is held as bits at a time
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -146,16 +143,24 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int c, int n, con
 // list's surplus once it is in order: the lists fill in any order, no sum depends on it.
 // A queue or list that runs over (long ties, a masked-out segment) sends the segment through k rounds of a plain maximum instead.
 // Rows longer than a segment leave their segments' lists and sums to a merge.
+// DEEP: a list of more than 16 from a row that one wave takes.  The k-th of only 64 maxima would leave most of the row for candidates,
+// so the maxima are those of single chunks (65536 rows of 1000 bf16, k = 64: 186 us; 726 with one maximum a thread).
 // ---------------------------------------------------------------------------------------------------------------------
-template <typename T, int NT, int NCH>
-__global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(const T* __restrict__ x, long ld, int C, int nseg, int k, float inv_t,
+template <typename T, int NT, int NCH, bool DEEP>
+__global__ void __launch_bounds__(NT, NT == 256 ? 7 : DEEP ? 4 : 5) top_segment_kernel(const T* __restrict__ x, long ld, int C, int nseg, int k, float inv_t,
                                                          float* __restrict__ values, int* __restrict__ indices, float* __restrict__ rest,
                                                          long* __restrict__ part_keys, Sum* __restrict__ part_sums) {
     constexpr int VEC = ElemTraits<T>::VEC;
+    constexpr int GROUPS = DEEP ? NT * NCH : NT;                        // maxima that the bound is found among
+    constexpr int kQueue = NT == 256 ? 256 : DEEP ? 128 : 64;           // chunks with candidates
+    constexpr int kCand = NT == 256 || DEEP ? 512 : 128;                // candidates that are ranked at once
+    constexpr int kShared = kQueue * 16 > kCand * 8 ? kQueue * 16 : kCand * 8;
     __shared__ long cand[kCand];
-    __shared__ uint4 queue[kQueue];
+    __shared__ __attribute__((aligned(16))) char shared_[kShared];
     __shared__ int queue_at[kQueue];
-    __shared__ int maxima[NT];
+    __shared__ int maxima[GROUPS];
+    uint4* queue = reinterpret_cast<uint4*>(shared_);
+    long* sorted = reinterpret_cast<long*>(shared_);  // once the queue has been read
     __shared__ Sum buf[NT / 64];
     __shared__ long lbuf[NT / 64];
     __shared__ int count, queued, bound;
@@ -180,14 +185,15 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(cons
         unpack16<T>(raw[j], f);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[e]);
+        if constexpr (DEEP) maxima[j * NT + t] = order_of(top), top = -INFINITY;
     }
-    maxima[t] = order_of(top);
+    if constexpr (!DEEP) maxima[t] = order_of(top);
     if (t == 0) count = queued = 0;
     __syncthreads();
     if (t < 64) {
-        int m[NT / 64];
+        int m[GROUPS / 64];
 #pragma unroll
-        for (int i = 0; i < NT / 64; ++i) m[i] = maxima[i * 64 + t];
+        for (int i = 0; i < GROUPS / 64; ++i) m[i] = maxima[i * 64 + t];
         // the 20 highest bits: 16-bit types whole, fp32 to 2^-11 of its value; a lower bound is all that is needed
         int b = kNothing;
 #pragma unroll 1
@@ -195,7 +201,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(cons
             const int raised = bit == 31 ? 0 : b | (1 << bit);
             int above = 0;
 #pragma unroll
-            for (int i = 0; i < NT / 64; ++i) above += __popcll(__ballot(m[i] >= raised));
+            for (int i = 0; i < GROUPS / 64; ++i) above += __popcll(__ballot(m[i] >= raised));
             if (above >= k) b = raised;
         }
         if (t == 0) bound = b;
@@ -244,7 +250,6 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : 5) top_segment_kernel(cons
     // The list decides when it holds every candidate.  The sum decides unless a NaN went by in it, or it is so small against its
     // reference that terms of it may have been flushed
     if (chunks <= kQueue && got <= kCand && (got >= n || below.s >= 1e-30f)) {
-        long* sorted = reinterpret_cast<long*>(queue);  // which has been read
         for (int i = t; i < got; i += NT) {
             const long key = cand[i];
             int rank = 0;
@@ -899,8 +904,13 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
     }
 }
 
-// rows that one thread takes: maps (their classes are not adjacent), and rows so short that a wave would idle
-bool by_thread(int classes, long inner) { return inner > 1 || classes <= 32; }
+// Rows that one thread takes: maps, whose classes are not adjacent, and short rows where there are very many.  A wave per row costs
+// about 1 ns a row, a thread per row 0.2 us a class however few the rows are (selection: 0.2 us up to k = 4, 0.4 - 0.9 up to 16).
+// bf16, k = 4, selection / loss by a wave and by a thread: 65536 rows of 64 classes 78 / 61 and 18 / 23 us, 65536 of 128 78 / 66 and
+// 29 / 37, 16384 of 64 23 / 21 and 17 / 22, 1024 of 64 7 / 8 and 16 / 21.
+bool by_thread(long rows, int classes, long inner, int k, bool select) {
+    return inner > 1 || (classes <= 128 && k <= 16 && rows >= classes * (select && k > 4 ? 1024L : 256L));
+}
 
 bool layout_ok(long outer, int classes, long inner, long ld) {
     return outer >= 0 && classes > 0 && inner > 0 && (outer <= 1 || ld >= classes * inner) && (inner == 1 || ld == classes * inner) &&
@@ -920,7 +930,7 @@ int segments(int dtype, int classes) {
 extern "C" int msfwsi_top_logits_workspace(int dtype, long outer, int classes, long inner, int k, long* bytes) {
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && bytes && outer >= 0 && classes > 0 && inner > 0 && k > 0 && k <= kMaxK);
     const int nseg = segments(dtype, classes);
-    *bytes = by_thread(classes, inner) || nseg == 1 ? 0 : outer * nseg * (k + 1L) * 8;
+    *bytes = inner > 1 || nseg == 1 ? 0 : outer * nseg * (k + 1L) * 8;
     return MSFWSI_OK;
 }
 
@@ -929,7 +939,7 @@ extern "C" int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, 
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && layout_ok(outer, classes, inner, ld) && k > 0 && k <= kMaxK && k <= classes && inv_t > 0.f);
     if (outer == 0) return MSFWSI_OK;
     MSFWSI_CHECK_ARG(x && values && indices && rest);
-    if (by_thread(classes, inner)) {
+    if (by_thread(outer, classes, inner, k, true)) {
         const long rows = outer * inner, blocks = (rows + kT - 1) / kT;
 #define TOP_THREAD(T, KM, SMALL)                                                                                                  \
     hipLaunchKernelGGL((top_thread_kernel<T, KM, SMALL>), dim3((unsigned)blocks), dim3(kT), 0, ST(stream), (const T*)x, ld, classes, \
@@ -953,11 +963,12 @@ extern "C" int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, 
     MSFWSI_CHECK_ARG(nseg == 1 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0));
     long* keys = (long*)workspace;
     Sum* sums = (Sum*)(keys + outer * nseg * (long)k);
-#define TOP_ROWS(NT, NCH)                                                                                                            \
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((top_segment_kernel<T, NT, NCH>), dim3((unsigned)(outer * nseg)), dim3(NT), 0, ST(stream), \
+#define TOP_ROWS(NT, NCH, DEEP)                                                                                                            \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((top_segment_kernel<T, NT, NCH, DEEP>), dim3((unsigned)(outer * nseg)), dim3(NT), 0, ST(stream), \
                                             (const T*)x, ld, classes, nseg, k, inv_t, values, indices, rest, keys, sums))
-    if (narrow) TOP_ROWS(64, 4);
-    else TOP_ROWS(256, 8);
+    if (narrow && k <= 16) TOP_ROWS(64, 4, false);
+    else if (narrow) TOP_ROWS(64, 4, true);
+    else TOP_ROWS(256, 8, false);
     const int rc = msfwsi_launch_status();
     if (rc != MSFWSI_OK || nseg == 1) return rc;
     if (nseg * k <= kMergeHeld)
@@ -969,9 +980,14 @@ extern "C" int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, 
     return msfwsi_launch_status();
 }
 
-// how many threads take a row of adjacent classes: a wave up to 2048 classes; a large workgroup where rows are too few to fill
-// the machine with small ones
-static int row_threads(long rows, int classes) { return classes <= 2048 ? 64 : rows < 512 && classes >= 16384 ? 1024 : 256; }
+// How many threads take a row of adjacent classes.  One wave (no barriers) for short rows, longer ones too once there are 2048 of them
+// (bf16 forward and backward, one wave / 256 threads: 4096 rows of 1000 20 / 31 us, 4096 of 8192 48 / 55, 1024 of 8192 23 / 21,
+// fp32 4096 of 16384 179 / 172); 1024 threads where so few long rows leave most of the machine idle (256 / 1024
+// threads: 64 rows of 65536 28 / 23 us, 400 rows 41 / 42).
+static int row_threads(long rows, int classes) {
+    if (classes <= 2048 || (rows >= 2048 && classes <= 8192)) return 64;
+    return rows < 256 && classes >= 16384 ? 1024 : 256;
+}
 
 extern "C" int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer, int classes, long inner, int k, const float* values,
                                   const int* indices, const float* rest, const unsigned char* mask, float temperature, int mean, float* stats,
@@ -981,11 +997,13 @@ extern "C" int msfwsi_distill_fwd(int dtype, const void* z, long ld, long outer,
     long blocks = 0;
     if (outer > 0) {
         MSFWSI_CHECK_ARG(z && values && indices && stats && (reinterpret_cast<uintptr_t>(stats) & 15) == 0);
-        const long rows = outer * inner, units = by_thread(classes, inner) ? (rows + kT - 1) / kT : rows;
+        const long rows = outer * inner;
+        const bool thread = by_thread(rows, classes, inner, k, false);
+        const long units = thread ? (rows + kT - 1) / kT : rows;
         const long each = (units + kMaxParts - 1) / kMaxParts;
         blocks = (units + each - 1) / each;
         const float inv_t = 1.f / temperature;
-        if (by_thread(classes, inner)) {
+        if (thread) {
 #define FWD_THREAD(KM)                                                                                                                   \
     MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((distill_thread_fwd_kernel<T, KM>), dim3((unsigned)blocks), dim3(kT), 0, ST(stream),        \
                                             (const T*)z, ld, classes, inner, rows, k, values, indices, rest, mask, temperature, inv_t, \
@@ -1019,7 +1037,7 @@ extern "C" int msfwsi_distill_bwd(int dtype, const void* z, long ld, long outer,
     MSFWSI_CHECK_ARG(z && values && indices && stats && (reinterpret_cast<uintptr_t>(stats) & 15) == 0 && g && dz);
     const long rows = outer * inner;
     const float inv_t = 1.f / temperature;
-    if (by_thread(classes, inner)) {
+    if (by_thread(rows, classes, inner, k, false)) {
 #define BWD_THREAD(KM)                                                                                                                      \
     MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((distill_thread_bwd_kernel<T, KM>), dim3((unsigned)((rows + kT - 1) / kT)), dim3(kT), 0,       \
                                             ST(stream), (const T*)z, ld, classes, inner, rows, k, values, indices, rest, temperature,     \

@@ -729,6 +729,16 @@ __global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
 long groups_of(long cols) { return (cols + kGroup - 1) / kGroup; }
 bool grid_ok(long blocks, int threads = kT) { return blocks > 0 && blocks <= 0xffffffffL / threads; }  // a grid holds fewer than 2^32 threads
 
+// How many parts a sum of `steps` is cut into: at most `most`, and no more than pay for the join, which writes and reads 8 bytes an
+// output and part (about 5 TB/s) while a step of a tile takes step_us.  steps step_us / s + s outputs 8 / 5e6 us is smallest at
+// s^2 = steps step_us 5e6 / 8 / outputs.
+int parts_of(long most, long steps, float step_us, long outputs) {
+    long s = 1;
+    while (s < most && (s + 1.0) * (s + 1.0) * outputs <= steps * step_us * 625e3) ++s;
+    const long per = (steps + s - 1) / s;
+    return (int)((steps + per - 1) / per);
+}
+
 // How the work of y = a b^T is cut.
 struct GemmPlan {
     int tile;        // 0: few rows, straight from memory; else the edge of a square tile
@@ -737,21 +747,24 @@ struct GemmPlan {
 };
 constexpr long kCus = 256;
 constexpr int NWR = 8;  // waves that share 16 columns of few rows
+// Few rows are multiplied straight from memory up to 32 (16) MB of b: below, tiles cannot fill the machine (4096 x 4096 at 16
+// rows 5.1 us, as tiles 9.9); above, DMA reads faster than the waves' own loads (18432 x 18432 at 2 / 16 / 32 rows 33 / 46 / 68 us, as
+// tiles 31 / 32 / 34).
+// Tiles of 256 x 256 take 1.15 times less per output than 128 x 128 (4096 x 4096 x 8192: 74 / 81 us), unless their last round leaves
+// more than that idle (4608 x 4096 x 4096, 1.13 rounds: 70 / 58 us; 6144, 1.5 rounds: 73 / 68).
+// Sums are cut where tiles are fewer than two workgroups per CU could take (512 x 2048 x 18432: 26 us, 52 in one part;
+// 1024 x 2048 x 8192: 24 us in 2 parts, 26 in one, 30 in 4); a part keeps at least 4 steps.
 GemmPlan gemm_plan(long M, long N, long G) {
     GemmPlan p = {0, 1, (N + 15) / 16, 1, (int)G};
-    if (M <= 32) return p;
-    const long big = ((M + 255) / 256) * ((N + 255) / 256);
-    p.tile = big >= kCus ? 256 : 128;
+    if (M <= 32 && N * G * (kGroupBytes + 8) <= (M <= 16 ? 1L << 25 : 1L << 24)) return p;
+    const long big = ((M + 255) / 256) * ((N + 255) / 256), rounds = (big + kCus - 1) / kCus;
+    p.tile = rounds * kCus * 100 <= big * 115 ? 256 : 128;
     p.mt = (M + p.tile - 1) / p.tile;
     p.nt = (N + p.tile - 1) / p.tile;
-    const long tiles = p.mt * p.nt;
-    if (p.tile == 128 && tiles < kCus) {  // two such workgroups run on a CU; a part keeps at least 4 steps
-        long s = (2 * kCus) / tiles;
-        if (s > G / 4) s = G / 4;
-        if (s > 1) {
-            p.per_split = (int)((G + s - 1) / s);
-            p.splits = (int)((G + p.per_split - 1) / p.per_split);
-        }
+    if (p.tile == 128) {
+        const long most = 2 * kCus / (p.mt * p.nt);
+        p.splits = parts_of(most < G / 4 ? most : G / 4, G, 0.7f, M * N);
+        p.per_split = (int)((G + p.splits - 1) / p.splits);
     }
     return p;
 }
@@ -766,15 +779,10 @@ DgradPlan dgrad_plan(int dtype, const void* dy, long ld, long M, long N, long co
     if (dtype == MSFWSI_DT_F32 || N % 8 != 0 || ld % 8 != 0 || ld > (1L << 21) || (reinterpret_cast<uintptr_t>(dy) & 15)) p.pitch = (N + 7) / 8 * 8;
     p.steps = p.parts * (int)((N + 63) / 64);
     p.per_split = p.steps;
-    const long tiles = p.mt * p.kt;
-    if (tiles < kCus) {
-        long s = kCus / tiles;
-        if (s > p.steps / 2) s = p.steps / 2;
-        if (s > 1) {
-            p.per_split = (int)((p.steps + s - 1) / s);
-            p.splits = (p.steps + p.per_split - 1) / p.per_split;
-        }
-    }
+    // 512 x 1000 x 512: 20 us, 33 in one part; 256 x 512 x 18432: 22 us in one part, 34 in three
+    const long most = kCus / (p.mt * p.kt);
+    p.splits = parts_of(most < p.steps / 2 ? most : p.steps / 2, p.steps, 1.6f, M * cols);
+    p.per_split = (p.steps + p.splits - 1) / p.splits;
     return p;
 }
 long round16(long bytes) { return (bytes + 15) / 16 * 16; }
@@ -855,10 +863,16 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
     return msfwsi_launch_status();
 }
 
-// workspace of a linear call: x's codes, its scales, the partial sums; a single row needs none
+// A single row is quantised by the waves that multiply it, in one launch and without a workspace, unless the weight is so large that
+// its time exceeds that of a launch more (18432 x 18432: 40 us, in two launches 34; 512 x 18432: 8 us, 11 + 3 in two)
+static bool row_alone(long M, long N, long cols) {
+    const long G = groups_of(cols);
+    return M == 1 && G <= kRowGroups && N * G * (kGroupBytes + 8) <= 1L << 26;
+}
+// workspace of a linear call: x's codes, its scales, the partial sums
 extern "C" int msfwsi_mx4_linear_workspace(long M, long N, long cols, long* bytes) {
     const int rc = msfwsi_mx4_gemm_workspace(M, N, cols, bytes);
-    if (rc == MSFWSI_OK) *bytes = M == 1 && groups_of(cols) <= kRowGroups ? 0 : *bytes + groups_of(cols) * M * kGroupBytes + round16(groups_of(cols) * M * 8);
+    if (rc == MSFWSI_OK) *bytes = row_alone(M, N, cols) ? 0 : *bytes + groups_of(cols) * M * kGroupBytes + round16(groups_of(cols) * M * 8);
     return rc;
 }
 
@@ -874,7 +888,7 @@ extern "C" int msfwsi_mx4_linear(int dtype, const void* x, long ld, long M, cons
     MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && msfwsi_dtype_ok(y_dtype) && M >= 0 && N > 0 && cols > 0);
     if (M == 0) return MSFWSI_OK;
     MSFWSI_CHECK_ARG(codes && scales && y);
-    if (M == 1 && groups_of(cols) <= kRowGroups) {
+    if (row_alone(M, N, cols)) {
         MSFWSI_CHECK_ARG(x && aligned16(codes) && aligned16(scales));
         if (N > (1L << 21)) return MSFWSI_EUNSUPPORTED;
         if (dtype == MSFWSI_DT_BF16) launch_row<__bf16>(y_dtype, x, codes, scales, N, cols, bias, y, stream);

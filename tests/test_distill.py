@@ -190,18 +190,44 @@ def test_maps_of_many_classes(hip_lib, dt):
 
 
 @pytest.mark.gpu
-def test_more_rows_than_2_to_the_24(hip_lib):
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("rows,C,k", [(300, 1, 1), (4100, 16, 4), (9000, 33, 7), (16500, 16, 16), (33000, 128, 3), (5000, 300, 40), (70, 2000, 64)])
+def test_many_short_rows(hip_lib, dt, rows, C, k):
+    """rows that a thread takes each, and long lists from rows that a wave takes; some of the rows are checked"""
     from msf_wsi_amd import losses
 
-    z = torch.zeros(2 ** 24 + 77, 40, dtype=torch.bfloat16, device="cuda")
+    T = 2.0
+    z, t = logits_of(rows, C, FP[dt], rows + C), logits_of(rows, C, FP[dt], rows * C + k)
+    teacher = losses.top_logits(t.cuda(), k, T)
+    pick = sorted({0, 1, 63, 64, 255, 256, rows // 2, rows - 2, rows - 1} & set(range(rows)))
+    some = losses.TopLogits(*(a[pick] for a in teacher))
+    same_top(t[pick], k, T, some)
+    zc = z.cuda().requires_grad_()
+    row = losses.TopLogitDistillLoss(T, "none")(zc, teacher)
+    grad, = torch.autograd.grad(row, zc, torch.ones(rows, device="cuda"))
+    check(z[pick], some.values, some.indices, some.rest, None, T, row.detach()[pick], grad[pick], FP[dt])
+    mean = losses.TopLogitDistillLoss(T)(zc, teacher)
+    want = float(row.detach().double().mean())
+    assert abs(mean.item() - want) <= 4 * U * abs(want) + 1e-30
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [40, 129])
+def test_more_rows_than_2_to_the_24(hip_lib, C):
+    from msf_wsi_amd import losses
+
+    z = torch.zeros(2 ** 24 + 77, C, dtype=torch.bfloat16, device="cuda")
     pick = [0, 2 ** 24 - 2, 2 ** 24 - 1, 2 ** 24, 2 ** 24 + 76]
-    z[pick] = logits_of(5, 40, torch.bfloat16, 3).cuda()
-    small = z[pick].clone()
-    big, few = losses.top_logits(z, 2), losses.top_logits(small, 2)
-    assert all(torch.equal(a[pick], b) for a, b in zip(big, few))
-    crit = losses.TopLogitDistillLoss(reduction="none")
-    a, b = crit(z, big), crit(small, few)
-    assert torch.equal(a[pick], b)
+    small = logits_of(5, C, torch.bfloat16, 3)
+    z[pick] = small.cuda()
+    teacher = losses.top_logits(z, 2)
+    some = losses.TopLogits(*(a[pick] for a in teacher))
+    same_top(small, 2, 1.0, some)
+    z[pick] = z[pick].flip(1)
+    z.requires_grad_()
+    row = losses.TopLogitDistillLoss(reduction="none")(z, teacher)
+    grad, = torch.autograd.grad(row, z, torch.ones_like(row))
+    check(small.flip(1), some.values, some.indices, some.rest, None, 1.0, row.detach()[pick], grad[pick], torch.bfloat16)
 
 
 @pytest.mark.gpu

@@ -165,7 +165,8 @@ def test_linear_forward_and_gradient(hip_lib, dt, M, K, N):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", list(FP))
-@pytest.mark.parametrize("M,K,N", [(1, 33000, 40), (3, 33100, 20), (100, 4096, 512), (700, 1100, 1300), (1, 300, 70000), (32, 8, 9)])
+@pytest.mark.parametrize("M,K,N", [(1, 33000, 40), (3, 33100, 20), (100, 4096, 512), (700, 1100, 1300), (1, 300, 70000), (32, 8, 9),
+                                   (7, 18432, 3000), (25, 9300, 3100), (1, 9300, 14400)])
 def test_linear_long_sums_and_split_ones(hip_lib, dt, M, K, N):
     test_linear_forward_and_gradient(hip_lib, dt, M, K, N)
 
