@@ -141,6 +141,7 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int c, int n, con
 // chunk at nearly every step: looking at them in place cost all lanes the walk twice over, 166 us instead of 149); what is
 // not below the bound goes into a list and is ranked by counting.  Everything else is summed for `rest`, each thread its own and the
 // list's surplus once it is in order: the lists fill in any order, no sum depends on it.
+// 4096 rows of 65536 bf16, k = 32: 134 us, 4.0 TB/s; 4 such rows of fp32 9 us.
 // A queue or list that runs over (long ties, a masked-out segment) sends the segment through k rounds of a plain maximum instead.
 // Rows longer than a segment leave their segments' lists and sums to a merge.
 // DEEP: a list of more than 16 from a row that one wave takes.  The k-th of only 64 maxima would leave most of the row for candidates,
@@ -537,7 +538,8 @@ __global__ void __launch_bounds__(kFinish) distill_finish_kernel(const double* _
 
 // Rows of adjacent classes, a workgroup per row (64 threads for short rows: one wave, no barriers between waves).  Lane i of
 // every wave holds entry i of the teacher's list; the classes it lists are a bit set in LDS, one byte (fp32: half a byte) per
-// 16-byte chunk.  One walk over the row sums the unlisted classes; the listed ones are gathered.
+// 16-byte chunk.  One walk over the row sums the unlisted classes; the listed ones are gathered.  Bound by reading the row and, near
+// that, by an exponential per class: 4096 rows of 65536 bf16 136 us, 3.9 TB/s.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z, long ld, int C, long rows, int k,
                                                          const float* __restrict__ values, const int* __restrict__ indices,
@@ -655,7 +657,8 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
     if (t == 0) parts[2 * blockIdx.x] = lsum, parts[2 * blockIdx.x + 1] = lcount;
 }
 
-// The unlisted form goes over the whole row; behind a barrier the lanes that hold the list put the listed classes right.
+// The unlisted form goes over the whole row; behind a barrier the lanes that hold the list put the listed classes right.  Bound by
+// memory: 4096 rows of 65536 bf16 204 us, 5.3 TB/s read and written.
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z, long ld, int C, long rows, int k,
                                                          const float* __restrict__ values, const int* __restrict__ indices,
@@ -717,7 +720,9 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
     if (idx >= 0 && idx < C) store_elem<T>(d, idx, gs * (exp2_((load_elem<T>(p, idx) - st.x) * c - st.y) - share));
 }
 
-// One thread per row: maps, and rows of a few classes.  KM > 0: lists of up to KM entries whose indices stay in registers;
+// One thread per row: maps, and rows of a few classes.  A class costs about 7 instructions: the listed ones are taken out of the
+// sum by a bit each, their own logits are asked for early and handled apart.  32 maps of 21 x 256 x 256 fp32, k = 4: forward 99 us
+// (2.9 TB/s; bound by instructions and latency at 4 waves per SIMD), backward 106 us (4.4 TB/s).  KM > 0: lists of up to KM entries whose indices stay in registers;
 // KM = 0: any length, read again where needed.
 template <int KM>
 struct List {
@@ -741,12 +746,32 @@ struct List {
         else return ip[s * inner];
     }
     __device__ __forceinline__ float value(int s) const { return index(s) >= 0 ? vp[s * inner] : -INFINITY; }
+    // the class of entry s is none that an entry before it lists
+    __device__ __forceinline__ bool first(int s) const {
+        bool yes = true;
+        for (int q = 0; q < s; ++q) yes &= index(q) != index(s);
+        return yes;
+    }
 };
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+// f, or -inf where bit e of w is set
+__device__ __forceinline__ float unless(unsigned w, int e, float f) {
+    const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)w, e, 1);
+    return __uint_as_float((m & 0xff800000u) | (~m & __float_as_uint(f)));
+}
+// classes c0 ... in groups of 8: a branch for each class would cost more registers than the classes; past the last class it again
 template <typename T, int U>
 __device__ __forceinline__ void load_classes(const T* __restrict__ p, int c0, int C, long inner, float* f) {
 #pragma unroll
-    for (int e = 0; e < U; ++e)
-        if (c0 + e < C) f[e] = load_elem<T>(p, (c0 + e) * inner);
+    for (int e0 = 0; e0 < U; e0 += 8)
+        if (c0 + e0 < C) {
+#pragma unroll
+            for (int e = e0; e < e0 + 8; ++e) f[e] = load_elem<T>(p, min(c0 + e, C - 1) * inner);
+        }
 }
 #define LIST_FOR(S) _Pragma("clang loop unroll_count(KM > 0 ? KM : 1)") for (int S = 0; S < (KM > 0 ? KM : list.k); ++S) if (KM == 0 || S < list.k)
 
@@ -779,35 +804,45 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
             if (row_loss != nullptr) row_loss[row] = 0.f;
             continue;
         }
+        float zl[KM > 0 ? KM : 1];  // the listed classes' logits: asked for early
+        if constexpr (KM > 0) {
+#pragma unroll
+            for (int s = 0; s < KM; ++s) zl[s] = list.idx[s] >= 0 && list.idx[s] < C ? load_elem<T>(p, list.idx[s] * inner) : -INFINITY;
+        }
         Sum un = {-INFINITY, 0.f}, in = {-INFINITY, 0.f};
         for (int c0 = 0; c0 < C; c0 += U) {
             if (c0 > 0) load_classes<T, U>(p, c0, C, inner, f);
-            unsigned w = 0;
+            unsigned w = C - c0 < U ? ~0u << (C - c0) : 0u;  // what drops out of the sum: the listed classes, and those past the last
             LIST_FOR(s) {
                 const unsigned at = (unsigned)(list.index(s) - c0);
                 w |= at < U ? 1u << at : 0u;
             }
-            float mu = un.m, mi = in.m;
+            float mu = un.m;
 #pragma unroll
-            for (int e = 0; e < U; ++e)
-                if (c0 + e < C) {
-                    const bool listed = (w >> e) & 1u;
-                    mu = fmaxf(mu, listed ? -INFINITY : f[e]);
-                    mi = fmaxf(mi, listed ? f[e] : -INFINITY);
+            for (int e0 = 0; e0 < U; e0 += 8)
+                if (c0 + e0 < C) {
+#pragma unroll
+                    for (int e = e0; e < e0 + 8; e += 2) {
+                        f[e] = unless(w, e, f[e]);
+                        f[e + 1] = unless(w, e + 1, f[e + 1]);
+                        mu = max3(mu, f[e], f[e + 1]);
+                    }
                 }
-            asm volatile("" : "+v"(w));  // its bits are tested again, not kept as 2 U scalar registers
-            const float ru = finite_ref(mu), ri = finite_ref(mi);
-            float su = un.s * exp2_((un.m - ru) * c), si = in.s * exp2_((in.m - ri) * c);
+            const float ru = finite_ref(mu);
+            float su = un.s * exp2_((un.m - ru) * c);
 #pragma unroll
-            for (int e = 0; e < U; ++e)
-                if (c0 + e < C) {
-                    const bool listed = (w >> e) & 1u;
-                    const float x = exp2_((f[e] - (listed ? ri : ru)) * c);
-                    su += listed ? 0.f : x;
-                    si += listed ? x : 0.f;
+            for (int e0 = 0; e0 < U; e0 += 8)
+                if (c0 + e0 < C) {
+#pragma unroll
+                    for (int e = e0; e < e0 + 8; ++e) su += exp2_((f[e] - ru) * c);
                 }
             un = {mu, su};
-            in = {mi, si};
+        }
+        LIST_FOR(s) {
+            float zi;
+            if constexpr (KM > 0) zi = zl[s];
+            else zi = list.index(s) >= 0 && list.index(s) < C ? load_elem<T>(p, list.index(s) * inner) : -INFINITY;
+            if (list.first(s)) in = join(in, one(zi), c);
         }
         float4 st = row_stats(un, join(un, in, c));
         if (bad) st.x = st.z = NAN;
@@ -820,7 +855,10 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
         LIST_FOR(s) {
             const float lp = (list.value(s) - vtop) * c - L, pi = exp2_(lp);
             const int at = list.index(s);
-            if (pi != 0.f && at >= 0 && at < C) loss += pi * (lp - ((load_elem<T>(p, at * inner) - st.x) * c - st.y));
+            float zi;
+            if constexpr (KM > 0) zi = zl[s];
+            else zi = at >= 0 && at < C ? load_elem<T>(p, at * inner) : 0.f;
+            if (pi != 0.f && at >= 0 && at < C) loss += pi * (lp - ((zi - st.x) * c - st.y));
         }
         loss = bad ? NAN : temp * temp * kLn2 * loss;
         stats[row] = st;
@@ -847,12 +885,15 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
     float f[U];
     load_classes<T, U>(p, 0, C, inner, f);  // asked for first: the list and what follows from it come in their shadow
     const float4 st = stats[row];
-    if (!row_counts(st)) {
-        for (int j = 0; j < C; ++j) store_elem<T>(d, j * inner, 0.f);
-        return;
-    }
+    // a row that does not count writes its zeros with its neighbours: lines written in two halves cost twice
+    const bool counts = row_counts(st);
     List<KM> list;
     list.open(values, indices, o, i, inner, k);
+    float zl[KM > 0 ? KM : 1];
+    if constexpr (KM > 0) {
+#pragma unroll
+        for (int s = 0; s < KM; ++s) zl[s] = list.idx[s] >= 0 && list.idx[s] < C ? load_elem<T>(p, list.idx[s] * inner) : 0.f;
+    }
     const float r = rest != nullptr ? rest[row] * temp : -INFINITY;
     float vtop = r;
     LIST_FOR(s) {
@@ -863,37 +904,34 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
     float total = exp2_(lr);
     LIST_FOR(s) total += exp2_((list.value(s) - vtop) * c);
     const float L = log2_(total);
-    float pi[KM > 0 ? KM : 1];
-    if constexpr (KM > 0) {
-#pragma unroll
-        for (int s = 0; s < KM; ++s) pi[s] = s < k ? exp2_((list.value(s) - vtop) * c - L) : 0.f;
-    }
     const float gs = g[g_rows ? row : 0] * (factor != nullptr ? *factor : 1.f) * temp;
     const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - exp2_(lr - L));
-    for (int c0 = 0; c0 < C; c0 += U) {
-        unsigned w = 0;
-        if (c0 > 0) load_classes<T, U>(p, c0, C, inner, f);
-        if constexpr (KM > 0) {
-            LIST_FOR(s) {
-                const unsigned at = (unsigned)(list.index(s) - c0);
-                w |= at < U ? 1u << at : 0u;
-            }
+    float listed[KM > 0 ? KM : 1];  // the listed classes' gradients
+    if constexpr (KM > 0) {
+        float pi[KM];
+#pragma unroll
+        for (int s = 0; s < KM; ++s) pi[s] = s < k ? exp2_((list.value(s) - vtop) * c - L) : 0.f;
+#pragma unroll
+        for (int s = 0; s < KM; ++s) {
+            float share = 0.f;
+#pragma unroll
+            for (int q = 0; q < KM; ++q) share += list.idx[q] == list.idx[s] ? pi[q] : 0.f;
+            listed[s] = gs * (exp2_((zl[s] - st.x) * c - st.y) - share);
         }
+    }
+    for (int c0 = 0; c0 < C; c0 += U) {
+        if (c0 > 0) load_classes<T, U>(p, c0, C, inner, f);
 #pragma unroll
         for (int e = 0; e < U; ++e)
             if (c0 + e < C) {
+                float v = outside * exp2_((f[e] - st.z) * c - st.w);
                 if constexpr (KM > 0) {
-                    const bool listed = (w >> e) & 1u;
-                    float share = 0.f;
-                    LIST_FOR(s) share += list.index(s) == c0 + e ? pi[s] : 0.f;
-                    const float x = exp2_((f[e] - (listed ? st.x : st.z)) * c - (listed ? st.y : st.w));
-                    store_elem<T>(d, (c0 + e) * inner, listed ? gs * (x - share) : outside * x);
-                } else {
-                    store_elem<T>(d, (c0 + e) * inner, outside * exp2_((f[e] - st.z) * c - st.w));
+                    LIST_FOR(s) v = list.idx[s] == c0 + e ? listed[s] : v;
                 }
+                store_elem<T>(d, (c0 + e) * inner, counts ? v : 0.f);
             }
     }
-    if constexpr (KM == 0) {
+    if (KM == 0 && counts) {
         for (int s = 0; s < k; ++s) {  // the same thread: these stores come after the ones above
             const int at = list.index(s);
             if (at < 0 || at >= C) continue;

@@ -80,7 +80,7 @@ __device__ __forceinline__ unsigned quantize8(const float* f, unsigned& E) {
 }
 
 // One half-wave (32 lanes x 8 elements) per group of a row, UG groups one after the other with their loads in flight together.
-// Bound by memory.
+// Bound by memory: 18432 x 18432 fp32 quantised in 346 us (4.5 TB/s read and written), widened to fp32 in 309 us (5.0 TB/s).
 constexpr int UG = 4;
 template <typename T>
 __global__ void __launch_bounds__(kT) mx4_quantize_kernel(const T* __restrict__ x, long ld, long rows, long cols, int G,
@@ -175,7 +175,7 @@ __device__ __forceinline__ void mx4_step(f32x16& acc, const int4& a, int sa, con
 // Few rows (up to 16 FA): 16 columns per workgroup straight from memory, the groups dealt over its NW waves and joined in LDS.
 // Bound by reading b once; nothing is shared between workgroups, so nothing is staged, and the next group's loads are on their
 // way while one is multiplied.  16 columns, because a CU's share is a whole number of workgroups: 576 of 32 columns on 256 CUs
-// (18432 rows of b) took 51 us, 1152 of 16 take 40.
+// (18432 rows of b) took 51 us, 1152 of 16 took 40.
 // A 16x16x128 step takes 32 elements from each lane; quarter q of the wave takes blocks 2q, 2q + 1 of a group in its two steps.
 // ROW: a single row of up to kRowGroups groups, which comes as it is (TX) and is quantised by every workgroup for itself, so that one
 // launch does it all; the codes wait in LDS.  (One group after the other, with its loads waited for, this took 13 us.)
@@ -342,7 +342,8 @@ struct GemmArgs {
 // stages in LDS filled by DMA.  A row's eight 16-byte chunks lie at (chunk ^ (row / 2 & 7)): the sixteen rows that a read takes
 // at a time then fall on all 64 banks.  The columns of a wave's 64 are dealt to its two fragments in turn (2 l + j: b's rows lie in
 // LDS in that order), so that a lane ends up with neighbours of a row and a wave writes whole 128-byte lines.
-// 8192 x 9216 x 9216: 392 us, 3.5 PFLOP/s (4.3 without the requests; registers alone reach 6.5 at this card's power).  Requests and
+// 8192 x 9216 x 9216: 382 us, 3.6 PFLOP/s (4.5 rounds of tiles); 8192 x 8192 x 8192: 268 us, 4.1 PFLOP/s (registers alone reach 6.5
+// at this card's power).  Requests and
 // products share the CU's LDS and issue slots; a four-stage ring of half groups (64-byte lines: 0.8 of the rate), fragments
 // read a step ahead by hand, a workgroup that runs through its tiles, and four waves of 128 x 128 were all 2 - 20 % slower.
 template <typename T, int TM, int TN, int WM, int WN>
@@ -489,10 +490,12 @@ __global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy,
 
 // dx = dy W for a frozen W: 256 rows x 256 columns (one group of W's) per workgroup of 8 waves, 64 rows of W a step.  dy comes
 // by DMA like the tiles above; W's codes (8 KB a step) are widened to 16 bits on the way into LDS [n][column] and read transposed
-// (ds_read_b64_tr_b16), even and odd columns apart as above.  The scale of a weight varies along the sum, so it is applied while widening -- relative to the
-// largest scale of its 32 columns over this workgroup's rows of W, which the outputs are multiplied with in the end:
+// (ds_read_b64_tr_b16), even and odd columns apart as above.  The scale of a weight varies along the sum, so it is applied while
+// widening -- relative to the largest scale of its 32 columns over this workgroup's rows of W, which the outputs are multiplied with in the end:
 // no weight can overflow, and bf16 keeps weights down to 2^-126 of the largest.  fp16 holds scales that are at most 2^26 apart
 // exactly; where a workgroup finds them further apart it cuts each dy value into two bf16 parts (8 + 3 bits) instead.
+// Bound by the 16-bit matrix rate and the widening beside it: 8192 x 8192 x 8192 bf16 991 us, 1.1 PFLOP/s (the library's product of 16-bit
+// matrices 1.38); 8192 x 9216 x 9216 fp16 1516 us.
 template <typename T, bool CUT>
 __device__ __forceinline__ void dgrad_mma(f32x16& acc, const uint4& a, const uint4& b) {
     if constexpr (!CUT) {
