@@ -753,8 +753,9 @@ constexpr int NWR = 8;  // waves that share 16 columns of few rows
 // Few rows are multiplied straight from memory up to 32 (16) MB of b: below, tiles cannot fill the machine (4096 x 4096 at 16
 // rows 5.1 us, as tiles 9.9); above, DMA reads faster than the waves' own loads (18432 x 18432 at 2 / 16 / 32 rows 33 / 46 / 68 us, as
 // tiles 31 / 32 / 34).
-// Tiles of 256 x 256 take 1.15 times less per output than 128 x 128 (4096 x 4096 x 8192: 74 / 81 us), unless their last round leaves
-// more than that idle (4608 x 4096 x 4096, 1.13 rounds: 70 / 58 us; 6144, 1.5 rounds: 73 / 68).
+// Tiles of 256 x 256 take a tenth less time than 128 x 128 (4096 x 4096 x 8192: 74 / 81 us, 4096 x 8192 x 8192: 146 / 162) where their
+// rounds of 256 are at most 15 % more than their number (8192 x 9216 x 9216, 4.5 rounds: 378 / 401 us), and are slower where the last
+// round leaves more idle (4608 x 4096 x 4096, 1.13 rounds: 70 / 58 us; 6144, 1.5 rounds: 73 / 68; 8192 x 5120, 2.5: 112 / 110).
 // Sums are cut where tiles are fewer than two workgroups per CU could take (512 x 2048 x 18432: 26 us, 52 in one part;
 // 1024 x 2048 x 8192: 24 us in 2 parts, 26 in one, 30 in 4); a part keeps at least 4 steps.
 GemmPlan gemm_plan(long M, long N, long G) {
