@@ -4,7 +4,7 @@
 // [N, C, H * W]); a "row" is one (outer, inner) position.
 //
 // Selection: the k largest logits of a row in descending order, equal ones by ascending index, NaN above every number; and
-//   rest = log sum over the OTHERS of exp(logit / T)          (-inf when nothing is left)
+//   rest = log sum over the OTHERS of exp(logit / T)          (-inf when nothing is left, +inf when one of them is +inf)
 // so that values and rest together hold the teacher's whole distribution up to the split of the rest.
 //
 // Loss of a row with teacher entries (v_i, idx_i) and rest; z the student's logits, a_j = z_j / T:
@@ -54,14 +54,17 @@ constexpr long kNoKey = (long)0x8000000000000000L;
 
 // sum of 2^((x - m) c) over some logits x: c = log2(e) / T, m the largest of them.  Nothing: m = -inf, s = 0; a NaN among them
 // makes s NaN.  The difference is taken before the product, so logits far from zero keep their precision and a row of the
-// type's lowest value does not overflow.  (c x - c m in one fma was no faster.)
+// type's lowest value does not overflow.  (c x - c m in one fma was no faster.)  A logit of +inf is a term of 1 relative to
+// itself: the logarithm of the sum is +inf.
 struct Sum {
     float m, s;
 };
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
+// 2^((x - ref) c); 1 for an infinite ref itself
+__device__ __forceinline__ float term(float x, float ref, float c) { return x == ref ? 1.f : exp2_((x - ref) * c); }
 __device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
     const float m = fmaxf(a.m, b.m), ref = finite_ref(m);
-    return {m, a.s * exp2_((a.m - ref) * c) + b.s * exp2_((b.m - ref) * c)};
+    return {m, a.s * term(a.m, ref, c) + b.s * term(b.m, ref, c)};
 }
 __device__ __forceinline__ Sum one(float x) { return {x, x == -INFINITY ? 0.f : 1.f}; }
 __device__ __forceinline__ float log_of(Sum v, float inv_t) { return v.s == 0.f ? -INFINITY : v.m * inv_t + log2_(v.s) * kLn2; }
@@ -475,7 +478,7 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
             out = value_of(a);
         }
         if (out != -INFINITY) {
-            const float d = out - sum.m, e = exp2_(-fabsf(d) * c);
+            const float d = out - sum.m, e = out == sum.m ? 1.f : exp2_(-fabsf(d) * c);
             sum.s = d > 0.f ? fmaf(sum.s, e, 1.f) : sum.s + e;
             sum.m = fmaxf(sum.m, out);
         }
@@ -842,7 +845,7 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
             float zi;
             if constexpr (KM > 0) zi = zl[s];
             else zi = list.index(s) >= 0 && list.index(s) < C ? load_elem<T>(p, list.index(s) * inner) : -INFINITY;
-            if (list.first(s)) in = join(in, one(zi), c);
+            if (list.first(s)) in = join(in, {zi, zi == -INFINITY ? 0.f : 1.f + (zi - zi)}, c);  // +inf has no softmax: NaN
         }
         float4 st = row_stats(un, join(un, in, c));
         if (bad) st.x = st.z = NAN;

@@ -559,3 +559,49 @@ def test_frozen_teacher_chain(hip_lib):
     want = grad @ w / 24
     lim = (2 * dy + 2 * error_of(y, 2.0)) * 2.0 * 3 * float(w.abs().max()) / 24 + 1508 * 3 * 2.0 ** -23 * float((grad.abs() @ w.abs()).max()) / 24
     assert float((x.grad.cpu().double() - want).abs().max()) <= lim
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("rows,C,k", [(10300, 40, 2), (6, 40, 2), (6, 900, 33), (6, 2000, 5), (6, 20011, 3), (6, 300001, 64)])
+def test_infinite_logits_left_over(hip_lib, dt, rows, C, k):
+    """+inf outside the list makes rest +inf, one or several of them, together or apart; a NaN outside makes it NaN"""
+    from msf_wsi_amd import losses
+
+    g = torch.Generator().manual_seed(C)
+    x = logits_of(rows, C, FP[dt], C)
+    at = [torch.randperm(C, generator=g) for _ in range(6)]
+    x[0, at[0][:k + 1]] = math.inf                          # one left over
+    x[1, at[1][:k + 3]] = math.inf
+    x[2, 1:k + 3] = math.inf                                # next to each other
+    x[3, at[3][:k + 1]], x[3, at[3][k + 1]] = math.inf, math.nan                 # the NaN is listed
+    x[4, at[4][:k + 2]], x[4, at[4][k + 2:k + 5]] = math.nan, math.inf           # NaN and +inf left over
+    x[5, at[5][:k]] = math.inf                              # all of them listed
+    if C > 1000:
+        x[5, at[5][k:]] = -math.inf                         # and nothing else in the row
+    got = losses.top_logits(x.cuda(), k, 2.0)
+    some = losses.TopLogits(*(a[:6] for a in got))
+    same_top(x[:6], k, 2.0, some)
+    assert some.rest.isposinf().tolist() == [True] * 4 + [False] * 2 and some.rest.isnan().tolist() == [False] * 4 + [True, False]
+    if rows == 6:                                           # the same as maps of three positions
+        maps = losses.top_logits(x.view(2, 3, C).movedim(-1, 1).contiguous().cuda(), k, 2.0, dim=1)
+        assert torch.equal(maps.indices.movedim(1, -1).reshape(6, k), some.indices)
+        assert torch.equal(maps.rest.reshape(6).isposinf(), some.rest.isposinf()) and torch.equal(maps.rest.reshape(6).isnan(), some.rest.isnan())
+
+
+@pytest.mark.gpu
+def test_infinite_student_logits(hip_lib):
+    """a logit of +inf has no softmax: its row's loss is NaN, whichever way the row is taken; other rows keep theirs"""
+    from msf_wsi_amd import losses
+
+    z = logits_of(4, 300, torch.float32, 1)
+    v, i, r = to.top_logits(logits_of(4, 300, torch.float32, 2), 4, 1.0)
+    z[1, int(i[1, 2])], z[2, (set(range(300)) - set(i[2].tolist())).pop()] = math.inf, math.inf
+    for dim in (-1, 1):
+        zl, vl, il = (a.t()[None].contiguous().cuda() if dim == 1 else a.cuda() for a in (z, v.float(), i.int()))
+        zl.requires_grad_()
+        row = losses.TopLogitDistillLoss(1.0, "none", dim=dim)(zl, losses.TopLogits(vl, il, r.float().cuda().view((1, 4) if dim == 1 else (4,))))
+        grad, = torch.autograd.grad(row, zl, torch.ones_like(row))
+        grad = grad[0].t() if dim == 1 else grad
+        assert row.reshape(-1).isnan().tolist() == [False, True, True, False]
+        assert grad.isnan().all(1).tolist() == [False, True, True, False] and bool(torch.isfinite(grad[[0, 3]]).all())
