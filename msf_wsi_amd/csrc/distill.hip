@@ -54,34 +54,38 @@ constexpr long kNoKey = (long)0x8000000000000000L;
 
 // sum of 2^((x - m) c) over some logits x: c = log2(e) / T, m the largest of them.  Nothing: m = -inf, s = 0; a NaN among them
 // makes s NaN.  The difference is taken before the product, so logits far from zero keep their precision and a row of the
-// type's lowest value does not overflow.  (c x - c m in one fma was no faster.)  A logit of +inf is a term of 1 relative to
-// itself: the logarithm of the sum is +inf.
+// type's lowest value does not overflow.  (c x - c m in one fma was no faster.)  With INF a logit of +inf is a term of 1 relative
+// to itself and the logarithm of the sum +inf; without, a NaN (the loss has no softmax there, and its kernels no registers to spare).
 struct Sum {
     float m, s;
 };
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.f : m; }
-// 2^((x - ref) c); 1 for an infinite ref itself
-__device__ __forceinline__ float term(float x, float ref, float c) { return x == ref ? 1.f : exp2_((x - ref) * c); }
+template <bool INF>
+__device__ __forceinline__ float term(float x, float ref, float c) {
+    return INF && x == ref ? 1.f : exp2_((x - ref) * c);
+}
+template <bool INF>
 __device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
     const float m = fmaxf(a.m, b.m), ref = finite_ref(m);
-    return {m, a.s * term(a.m, ref, c) + b.s * term(b.m, ref, c)};
+    return {m, a.s * term<INF>(a.m, ref, c) + b.s * term<INF>(b.m, ref, c)};
 }
 __device__ __forceinline__ Sum one(float x) { return {x, x == -INFINITY ? 0.f : 1.f}; }
 __device__ __forceinline__ float log_of(Sum v, float inv_t) { return v.s == 0.f ? -INFINITY : v.m * inv_t + log2_(v.s) * kLn2; }
+template <bool INF>
 __device__ __forceinline__ Sum wave_join(Sum v, float c) {
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = join(v, {__shfl_xor(v.m, off, 64), __shfl_xor(v.s, off, 64)}, c);
+    for (int off = 32; off > 0; off >>= 1) v = join<INF>(v, {__shfl_xor(v.m, off, 64), __shfl_xor(v.s, off, 64)}, c);
     return v;
 }
 // over the workgroup; every thread has the result
-template <int NT>
+template <int NT, bool INF>
 __device__ __forceinline__ Sum block_join(Sum v, Sum* buf, float c) {
-    v = wave_join(v, c);
+    v = wave_join<INF>(v, c);
     if constexpr (NT > 64) {
         if ((threadIdx.x & 63) == 0) buf[threadIdx.x >> 6] = v;
         __syncthreads();
         v = buf[0];
-        for (int i = 1; i < NT / 64; ++i) v = join(v, buf[i], c);
+        for (int i = 1; i < NT / 64; ++i) v = join<INF>(v, buf[i], c);
         __syncthreads();
     }
     return v;
@@ -247,7 +251,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : DEEP ? 4 : 5) top_segment_
                 if (slot < kCand) cand[slot] = key_of(v, c0 + at);
             }
         }
-    const Sum below = block_join<NT>({s == 0.f ? -INFINITY : finite_ref(lim), s}, buf, c);
+    const Sum below = block_join<NT, true>({s == 0.f ? -INFINITY : finite_ref(lim), s}, buf, c);
     __syncthreads();
     const int got = count;
     Sum left = {-INFINITY, 0.f};
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : DEEP ? 4 : 5) top_segment_
         for (int i = t; i < got; i += NT) {
             const long key = sorted[i];
             if (i >= want) {
-                left = join(left, one(value_of((int)(key >> 32))), c);
+                left = join<true>(left, one(value_of((int)(key >> 32))), c);
             } else if (nseg == 1) {
                 values[row * k + i] = value_of((int)(key >> 32));
                 indices[row * k + i] = index_of(key);
@@ -272,8 +276,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : DEEP ? 4 : 5) top_segment_
                 keys_out[i] = key;
             }
         }
-        left = block_join<NT>(left, buf, c);
-        if (got < n) left = join(below, left, c);  // else there is nothing below, and a NaN in that sum is a candidate
+        left = block_join<NT, true>(left, buf, c);
+        if (got < n) left = join<true>(below, left, c);  // else there is nothing below, and a NaN in that sum is a candidate
     } else {
         long last = 0x7fffffffffffffffL;
         for (int r = 0; r < want; ++r) {
@@ -320,10 +324,10 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : DEEP ? 4 : 5) top_segment_
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 const int at = (j * NT + t) * VEC + e;
-                if (at < n && key_of(f[e], c0 + at) < last) left = join(left, one(f[e]), c);
+                if (at < n && key_of(f[e], c0 + at) < last) left = join<true>(left, one(f[e]), c);
             }
         }
-        left = block_join<NT>(left, buf, c);
+        left = block_join<NT, true>(left, buf, c);
     }
     if (t == 0) {
         if (nseg == 1) rest[row] = log_of(left, inv_t);
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(kT) top_merge_kernel(const long* __restrict__ 
     for (int i = t; i < n; i += kT) held[i] = keys[i];
     __syncthreads();
     Sum sum = {-INFINITY, 0.f};
-    for (int i = t; i < nseg; i += kT) sum = join(sum, part_sums[row * nseg + i], c);
+    for (int i = t; i < nseg; i += kT) sum = join<true>(sum, part_sums[row * nseg + i], c);
     for (int i = t; i < n; i += kT) {
         const long key = held[i];
         if (key == kNoKey) continue;
@@ -359,10 +363,10 @@ __global__ void __launch_bounds__(kT) top_merge_kernel(const long* __restrict__ 
             values[row * k + rank] = value_of((int)(key >> 32));
             indices[row * k + rank] = index_of(key);
         } else {
-            sum = join(sum, one(value_of((int)(key >> 32))), c);
+            sum = join<true>(sum, one(value_of((int)(key >> 32))), c);
         }
     }
-    sum = block_join<kT>(sum, buf, c);
+    sum = block_join<kT, true>(sum, buf, c);
     if (t == 0) rest[row] = log_of(sum, inv_t);
 }
 // The same for more entries than are worth counting: one wave per row, k rounds over the heads of the sorted lists.
@@ -399,13 +403,13 @@ __global__ void __launch_bounds__(64) top_merge_long_kernel(const long* __restri
     }
     Sum sum = {-INFINITY, 0.f};
     for (int i = l; i < nseg; i += 64) {
-        sum = join(sum, part_sums[row * nseg + i], c);
+        sum = join<true>(sum, part_sums[row * nseg + i], c);
         for (int r = head[i]; r < k; ++r) {
             const long key = keys[(long)i * k + r];
-            if (key != kNoKey) sum = join(sum, one(value_of((int)(key >> 32))), c);
+            if (key != kNoKey) sum = join<true>(sum, one(value_of((int)(key >> 32))), c);
         }
     }
-    sum = wave_join(sum, c);
+    sum = wave_join<true>(sum, c);
     if (l == 0) rest[row] = log_of(sum, inv_t);
 }
 
@@ -626,7 +630,7 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
             __syncthreads();
             if (here) bits[(idx - s0) >> 5] = 0;
         }
-        const Sum unlisted = block_join<NT>(sum, buf, c);
+        const Sum unlisted = block_join<NT, false>(sum, buf, c);
         if (t < 64) {
             const bool valid = idx >= 0 && idx < C, bad = __any(idx >= C);
             const float zi = valid ? load_elem<T>(p, idx) : -INFINITY;
@@ -845,9 +849,9 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
             float zi;
             if constexpr (KM > 0) zi = zl[s];
             else zi = list.index(s) >= 0 && list.index(s) < C ? load_elem<T>(p, list.index(s) * inner) : -INFINITY;
-            if (list.first(s)) in = join(in, {zi, zi == -INFINITY ? 0.f : 1.f + (zi - zi)}, c);  // +inf has no softmax: NaN
+            if (list.first(s)) in = join<false>(in, one(zi), c);
         }
-        float4 st = row_stats(un, join(un, in, c));
+        float4 st = row_stats(un, join<false>(un, in, c));
         if (bad) st.x = st.z = NAN;
         const float lr = (r - vtop) * c;
         float total = exp2_(lr);
