@@ -70,6 +70,27 @@ __device__ __forceinline__ Sum join(Sum a, Sum b, float c) {
     return {m, a.s * term<INF>(a.m, ref, c) + b.s * term<INF>(b.m, ref, c)};
 }
 __device__ __forceinline__ Sum one(float x) { return {x, x == -INFINITY ? 0.f : 1.f}; }
+// The same taken by one lane over any number of logits, 32 at a time: the sums of 32 are added with what the additions before lost
+// put back (compensated), and the reference moves only where a logit exceeds it by more than kRaise powers of two, so the error
+// is that of 32 additions whatever the number (70001 equal logits behind one a little larger, added one by one: the logarithm 6.5e-4 off).
+constexpr float kRaise = 8.f;
+constexpr int kAtOnce = 32;
+struct LongSum {
+    float ref = -INFINITY, total = 0.f, lost = 0.f;
+    __device__ __forceinline__ bool raises(float x, float c) const { return (x - ref) * c > kRaise; }
+    __device__ __forceinline__ float raise(float to, float c) {  // the factor, for what has not been added yet
+        const float f = exp2_((ref - to) * c);
+        total *= f;
+        lost *= f;
+        ref = to;
+        return f;
+    }
+    __device__ __forceinline__ void add(float part) {
+        const float y = part - lost, t = total + y;
+        lost = (t - total) - y;
+        total = t;
+    }
+};
 __device__ __forceinline__ float log_of(Sum v, float inv_t) { return v.s == 0.f ? -INFINITY : v.m * inv_t + log2_(v.s) * kLn2; }
 template <bool INF>
 __device__ __forceinline__ Sum wave_join(Sum v, float c) {
@@ -256,8 +277,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 7 : DEEP ? 4 : 5) top_segment_
     const int got = count;
     Sum left = {-INFINITY, 0.f};
     // The list decides when it holds every candidate.  The sum decides unless a NaN went by in it, or it is so small against its
-    // reference that terms of it may have been flushed
-    if (chunks <= kQueue && got <= kCand && (got >= n || below.s >= 1e-30f)) {
+    // reference that the terms flushed from it count: up to 16384, each below 2^-126, are under 2^-24 of a sum of 2^-88
+    if (chunks <= kQueue && got <= kCand && (got >= n || below.s >= 0x1p-88f)) {
         for (int i = t; i < got; i += NT) {
             const long key = cand[i];
             int rank = 0;
@@ -452,7 +473,8 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
 #pragma unroll
         for (int s = 0; s < KM; ++s) at[s] = 0;
     }
-    Sum sum = {-INFINITY, 0.f};
+    LongSum sum;
+    float part = 0.f;
 #pragma unroll 4
     for (int j = 0; j < C; ++j) {
         float out;
@@ -481,12 +503,14 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
                 }
             out = value_of(a);
         }
-        if (out != -INFINITY) {
-            const float d = out - sum.m, e = out == sum.m ? 1.f : exp2_(-fabsf(d) * c);
-            sum.s = d > 0.f ? fmaf(sum.s, e, 1.f) : sum.s + e;
-            sum.m = fmaxf(sum.m, out);
+        if (sum.raises(out, c)) part *= sum.raise(out, c);
+        part += out == -INFINITY ? 0.f : term<true>(out, sum.ref, c);
+        if ((j & (kAtOnce - 1)) == kAtOnce - 1) {
+            sum.add(part);
+            part = 0.f;
         }
     }
+    sum.add(part);
 #pragma unroll
     for (int s = 0; s < KM; ++s)
         if (s < k) {
@@ -494,7 +518,7 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
             else values[(o * k + s) * inner + i] = value_of(v[s]);
             indices[(o * k + s) * inner + i] = SMALL ? 0xffff - (v[s] & 0xffff) : at[s];
         }
-    rest[row] = log_of(sum, inv_t);
+    rest[row] = log_of({sum.ref, sum.total}, inv_t);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -598,12 +622,12 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
                     for (int e = 0; e < VEC; ++e) top = fmaxf(top, f[u][e]);
                 }
                 const float m = fmaxf(sum.m, top), ref = finite_ref(m);
-                float s = sum.s * exp2_((sum.m - ref) * c);
+                float s = 0.f;  // a turn's terms by themselves: the long row's sum takes one addition for them
 #pragma unroll
                 for (int u = 0; u < N; ++u)
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) s += exp2_((f[u][e] - ref) * c);
-                sum = {m, s};
+                sum = {m, fmaf(sum.s, exp2_((sum.m - ref) * c), s)};
             };
             // whole turns of U chunks a thread, loaded without a test each (a load behind a branch of its own is waited for there)
             // and one turn ahead; then the rest chunk by chunk
@@ -788,7 +812,7 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
                                                                 const float* __restrict__ rest, const unsigned char* __restrict__ mask,
                                                                 float temp, float inv_t, float4* __restrict__ stats,
                                                                 float* __restrict__ row_loss, double* __restrict__ parts) {
-    constexpr int U = 32;  // classes at a time
+    constexpr int U = kAtOnce;  // classes at a time
     const float c = inv_t * kLog2e;
     double lsum = 0.0, lcount = 0.0;
     for (long row = blockIdx.x * (long)kT + threadIdx.x; row < rows; row += (long)gridDim.x * kT) {
@@ -816,7 +840,7 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
 #pragma unroll
             for (int s = 0; s < KM; ++s) zl[s] = list.idx[s] >= 0 && list.idx[s] < C ? load_elem<T>(p, list.idx[s] * inner) : -INFINITY;
         }
-        Sum un = {-INFINITY, 0.f}, in = {-INFINITY, 0.f};
+        LongSum sum;
         for (int c0 = 0; c0 < C; c0 += U) {
             if (c0 > 0) load_classes<T, U>(p, c0, C, inner, f);
             unsigned w = C - c0 < U ? ~0u << (C - c0) : 0u;  // what drops out of the sum: the listed classes, and those past the last
@@ -824,7 +848,7 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
                 const unsigned at = (unsigned)(list.index(s) - c0);
                 w |= at < U ? 1u << at : 0u;
             }
-            float mu = un.m;
+            float mu = -INFINITY;
 #pragma unroll
             for (int e0 = 0; e0 < U; e0 += 8)
                 if (c0 + e0 < C) {
@@ -835,16 +859,19 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
                         mu = max3(mu, f[e], f[e + 1]);
                     }
                 }
-            const float ru = finite_ref(mu);
-            float su = un.s * exp2_((un.m - ru) * c);
+            if (sum.raises(mu, c)) sum.raise(mu, c);
+            const float ru = finite_ref(sum.ref);
+            float su = 0.f;
 #pragma unroll
             for (int e0 = 0; e0 < U; e0 += 8)
                 if (c0 + e0 < C) {
 #pragma unroll
                     for (int e = e0; e < e0 + 8; ++e) su += exp2_((f[e] - ru) * c);
                 }
-            un = {mu, su};
+            sum.add(su);
         }
+        const Sum un = {sum.ref, sum.total};
+        Sum in = {-INFINITY, 0.f};
         LIST_FOR(s) {
             float zi;
             if constexpr (KM > 0) zi = zl[s];

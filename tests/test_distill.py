@@ -605,3 +605,68 @@ def test_infinite_student_logits(hip_lib):
         grad = grad[0].t() if dim == 1 else grad
         assert row.reshape(-1).isnan().tolist() == [False, True, True, False]
         assert grad.isnan().all(1).tolist() == [False, True, True, False] and bool(torch.isfinite(grad[[0, 3]]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("kind", ["equal", "ascending", "descending", "far apart", "random"])
+@pytest.mark.parametrize("C,k", [(70001, 1), (131072, 8), (70001, 40)])
+def test_long_sums_of_one_lane(hip_lib, dt, kind, C, k):
+    """maps give a lane all classes of a position: an addition at a time would lose n / 2 steps where the terms are alike.  The sums
+    are taken 32 terms at a time and added with compensation, so 32 roundings (and 2) stand in the place of the n / 16 above."""
+    from msf_wsi_amd import losses
+
+    dt = FP[dt]
+    if kind == "equal":                                     # behind two that are a little larger
+        one = torch.zeros(C)
+        one[0], one[1] = 0.3, 0.2
+    elif kind == "ascending":
+        one = torch.arange(C) / C
+    elif kind == "descending":
+        one = -torch.arange(C) / C
+    elif kind == "far apart":                               # the reference of the sum moves again and again
+        one = torch.arange(C) / C * 300 - 200
+    else:
+        one = torch.randn(C, generator=torch.Generator().manual_seed(C))
+    x = torch.stack([one, one.roll(C // 2), one + 0.25, one.roll(77)]).to(dt)
+    E = (3 * float((x.double().amax(1) - x.double().amin(1)).max()) + 34 + 64) * U
+    maps = x.view(2, 2, C).movedim(-1, 1).contiguous().cuda()
+    got = losses.top_logits(maps, k, dim=1)
+    v, i, r = to.top_logits(x, k, 1.0)
+    assert torch.equal(got.indices.movedim(1, -1).reshape(4, k).cpu().long(), i)
+    assert bool(((got.rest.reshape(4).cpu().double() - r).abs() <= E + 2 * U * r.abs()).all())
+    teacher = losses.TopLogits(torch.zeros(2, k, 2, device="cuda"), torch.arange(k, dtype=torch.int32, device="cuda").view(1, k, 1).repeat(2, 1, 2))
+    z = maps.requires_grad_()
+    row = losses.TopLogitDistillLoss(1.0, "none", dim=1)(z, teacher)
+    grad, = torch.autograd.grad(row, z, torch.ones_like(row))
+    want, wgrad, _ = to.distill(x, torch.zeros(4, k), torch.arange(k).repeat(4, 1), None, None, 1.0)
+    # the k entries' terms are added one by one, each addition off by U of a sum of at most the loss itself (here up to 302, U of which
+    # times 40 is 7e-4, while E is 6e-5), each term by two roundings
+    assert bool(((row.detach().reshape(4).cpu().double() - want).abs() <= E + (k + 2) * U * want.abs()).all())
+    size = torch.softmax(x.double(), 1)
+    size[:, :k] += 1.0 / k
+    # An exponential below 2^-126 is 0 in the kernels and its factor T (q_r - p_r) here at most 1, so an element may be off by up to
+    # 2^-126 (300 apart, the smallest q are e^-300: all elements past the tolerance without this term held less than 2^-126)
+    tiny = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24}[dt]
+    err = (grad.movedim(1, -1).reshape(4, C).cpu().double() - wgrad).abs()
+    assert bool((err <= 2 * E * size + torch.finfo(dt).eps / 2 * wgrad.abs() * (1 + 1e-5) + tiny).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+@pytest.mark.parametrize("small", [-68.5, -62.0, -60.5])
+def test_rest_far_below_the_list(hip_lib, dt, small):
+    """one class small enough that the thousands below it, each just too small for the list's scale, make a part of its size: a
+    lane's 64 terms and the sums' tree are all that may be lost"""
+    from msf_wsi_amd import losses
+
+    C = 8192 if dt == "fp32" else 16384
+    x = torch.full((3, C), -87.5)
+    x[:, [5, 777, 2100, 4000]] = 0.0
+    for r, at in enumerate((0, 3001, C - 1)):
+        x[r, at] = small
+    x = x.to(FP[dt])
+    got = losses.top_logits(x.cuda(), 4)
+    _, i, r = to.top_logits(x, 4, 1.0)
+    assert torch.equal(got.indices.cpu().long(), i)
+    assert bool(((got.rest.cpu().double() - r).abs() <= (3 * 87.5 + 128 + 64) * U + 2 * U * r.abs()).all())
