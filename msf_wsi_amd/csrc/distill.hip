@@ -524,17 +524,20 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// The loss.  What the backward keeps of a row, in four floats: m and ls = log2 s of the sum over all classes (struct Sum), and the
-// same, mt and lt, over the unlisted ones.  Two maxima, because the unlisted classes may lie so far below the
-// listed ones that their sum relative to m would vanish.  A sum is at least 1, its logarithm at least 0: ls = -1 marks a row that
-// does not count.
+// The loss.  What the backward keeps of a row, in four floats: m and s of the sum over all classes (struct Sum), and the
+// same, mt and st, over the unlisted ones.  Two maxima, because the unlisted classes may lie so far below the
+// listed ones that their sum relative to m would vanish.  s = -1 marks a row that does not count.  The sums themselves and not their
+// logarithms: log2 s of 65536 classes has a step of 2^-20, and as a part of the exponent it put every q of a row off by up to
+// 6 2^-24; a product with 1 / s is off by 2 2^-24.
 // ---------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float4 row_stats(Sum unlisted, Sum all) {
     const float m = finite_ref(all.m);
-    return make_float4(m, all.s == 0.f ? 0.f : log2_(all.s), unlisted.m == -INFINITY ? m : unlisted.m,
-                       unlisted.s == 0.f ? 0.f : log2_(unlisted.s));
+    return make_float4(m, all.s, unlisted.m == -INFINITY ? m : unlisted.m, unlisted.s);
 }
 __device__ __forceinline__ bool row_counts(const float4& st) { return st.y != -1.f; }
+__device__ __forceinline__ float log2_sum(float s) { return s == 0.f ? 0.f : log2_(s); }
+// 1 / s, 1 ulp; 0 of an empty sum, so that a softmax over nothing is zero
+__device__ __forceinline__ float part_of(float s) { return s == 0.f ? 0.f : __builtin_amdgcn_rcpf(s); }
 
 // (sum, count) of the rows that count, one pair per workgroup, joined in a fixed order
 template <int NT>
@@ -669,13 +672,14 @@ __global__ void __launch_bounds__(NT) distill_fwd_kernel(const T* __restrict__ z
             const Sum all = {m, unlisted.s * exp2_((unlisted.m - ref) * c) + wave_sum(first ? exp2_((zi - ref) * c) : 0.f)};
             float4 st = row_stats(unlisted, all);
             if (bad) st.x = st.z = NAN;
+            const float ls = log2_sum(st.y), lt = log2_sum(st.w);
             // teacher, in base-2 units relative to its largest entry
             const float lv = (v - vtop) * c, lr = (r - vtop) * c;
             const float L = log2_(wave_sum(lane < k ? exp2_(lv) : 0.f) + exp2_(lr));
             const float pi = lane < k ? exp2_(lv - L) : 0.f, pr = exp2_(lr - L);
-            float term = pi != 0.f ? pi * ((lv - L) - ((zi - st.x) * c - st.y)) : 0.f;
+            float term = pi != 0.f ? pi * ((lv - L) - ((zi - st.x) * c - ls)) : 0.f;
             if (lane == 0 && pr != 0.f) {
-                const float lq = unlisted.s == 0.f ? -INFINITY : (st.z - st.x) * c + st.w - st.y;
+                const float lq = unlisted.s == 0.f ? -INFINITY : (st.z - st.x) * c + lt - ls;
                 term += pr * ((lr - L) - lq);
             }
             const float loss = temp * temp * kLn2 * wave_sum(term);
@@ -716,11 +720,10 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
     const int idx = lane < k ? indices[row * k + lane] : -1;
     const float v = idx >= 0 ? values[row * k + lane] : -INFINITY, r = rest != nullptr ? rest[row] * temp : -INFINITY;
     const float vtop = wave_max(v != v || r <= v ? v : r);
-    const float lv = (v - vtop) * c, lr = (r - vtop) * c;
-    const float L = log2_(wave_sum(lane < k ? exp2_(lv) : 0.f) + exp2_(lr));
-    const float pi = lane < k ? exp2_(lv - L) : 0.f, pr = exp2_(lr - L);
+    const float wi = lane < k ? exp2_((v - vtop) * c) : 0.f, wr = exp2_((r - vtop) * c);
+    const float share_of = part_of(wave_sum(wi) + wr), pi = wi * share_of, pr = wr * share_of;
     const float gs = g[g_rows ? row : 0] * (factor != nullptr ? *factor : 1.f) * temp;
-    const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - pr);
+    const float q_of = part_of(st.y), outside = gs * (exp2_((st.z - st.x) * c) * (st.w * q_of) - pr) * part_of(st.w);
     int a = 0;
     for (; a + U * NT * VEC <= C; a += U * NT * VEC) {
         uint4 raw[U];
@@ -731,7 +734,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
             float f[VEC];
             unpack16<T>(raw[u], f);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) f[e] = outside * exp2_((f[e] - st.z) * c - st.w);
+            for (int e = 0; e < VEC; ++e) f[e] = outside * exp2_((f[e] - st.z) * c);
             store_chunk<T>(d, a + (u * NT + t) * VEC, C, f);
         }
     }
@@ -739,7 +742,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
         float f[VEC];
         unpack16<T>(load_chunk<T>(p, a, C), f);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f[e] = outside * exp2_((f[e] - st.z) * c - st.w);
+        for (int e = 0; e < VEC; ++e) f[e] = outside * exp2_((f[e] - st.z) * c);
         store_chunk<T>(d, a, C, f);
     }
     __syncthreads();
@@ -750,7 +753,7 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
         const float po = __shfl(pi, q, 64);
         share += other == idx ? po : 0.f;
     }
-    if (idx >= 0 && idx < C) store_elem<T>(d, idx, gs * (exp2_((load_elem<T>(p, idx) - st.x) * c - st.y) - share));
+    if (idx >= 0 && idx < C) store_elem<T>(d, idx, gs * (exp2_((load_elem<T>(p, idx) - st.x) * c) * q_of - share));
 }
 
 // One thread per row: maps, and rows of a few classes.  A class costs about 7 instructions: the listed ones are taken out of the
@@ -882,19 +885,20 @@ __global__ void __launch_bounds__(kT) distill_thread_fwd_kernel(const T* __restr
         }
         float4 st = row_stats(un, join<false>(un, in, c));
         if (bad) st.x = st.z = NAN;
+        const float ls = log2_sum(st.y), lt = log2_sum(st.w);
         const float lr = (r - vtop) * c;
         float total = exp2_(lr);
         LIST_FOR(s) total += exp2_((list.value(s) - vtop) * c);
         const float L = log2_(total), pr = exp2_(lr - L);
         float loss = 0.f;
-        if (pr != 0.f) loss = pr * ((lr - L) - (un.s == 0.f ? -INFINITY : (st.z - st.x) * c + st.w - st.y));
+        if (pr != 0.f) loss = pr * ((lr - L) - (un.s == 0.f ? -INFINITY : (st.z - st.x) * c + lt - ls));
         LIST_FOR(s) {
             const float lp = (list.value(s) - vtop) * c - L, pi = exp2_(lp);
             const int at = list.index(s);
             float zi;
             if constexpr (KM > 0) zi = zl[s];
             else zi = at >= 0 && at < C ? load_elem<T>(p, at * inner) : 0.f;
-            if (pi != 0.f && at >= 0 && at < C) loss += pi * (lp - ((zi - st.x) * c - st.y));
+            if (pi != 0.f && at >= 0 && at < C) loss += pi * (lp - ((zi - st.x) * c - ls));
         }
         loss = bad ? NAN : temp * temp * kLn2 * loss;
         stats[row] = st;
@@ -936,23 +940,23 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
         const float v = list.value(s);
         vtop = vtop != vtop || v <= vtop ? vtop : v;
     }
-    const float lr = (r - vtop) * c;
-    float total = exp2_(lr);
+    const float wr = exp2_((r - vtop) * c);
+    float total = wr;
     LIST_FOR(s) total += exp2_((list.value(s) - vtop) * c);
-    const float L = log2_(total);
+    const float share_of = part_of(total), q_of = part_of(st.y);
     const float gs = g[g_rows ? row : 0] * (factor != nullptr ? *factor : 1.f) * temp;
-    const float outside = gs * (exp2_((st.z - st.x) * c + st.w - st.y) - exp2_(lr - L));
+    const float outside = gs * (exp2_((st.z - st.x) * c) * (st.w * q_of) - wr * share_of) * part_of(st.w);
     float listed[KM > 0 ? KM : 1];  // the listed classes' gradients
     if constexpr (KM > 0) {
         float pi[KM];
 #pragma unroll
-        for (int s = 0; s < KM; ++s) pi[s] = s < k ? exp2_((list.value(s) - vtop) * c - L) : 0.f;
+        for (int s = 0; s < KM; ++s) pi[s] = s < k ? exp2_((list.value(s) - vtop) * c) * share_of : 0.f;
 #pragma unroll
         for (int s = 0; s < KM; ++s) {
             float share = 0.f;
 #pragma unroll
             for (int q = 0; q < KM; ++q) share += list.idx[q] == list.idx[s] ? pi[q] : 0.f;
-            listed[s] = gs * (exp2_((zl[s] - st.x) * c - st.y) - share);
+            listed[s] = gs * (exp2_((zl[s] - st.x) * c) * q_of - share);
         }
     }
     for (int c0 = 0; c0 < C; c0 += U) {
@@ -960,7 +964,7 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
 #pragma unroll
         for (int e = 0; e < U; ++e)
             if (c0 + e < C) {
-                float v = outside * exp2_((f[e] - st.z) * c - st.w);
+                float v = outside * exp2_((f[e] - st.z) * c);
                 if constexpr (KM > 0) {
                     LIST_FOR(s) v = list.idx[s] == c0 + e ? listed[s] : v;
                 }
@@ -972,8 +976,8 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
             const int at = list.index(s);
             if (at < 0 || at >= C) continue;
             float share = 0.f;
-            for (int q = 0; q < k; ++q) share += list.index(q) == at ? exp2_((list.value(q) - vtop) * c - L) : 0.f;
-            store_elem<T>(d, at * inner, gs * (exp2_((load_elem<T>(p, at * inner) - st.x) * c - st.y) - share));
+            for (int q = 0; q < k; ++q) share += list.index(q) == at ? exp2_((list.value(q) - vtop) * c) * share_of : 0.f;
+            store_elem<T>(d, at * inner, gs * (exp2_((load_elem<T>(p, at * inner) - st.x) * c) * q_of - share));
         }
     }
 }

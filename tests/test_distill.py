@@ -670,3 +670,25 @@ def test_rest_far_below_the_list(hip_lib, dt, small):
     _, i, r = to.top_logits(x, 4, 1.0)
     assert torch.equal(got.indices.cpu().long(), i)
     assert bool(((got.rest.cpu().double() - r).abs() <= (3 * 87.5 + 128 + 64) * U + 2 * U * r.abs()).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["rows", "maps"])
+@pytest.mark.parametrize("k", [2, 9, 40])
+def test_gradient_keeps_the_last_bits(hip_lib, layout, k):
+    """equal logits: every exponential is 1 and every sum exact, so what is left are the two reciprocals (2 U each), q_r's two products,
+    the one with its share and the one with the gradient that arrives: 8 U of an unlisted class; of a listed one 4 U of q and of p"""
+    from msf_wsi_amd import losses
+
+    for C in (1000, 5003, 20011, 40003, 60000, 65535, 100003):
+        z = torch.full((2, C), -0.75)
+        i = (torch.arange(k) * 7).int().repeat(2, 1)
+        zl, il = (a.t()[None].contiguous().cuda() if layout == "maps" else a.cuda() for a in (z, i))
+        zl.requires_grad_()
+        row = losses.TopLogitDistillLoss(1.0, "none", dim=1 if layout == "maps" else -1)(zl, losses.TopLogits(torch.zeros_like(il, dtype=torch.float32), il))
+        grad, = torch.autograd.grad(row, zl, torch.ones_like(row))
+        grad = (grad[0].t() if layout == "maps" else grad).double().cpu()
+        listed = torch.zeros(C, dtype=torch.bool)
+        listed[i[0].long()] = True
+        assert float((grad[:, ~listed] - 1 / C).abs().max()) <= 8 * U / C, C
+        assert float((grad[:, listed] - (1 / C - 1 / k)).abs().max()) <= 4 * U * (1 / C + 1 / k), C
