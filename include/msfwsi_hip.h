@@ -534,7 +534,10 @@ int msfwsi_inverse_perm(const long* perm, long* inv, long rows, int K, void* str
  *   msfwsi_mx4_gemm:       y[m][n] = sum_k a[m][k] b[n][k] (+ bias[n], fp32), both operands quantised, fp32 sums, y [M][N]
  *   msfwsi_mx4_linear:     mx4_quantize of x [M][cols] and mx4_gemm of the result with w [N][cols], in one call
  *   msfwsi_mx4_dgrad:      dx[m][k] = sum_n dy[m][n] w[n][k], w [N][cols] quantised; dy rows `ld` elements apart, dx [M][cols];
- *                          the products are exact whatever dy's type.  N, cols <= 2^21 (N also for mx4_gemm)
+ *                          the products are exact whatever dy's type and size, with one exception: beside an E >= 96 in the
+ *                          same 32 columns, weights with E < 8 meet the first 8 bits of an fp32 dy alone and weights with E < 16
+ *                          the first 16 (and beside an E > 252 weights with E < 2 count as 0).  N, cols <= 2^21 (N also for
+ *                          mx4_gemm)
  *   msfwsi_mx4_*_workspace:  host calls; *bytes = what the launch with the same arguments needs at `workspace` (16-byte
  *                          aligned; NULL when it is 0) */
 int msfwsi_mx4_quantize(int dtype, const void* x, long ld, long rows, long cols, void* codes, void* scales, void* stream);

@@ -468,7 +468,10 @@ __global__ void __launch_bounds__(kT) mx4_join_kernel(const float* __restrict__ 
 }
 
 // dy in the form the gradient's tiles take: `parts` matrices [M][pitch] of 16-bit values, zeros behind the last column.  fp32 is
-// cut into three bf16 parts that add up to it exactly (each takes the next 8 bits); 16-bit types are copied.
+// cut into three bf16 parts, each the next 8 bits, part p times 2^(kPartUp p) (it meets weights that much smaller): they add up to it
+// exactly over all of fp32's range, where plain parts of values below 2^-110 would lose the bits below bf16's last, 2^-133.
+// 16-bit types are copied.
+constexpr int kPartUp = 8;
 template <typename T, int PARTS>
 __global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy, long ld, long M, long N, long pitch, unsigned short* __restrict__ out) {
     const long total = M * pitch;
@@ -482,7 +485,7 @@ __global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy,
             for (int p = 0; p < PARTS; ++p) {
                 const unsigned top = __float_as_uint(left) & 0xffff0000u;  // towards zero: never past the largest number
                 out[p * total + i] = (unsigned short)(left != left ? 0x7fc0u : top >> 16);
-                left = left != left || __uint_as_float(top) == left ? 0.f : left - __uint_as_float(top);
+                left = left != left || __uint_as_float(top) == left ? 0.f : (left - __uint_as_float(top)) * (float)(1 << kPartUp);
             }
         }
     }
@@ -491,9 +494,11 @@ __global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy,
 // dx = dy W for a frozen W: 256 rows x 256 columns (one group of W's) per workgroup of 8 waves, 64 rows of W a step.  dy comes
 // by DMA like the tiles above; W's codes (8 KB a step) are widened to 16 bits on the way into LDS [n][column] and read transposed
 // (ds_read_b64_tr_b16), even and odd columns apart as above.  The scale of a weight varies along the sum, so it is applied while
-// widening -- relative to the largest scale of its 32 columns over this workgroup's rows of W, which the outputs are multiplied with in the end:
-// no weight can overflow, and bf16 keeps weights down to 2^-126 of the largest.  fp16 holds scales that are at most 2^26 apart
-// exactly; where a workgroup finds them further apart it cuts each dy value into two bf16 parts (8 + 3 bits) instead.
+// widening.  bf16 holds every weight as it is (subnormals too, which conversion and products keep), so that sums overflow where the
+// result does and not before; raised() says where the weights of 32 columns are moved by a power of two, undone in the end.  fp16
+// weights are taken relative to the largest scale of their 32 columns over all rows of W (dy is at most 65504: no sum can overflow), which
+// holds scales that are at most 2^26 apart exactly; where a workgroup finds them further apart it cuts each dy value into two bf16
+// parts (8 + 3 bits) instead.
 // Bound by the 16-bit matrix rate and the widening beside it: 8192 x 8192 x 8192 bf16 991 us, 1.1 PFLOP/s (the library's product of 16-bit
 // matrices 1.38); 8192 x 9216 x 9216 fp16 1516 us.
 template <typename T, bool CUT>
@@ -528,6 +533,11 @@ __device__ __forceinline__ uint4 widen8(unsigned codes, float scale) {
 }
 
 typedef __attribute__((ext_vector_type(2))) unsigned short u16x2;
+
+// The power of two that bf16 weights of 32 columns are raised by, from their largest E.  Above 252, 6 * 2^(E - 127) is past bf16's
+// largest number.  Below 96 there is room: 2^21 products of fp32's largest number stay under 2^121, and the weights that the low
+// parts of an fp32 dy meet, smaller by 2^8 and 2^16, stay above the smallest scale.
+__device__ __forceinline__ int raised(int emax) { return emax > 252 ? 252 - emax : min(max(96 - emax, 0), 32); }
 
 struct DgradArgs {
     const unsigned char *dy, *codes, *scales;
@@ -572,10 +582,11 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
             e = 0;
         }
     };
-    const int base = emax[kb];
-    auto store_b = [&](const uint4& c, int e, char* st) {
-        const int x = e == 255 ? 255 : max(e - base + (CUT || !__is_same(T, _Float16) ? 127 : 140), 0);
-        const float scale = __uint_as_float(x == 255 ? 0x7fc00000u : (unsigned)x << 23);  // NaN whatever the codes
+    const int add = __is_same(TW, _Float16) ? 140 - emax[kb] : raised(emax[kb]);
+    auto store_b = [&](uint4 c, int e, char* st, int part) {
+        int x = e == 255 ? 255 : e + add - kPartUp * part;
+        if (x < 0) x = 0, c = make_uint4(0, 0, 0, 0);  // below the smallest scale
+        const float scale = __uint_as_float(x == 255 ? 0x7fc00000u : (unsigned)x << 23);  // 0 is 2^-127 here; NaN whatever the codes
         // columns 2i and 2i + 1 go to different fragments: the even ones of 64 columns first, then the odd ones, 64 bytes each.
         // Eight of them come from two words of codes in the order 0 4 1 5 2 6 3 7 (out_pair undoes it); which half of the 16 a
         // lane writes first depends on its block, so that a write's sixteen lanes fall on all 64 banks
@@ -620,7 +631,7 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
     uint4 c;
     int e;
     load_b(s0, c, e);
-    store_b(c, e, smem + 2 * kDA);
+    store_b(c, e, smem + 2 * kDA, s0 / nsteps);
     fill_a(s0, smem);
     load_b(min(s0 + 1, s1 - 1), c, e);
     for (int s = s0; s < s1; ++s) {
@@ -632,7 +643,7 @@ __device__ __forceinline__ void dgrad_loop(const DgradArgs& p, char* smem, const
         if (more) fill_a(s + 1, smem + (cur ^ 1) * kDA);
         compute(smem + cur * kDA, smem + 2 * kDA + cur * kDB, 0, 2);
         if (more) {
-            store_b(c, e, smem + 2 * kDA + (cur ^ 1) * kDB);
+            store_b(c, e, smem + 2 * kDA + (cur ^ 1) * kDB, (s + 1) / nsteps);
             load_b(min(s + 2, s1 - 1), c, e);
         }
         compute(smem + cur * kDA, smem + 2 * kDA + cur * kDB, 2, 4);
@@ -691,7 +702,7 @@ __global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    int bias = 127;
+    bool relative = false;
     if constexpr (__is_same(T, _Float16)) {
         bool wide = false;
         for (int i = 0; i < 8; ++i) wide |= emax[i] - emin[i] > 26;
@@ -699,7 +710,7 @@ __global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
             dgrad_loop<T, true>(p, smem, emax, acc, m0, g, s0, s1);
         } else {
             dgrad_loop<T, false>(p, smem, emax, acc, m0, g, s0, s1);
-            bias = 140;
+            relative = true;
         }
     } else {
         dgrad_loop<T, false>(p, smem, emax, acc, m0, g, s0, s1);
@@ -707,7 +718,7 @@ __global__ void __launch_bounds__(512) mx4_dgrad_kernel(const DgradArgs p) {
     const int wm = w >> 2, wn = w & 3, kc = wn * 64 + 2 * out_pair(l), left = (int)min(256L, p.cols - k0) - kc;
     const int mrows = (int)min(256L, p.M - m0), r0 = wm * 128 + 4 * h, cols = (int)p.cols;
     if (left <= 0) return;
-    const int up = emax[kc >> 5] - bias;
+    const int up = relative ? emax[kc >> 5] - 140 : -raised(emax[kc >> 5]);
     auto put = [&](auto* to, auto whole) {
         constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll

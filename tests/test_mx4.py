@@ -467,3 +467,74 @@ def test_module_cast_to_16_bits(hip_lib):
     x = features(5, 70, torch.bfloat16, 1).cuda()
     want = quant.mx4_linear(x, quant.MX4Tensor(layer.codes, layer.scales, 70), layer.bias.bfloat16().float())
     assert torch.equal(layer.bfloat16()(x), want)
+
+
+def stored(scale_codes, seed):
+    """a weight [rows, 64] of the given E, one a row, every code among its elements: (MX4Tensor, its values in float64)"""
+    from msf_wsi_amd import quant
+
+    rows = len(scale_codes)
+    g = torch.Generator().manual_seed(seed)
+    code = torch.randint(0, 16, (rows, 64), generator=g)
+    code[:, :16] = torch.arange(16)
+    codes = torch.zeros(1, rows, 128, dtype=torch.uint8)
+    codes[0, :, :32] = (code[:, 0::2] + 16 * code[:, 1::2]).to(torch.uint8)
+    e = torch.tensor(scale_codes)
+    level = torch.tensor(to.LEVELS, dtype=torch.float64)
+    values = torch.where(code > 7, -level[code % 8], level[code % 8]) * torch.exp2(e.double() - 127).view(rows, 1)
+    scales = torch.zeros(1, rows, 8, dtype=torch.uint8)
+    scales[0, :, :2] = e.view(rows, 1).to(torch.uint8)
+    return quant.MX4Tensor(codes.cuda(), scales.cuda(), 64), values
+
+
+def input_gradient(dy, w4):
+    from msf_wsi_amd import kernels as kn
+
+    dx = torch.empty(dy.shape[0], w4.shape[1], dtype=torch.float32, device="cuda")
+    kn.mx4_dgrad(dy.cuda(), w4.codes, w4.scales, dx)
+    return dx.cpu().double()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["fp32", "bf16"])
+@pytest.mark.parametrize("E", [20, 40, 100, 107, 127, 150, 200, 252])
+def test_gradient_over_the_whole_range_of_dy(hip_lib, dt, E):
+    """every output is one product: exact but for the additions of an fp32 value's three parts (2^-23) and the smallest subnormal,
+    and infinite only where the product itself is past the largest number"""
+    dt = FP[dt]
+    d = torch.tensor([3e38, -1e38, 1.7e37 * (1 + 2.0 ** -23), 1e30, 1.2345678, 2.0 ** -100 * (1 + 2.0 ** -23), 2.0 ** -115 * (1 + 2.0 ** -23),
+                      -(2.0 ** -125) * 1.2345678, 2.0 ** -126 * (2 - 2.0 ** -23), 2.0 ** -130 * 1.2345678, 2.0 ** -140 * 1.2345678, 2.0 ** -149]).to(dt)
+    w4, values = stored([E] * len(d), E)
+    want = d.double().view(-1, 1) * values
+    got = input_gradient(torch.diag(d), w4)
+    fits = want.abs() <= torch.finfo(torch.float32).max * (1 - 2.0 ** -22)
+    assert bool(((got - want).abs() <= 2.0 ** -23 * want.abs() + 2.0 ** -149)[fits].all())
+    over = want.abs() > torch.finfo(torch.float32).max * (1 + 2.0 ** -22)
+    assert bool(got[over].isinf().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", list(FP))
+def test_gradient_of_scales_far_apart(hip_lib, dt):
+    """all scales there are in the same columns; zeros of dy leave one weight to an output: exact, the smallest ones too"""
+    w4, values = stored(list(range(253)), 1)
+    assert torch.equal(input_gradient(torch.eye(253).to(FP[dt]), w4), values)
+    some = [3, 0, 17, 110, 120]                              # close together, the smallest among them
+    for k in range(1, 6):
+        w4, values = stored(some[:k], k)
+        assert torch.equal(input_gradient(torch.eye(k).to(FP[dt]) * 4, w4), values * 4)
+    w4, values = stored([254, 253, 252, 2, 127], 2)
+    d = torch.diag(torch.full((5,), 2.0 ** -10)).to(FP[dt])
+    want = values * 2.0 ** -10
+    assert bool(((input_gradient(d, w4) - want).abs() <= 2.0 ** -149).all())
+
+
+@pytest.mark.gpu
+def test_gradient_of_low_bits_beside_large_weights(hip_lib):
+    """fp32: 24 bits from E = 16 up whatever stands beside them, 16 from E = 8, 8 below"""
+    e = [0, 7, 8, 15, 16, 30, 252]
+    w4, values = stored(e, 3)
+    d = torch.full((7,), 1 + 2.0 ** -7 + 2.0 ** -15 + 2.0 ** -23)
+    got, want = input_gradient(torch.diag(d), w4), values * float(d[0])
+    for row, lost in enumerate([2.0 ** -7] * 2 + [2.0 ** -15] * 2 + [2.0 ** -23] * 3):
+        assert bool(((got[row] - want[row]).abs() <= lost * want[row].abs() + 2.0 ** -149).all()), e[row]
