@@ -538,3 +538,15 @@ def test_gradient_of_low_bits_beside_large_weights(hip_lib):
     got, want = input_gradient(torch.diag(d), w4), values * float(d[0])
     for row, lost in enumerate([2.0 ** -7] * 2 + [2.0 ** -15] * 2 + [2.0 ** -23] * 3):
         assert bool(((got[row] - want[row]).abs() <= lost * want[row].abs() + 2.0 ** -149).all()), e[row]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,cols", [(3, 33), (17, 300), (64, 1024)])
+def test_widened_to_16_bits(hip_lib, rows, cols):
+    """values rounded once to fp16 and bf16, large ones to infinity, small ones to subnormals and zero"""
+    from msf_wsi_amd import quant
+
+    x = features(rows, cols, torch.float32, rows) * torch.exp2(torch.linspace(-30, 20, rows)).view(-1, 1)
+    q, v = quant.quantize_mx4(x.cuda()), to.mx4_round(x)[0]
+    for dt in (torch.float16, torch.bfloat16):
+        assert torch.equal(q.dequantize(dt).cpu(), v.to(dt))
