@@ -550,3 +550,29 @@ def test_widened_to_16_bits(hip_lib, rows, cols):
     q, v = quant.quantize_mx4(x.cuda()), to.mx4_round(x)[0]
     for dt in (torch.float16, torch.bfloat16):
         assert torch.equal(q.dequantize(dt).cpu(), v.to(dt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 4, 20])
+def test_products_of_all_scales(hip_lib, rows):
+    """one product an output, scales from the smallest to the largest in both operands: exact, subnormal and infinite where the value is"""
+    from msf_wsi_amd import kernels as kn
+
+    e = [0, 1, 2, 40, 100, 126, 127, 128, 160, 230, 252, 253, 254]
+    b4, b = stored(e, 5)
+    for shift in range(0, len(e), 4):
+        a4, a = stored((e[shift:] + e[:shift]) * rows, 6)
+        only = torch.zeros(64, dtype=torch.bool)
+        only[[5, 40]] = True                                # one element of either block, never both of an output
+        keep = torch.zeros_like(a)
+        odd = torch.arange(a.shape[0]) % 2
+        keep[odd == 0, 5], keep[odd == 1, 40] = 1.0, 1.0
+        codes = a4.codes.cpu()
+        mask = torch.zeros(a.shape[0], 64, dtype=torch.uint8)
+        mask[keep > 0] = 15
+        codes[0, :, :32] &= mask[:, 0::2] | (mask[:, 1::2] << 4)
+        y = torch.empty(a.shape[0], len(e), dtype=torch.float32, device="cuda")
+        kn.mx4_gemm(codes.cuda(), a4.scales, b4.codes, b4.scales, 64, y)
+        want = (a * keep) @ b.t()
+        top = torch.finfo(torch.float32).max
+        assert torch.equal(y.cpu().double().clamp(-2 * top, 2 * top), torch.where(want.abs() > top, torch.sign(want) * 2 * top, want.float().double()))
