@@ -990,6 +990,8 @@ bool by_thread(long rows, int classes, long inner, int k, bool select) {
     return inner > 1 || (classes <= 128 && k <= 16 && rows >= classes * (select && k > 4 ? 1024L : 256L));
 }
 
+constexpr long kGridThreads = 0xffffffffL;  // of a launch; more rows take several
+
 bool layout_ok(long outer, int classes, long inner, long ld) {
     return outer >= 0 && classes > 0 && inner > 0 && (outer <= 1 || ld >= classes * inner) && (inner == 1 || ld == classes * inner) &&
            (outer == 0 || inner <= 0x7fffffffL / outer);
@@ -1036,26 +1038,34 @@ extern "C" int msfwsi_top_logits(int dtype, const void* x, long ld, long outer, 
     }
     const int nseg = segments(dtype, classes);
     const bool narrow = classes <= 64 * 4 * msfwsi_vec_of(dtype);
-    // heads of a merge in LDS; a grid holds < 2^32 threads
-    if (nseg > 4096 || outer > 0xffffffffL / ((narrow ? 64 : 256) * (long)nseg)) return MSFWSI_EUNSUPPORTED;
+    if (nseg > 4096) return MSFWSI_EUNSUPPORTED;  // heads of a merge in LDS
     MSFWSI_CHECK_ARG(nseg == 1 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0));
-    long* keys = (long*)workspace;
-    Sum* sums = (Sum*)(keys + outer * nseg * (long)k);
-#define TOP_ROWS(NT, NCH, DEEP)                                                                                                            \
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((top_segment_kernel<T, NT, NCH, DEEP>), dim3((unsigned)(outer * nseg)), dim3(NT), 0, ST(stream), \
-                                            (const T*)x, ld, classes, nseg, k, inv_t, values, indices, rest, keys, sums))
-    if (narrow && k <= 16) TOP_ROWS(64, 4, false);
-    else if (narrow) TOP_ROWS(64, 4, true);
-    else TOP_ROWS(256, 8, false);
-    const int rc = msfwsi_launch_status();
-    if (rc != MSFWSI_OK || nseg == 1) return rc;
-    if (nseg * k <= kMergeHeld)
-        hipLaunchKernelGGL(top_merge_kernel, dim3((unsigned)outer), dim3(kT), (size_t)nseg * k * 8, ST(stream), keys, sums, nseg, k, inv_t, values,
-                           indices, rest);
-    else
-        hipLaunchKernelGGL(top_merge_long_kernel, dim3((unsigned)outer), dim3(64), nseg * sizeof(int), ST(stream), keys, sums, nseg, k, inv_t,
-                           values, indices, rest);
-    return msfwsi_launch_status();
+    long* all_keys = (long*)workspace;
+    Sum* all_sums = (Sum*)(all_keys + outer * nseg * (long)k);
+    const long most = kGridThreads / (kT * (long)nseg);  // rows a launch; a merge takes kT threads a row
+    for (long r = 0; r < outer; r += most) {
+        const long rows = outer - r < most ? outer - r : most;
+        float *v = values + r * k, *re = rest + r;
+        int* at = indices + r * k;
+        long* keys = all_keys + r * nseg * k;
+        Sum* sums = all_sums + r * nseg;
+#define TOP_ROWS(NT, NCH, DEEP)                                                                                                           \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((top_segment_kernel<T, NT, NCH, DEEP>), dim3((unsigned)(rows * nseg)), dim3(NT), 0, ST(stream), \
+                                            (const T*)x + r * ld, ld, classes, nseg, k, inv_t, v, at, re, keys, sums))
+        if (narrow && k <= 16) TOP_ROWS(64, 4, false);
+        else if (narrow) TOP_ROWS(64, 4, true);
+        else TOP_ROWS(256, 8, false);
+        int rc = msfwsi_launch_status();
+        if (rc != MSFWSI_OK) return rc;
+        if (nseg == 1) continue;
+        if (nseg * k <= kMergeHeld)
+            hipLaunchKernelGGL(top_merge_kernel, dim3((unsigned)rows), dim3(kT), (size_t)nseg * k * 8, ST(stream), keys, sums, nseg, k, inv_t, v, at, re);
+        else
+            hipLaunchKernelGGL(top_merge_long_kernel, dim3((unsigned)rows), dim3(64), nseg * sizeof(int), ST(stream), keys, sums, nseg, k, inv_t, v, at, re);
+        rc = msfwsi_launch_status();
+        if (rc != MSFWSI_OK) return rc;
+    }
+    return MSFWSI_OK;
 }
 
 // How many threads take a row of adjacent classes.  One wave (no barriers) for short rows, longer ones too once there are 2048 of them
@@ -1126,13 +1136,18 @@ extern "C" int msfwsi_distill_bwd(int dtype, const void* z, long ld, long outer,
         return msfwsi_launch_status();
     }
     const int nt = row_threads(rows, classes);
-    if (rows > 0xffffffffL / nt) return MSFWSI_EUNSUPPORTED;  // a grid holds fewer than 2^32 threads
-#define BWD_ROWS(NT)                                                                                                                      \
-    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((distill_bwd_kernel<T, NT>), dim3((unsigned)rows), dim3(NT), 0, ST(stream), (const T*)z, ld, \
-                                            classes, rows, k, values, indices, rest, temperature, inv_t, (const float4*)stats, factor,   \
-                                            g, g_rows, (T*)dz))
-    if (nt == 64) BWD_ROWS(64);
-    else if (nt == 256) BWD_ROWS(256);
-    else BWD_ROWS(1024);
-    return msfwsi_launch_status();
+    const long most = kGridThreads / nt;
+    for (long r = 0; r < rows; r += most) {
+        const long n = rows - r < most ? rows - r : most;
+#define BWD_ROWS(NT)                                                                                                                          \
+    MSFWSI_WITH_T(dtype, hipLaunchKernelGGL((distill_bwd_kernel<T, NT>), dim3((unsigned)n), dim3(NT), 0, ST(stream), (const T*)z + r * ld, ld, \
+                                            classes, n, k, values + r * k, indices + r * k, rest != nullptr ? rest + r : nullptr, temperature, \
+                                            inv_t, (const float4*)stats + r, factor, g + (g_rows ? r : 0), g_rows, (T*)dz + r * classes))
+        if (nt == 64) BWD_ROWS(64);
+        else if (nt == 256) BWD_ROWS(256);
+        else BWD_ROWS(1024);
+        const int rc = msfwsi_launch_status();
+        if (rc != MSFWSI_OK) return rc;
+    }
+    return MSFWSI_OK;
 }

@@ -692,3 +692,27 @@ def test_gradient_keeps_the_last_bits(hip_lib, layout, k):
         listed[i[0].long()] = True
         assert float((grad[:, ~listed] - 1 / C).abs().max()) <= 8 * U / C, C
         assert float((grad[:, listed] - (1 / C - 1 / k)).abs().max()) <= 4 * U * (1 / C + 1 / k), C
+
+
+@pytest.mark.gpu
+def test_more_rows_than_a_launch_takes(hip_lib):
+    """2^26 rows of a wave each are all the threads of one launch: selection, loss and gradient of a few more, either side of that row"""
+    from msf_wsi_amd import losses
+
+    rows, C, k = 2 ** 26 + 77, 20, 17
+    pick = [0, 1, 2 ** 24 - 1, 2 ** 24, 2 ** 26 - 1, 2 ** 26, 2 ** 26 + 1, rows - 1]
+    small = logits_of(len(pick), C, torch.bfloat16, 9)
+    z = torch.zeros(rows, C, dtype=torch.bfloat16, device="cuda")
+    z[pick] = small.cuda()
+    teacher = losses.top_logits(z, k, 2.0)
+    some = losses.TopLogits(*(a[pick] for a in teacher))
+    same_top(small, k, 2.0, some)
+    assert teacher.indices[3].tolist() == list(range(k)) and teacher.indices[rows - 2].tolist() == list(range(k))
+    z[pick] = z[pick].flip(1)
+    z.requires_grad_()
+    weight = torch.zeros(rows, device="cuda")
+    weight[pick] = 1.0
+    row = losses.TopLogitDistillLoss(2.0, "none")(z, teacher)
+    grad, = torch.autograd.grad(row, z, weight)
+    check(small.flip(1), some.values, some.indices, some.rest, None, 2.0, row.detach()[pick], grad[pick], torch.bfloat16)
+    assert float(grad[3].abs().max()) == 0.0 and float(grad[rows - 2].abs().max()) == 0.0
