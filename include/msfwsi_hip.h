@@ -554,10 +554,10 @@ int msfwsi_mx4_dgrad(int dy_dtype, const void* dy, long ld, long M, const void* 
 
 /* ---- distillation from a teacher's largest logits (csrc/distill.hip: the formulas) ------------------------------------
  * Logits [outer][classes][inner]: inner = 1 with rows `ld` elements apart, or contiguous maps (ld = classes * inner).  values /
- * indices [outer][k][inner], rest and mask [outer * inner]; k <= 64.  No operator of the reference: no parity to pin.
+ * indices [outer][k][inner], rest and mask [outer * inner]; k <= 64, classes <= 2^30.  No operator of the reference: no parity to pin.
  *   msfwsi_top_logits:  the k largest (descending; ties by ascending index; NaN above all numbers), their indices, and
  *                       rest = log sum over the others of exp(logit * inv_t).  workspace: msfwsi_top_logits_workspace
- *                       bytes, 16-byte aligned (a host call; NULL when it says 0)
+ *                       bytes, 16-byte aligned (a host call; NULL when it says 0).  inner = 1: at most 2^26 classes (fp32: 2^25)
  *   msfwsi_distill_fwd: row_loss [rows] or NULL (0 where a row does not count), stats [rows][4] (16-byte aligned) for the
  *                       backward, partials [8192][2] scratch, *loss = sum or mean over the rows that count, *factor = the
  *                       gradient's (1 / their number for the mean, else 1).  rest / mask may be NULL.  outer = 0 writes loss and

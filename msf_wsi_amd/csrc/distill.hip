@@ -992,8 +992,10 @@ bool by_thread(long rows, int classes, long inner, int k, bool select) {
 
 constexpr long kGridThreads = 0xffffffffL;  // of a launch; more rows take several
 
+constexpr int kMaxClasses = 1 << 30;  // an int holds every class a walk steps to, past the last one too
+
 bool layout_ok(long outer, int classes, long inner, long ld) {
-    return outer >= 0 && classes > 0 && inner > 0 && (outer <= 1 || ld >= classes * inner) && (inner == 1 || ld == classes * inner) &&
+    return outer >= 0 && classes > 0 && classes <= kMaxClasses && inner > 0 && (outer <= 1 || ld >= classes * inner) && (inner == 1 || ld == classes * inner) &&
            (outer == 0 || inner <= 0x7fffffffL / outer);
 }
 
@@ -1008,7 +1010,7 @@ int segments(int dtype, int classes) {
 #define ST(s) reinterpret_cast<hipStream_t>(s)
 
 extern "C" int msfwsi_top_logits_workspace(int dtype, long outer, int classes, long inner, int k, long* bytes) {
-    MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && bytes && outer >= 0 && classes > 0 && inner > 0 && k > 0 && k <= kMaxK);
+    MSFWSI_CHECK_ARG(msfwsi_dtype_ok(dtype) && bytes && outer >= 0 && classes > 0 && classes <= kMaxClasses && inner > 0 && k > 0 && k <= kMaxK);
     const int nseg = segments(dtype, classes);
     *bytes = inner > 1 || nseg == 1 ? 0 : outer * nseg * (k + 1L) * 8;
     return MSFWSI_OK;

@@ -1674,6 +1674,7 @@ def dice_loss(logits, target, C1: int, classes, weight: float, loss_accum, dlogi
 # operand's device, whichever device is current; the small calls are bound by the host, so the checks are kept lean.
 MX4_GROUP = 256  # elements of a row stored together: 128 code bytes, 8 scale bytes
 TOP_LOGITS_MAX_K = 64
+LOGITS_MAX_CLASSES = 1 << 30  # the entry points take an int, which ctypes would cut a larger number down to
 _DT = {torch.float32: DT_F32, torch.bfloat16: DT_BF16, torch.float16: DT_F16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
 
@@ -1821,6 +1822,8 @@ def mx4_dgrad(dy, codes, scales, dx):
 
 def _logit_layout(z, name):
     """[rows, C] (any row pitch) or contiguous [N, C, inner]: (outer, classes, inner, ld)"""
+    if z.shape[1:] and z.shape[1] > LOGITS_MAX_CLASSES:
+        raise ValueError(f"{name}: {z.shape[1]} classes; at most {LOGITS_MAX_CLASSES} are supported")
     if z.dim() != 3:
         rows, Cn, ld = _rows2d(z, name)
         return rows, Cn, 1, ld

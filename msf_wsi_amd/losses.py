@@ -86,6 +86,8 @@ def _class_dim(logits: torch.Tensor, dim: int, what: str) -> int:
         raise ValueError(f"{what}: the class dimension must be the last one or dimension 1")
     if logits.shape[dim] == 0:
         raise ValueError(f"{what}: no classes in {tuple(logits.shape)}")
+    if logits.shape[dim] > kn.LOGITS_MAX_CLASSES:
+        raise ValueError(f"{what}: {logits.shape[dim]} classes; at most {kn.LOGITS_MAX_CLASSES} are supported")
     return dim
 
 

@@ -716,3 +716,21 @@ def test_more_rows_than_a_launch_takes(hip_lib):
     grad, = torch.autograd.grad(row, z, weight)
     check(small.flip(1), some.values, some.indices, some.rest, None, 2.0, row.detach()[pick], grad[pick], torch.bfloat16)
     assert float(grad[3].abs().max()) == 0.0 and float(grad[rows - 2].abs().max()) == 0.0
+
+
+def test_too_many_classes_are_refused(hip_lib):
+    """class counts that an int cannot step past (or hold at all) come back as errors before anything is launched"""
+    import ctypes
+
+    from msf_wsi_amd import kernels as kn
+
+    for C in (2 ** 30 + 1, 2 ** 31 - 1, 2 ** 32 + 5):
+        for shape in ((1, C), (2, C, 3)):
+            with pytest.raises(ValueError):
+                kn._logit_layout(torch.empty(shape, dtype=torch.bfloat16, device="meta"), "z")
+    need, at = ctypes.c_long(), 4096                        # an address that nothing reads
+    for C in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert hip_lib.msfwsi_top_logits_workspace(1, 1, C, 1, 2, ctypes.byref(need)) == -1
+        assert hip_lib.msfwsi_top_logits(1, at, C, 1, C, 1, 2, 1.0, at, at, at, at, None) == -1
+        assert hip_lib.msfwsi_distill_fwd(1, at, C, 1, C, 1, 2, at, at, None, None, 1.0, 1, at, None, at, at, at, None) == -1
+        assert hip_lib.msfwsi_distill_bwd(1, at, C, 1, C, 1, 2, at, at, None, 1.0, at, None, at, 0, at, None) == -1
