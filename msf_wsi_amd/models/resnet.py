@@ -140,8 +140,9 @@ class ResNet(nn.Module):
 
         feats = engine.encoder_apply(self, x)
         last = feats[3]
-        if not isinstance(self.fc, nn.Identity):  # classifier head is outside the hot path: plain torch
-            last = self.fc(last.to(next(self.fc.parameters()).dtype))
+        if not isinstance(self.fc, nn.Identity):  # classifier head is outside the hot path: plain torch, or a frozen quant.MX4Linear
+            weight = next(self.fc.parameters(), None)  # a 4-bit head holds buffers alone and takes features of any type
+            last = self.fc(last if weight is None else last.to(weight.dtype))
         if self.return_features:
             return (feats[0], feats[1], feats[2], last)
         return last

@@ -1,16 +1,19 @@
 """4-bit storage for the weights of frozen layers, and products with it.
 
-A trained encoder or head that no longer changes -- a teacher, a feature extractor -- keeps its Linear weights (the fuser
-layers of src/models/backbone.py:12-31 reach 18432 x 18432) in 4.25 bits an element instead of 16 or 32.  A layer with few
+A trained classifier that no longer changes -- a teacher -- keeps the weight of its Linear head (`ResNet.fc`, or heads of
+the user's own behind the encoder's features) in 4.25 bits an element instead of 16 or 32.  A layer with few
 rows is bound by reading its weight, one with many by the matrix rate, and 4-bit operands help both:
 
     w = quantize_mx4(linear.weight)                    # once per checkpoint
     y = mx4_linear(x, w, linear.bias.detach())         # x is quantised the same way on its way in; fp32 sums
-    layer = MX4Linear.from_linear(linear)              # the same as a module
+    model.fc = MX4Linear.from_linear(model.fc)         # the same as a module, in a models.resnet.ResNet
 
 Format: 32 consecutive elements of a row share a power-of-two scale 2^(E - 127) and are rounded to
 {0, .5, 1, 1.5, 2, 3, 4, 6} with a sign (to nearest, ties to the even code, saturating).  E is the exponent of the block's largest
 magnitude less two; a block that holds an infinity or a NaN becomes NaN as a whole.
+
+The projector, predictor and fuser MLPs of the pre-train model (src/models/backbone.py:12-31) are trained by the engine, which
+takes nn.Linear alone there and refuses other layers with an error.
 
 The gradient runs through to x (`dx = dy W`, the rounding of x passed straight through); the weight is frozen and has none.
 All arithmetic is in csrc/mx4.hip; there is no CPU path."""

@@ -576,3 +576,45 @@ def test_products_of_all_scales(hip_lib, rows):
         want = (a * keep) @ b.t()
         top = torch.finfo(torch.float32).max
         assert torch.equal(y.cpu().double().clamp(-2 * top, 2 * top), torch.where(want.abs() > top, torch.sign(want) * 2 * top, want.float().double()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("arch,classes", [("resnet18", 1000), ("resnet50", 21)])
+def test_resnet_with_a_4_bit_head(hip_lib, arch, classes):
+    """the framework's own classifier as a frozen teacher: its head in 4 bits, its top logits, a student ResNet trained on them;
+    and a 4-bit head on the student, which passes the gradient on to the encoder as the widened weight would"""
+    from msf_wsi_amd import losses, quant
+    from msf_wsi_amd.models import resnet
+
+    torch.manual_seed(5)
+    teacher, student = (getattr(resnet, arch)(num_classes=classes).cuda().train() for _ in range(2))
+    x = torch.randn(4, 3, 64, 64, generator=torch.Generator().manual_seed(6)).cuda()
+    fc, seen = teacher.fc, []
+    teacher.fc = quant.MX4Linear.from_linear(fc)
+    teacher.fc.register_forward_pre_hook(lambda module, args: seen.append(args[0]))
+    with torch.no_grad():
+        logits = teacher(x)
+    feats, = seen
+    w, b = teacher.fc, fc.bias.detach().double().cpu()
+    wv = quant.MX4Tensor(w.codes, w.scales, w.in_features).dequantize().double().cpu()
+    xq = to.mx4_round(feats.float().cpu())[0]
+    want, mass = xq @ wv.t() + b, xq.abs() @ wv.abs().t() + b.abs()
+    assert logits.shape == (4, classes) and bool(((logits.double().cpu() - want).abs() <= bound(w.in_features, mass, want, logits.dtype)).all())
+    top = losses.top_logits(logits, 5, temperature=2.0)
+    crit = losses.TopLogitDistillLoss(2.0)
+    crit(student(x), top).backward()
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in student.parameters())
+    # the gradient of the features through a 4-bit head
+    head = quant.MX4Linear.from_linear(student.fc)
+    f = feats.detach().requires_grad_()
+    y = head(f)
+    dy, = torch.autograd.grad(crit(y, top), y, retain_graph=True)
+    df, = torch.autograd.grad(y, f, dy)
+    hv = quant.MX4Tensor(head.codes, head.scales, head.in_features).dequantize().double().cpu()
+    want, mass = dy.double().cpu() @ hv, dy.double().cpu().abs() @ hv.abs()
+    assert bool(((df.double().cpu() - want).abs() <= bound(3 * classes, mass, want, f.dtype)).all())
+    student.zero_grad(set_to_none=True)
+    student.fc = head
+    crit(student(x), top).backward()
+    assert not [n for n, _ in student.named_parameters() if n.startswith("fc.")]
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) and float(p.grad.abs().max()) > 0 for p in student.parameters())
