@@ -82,7 +82,7 @@ __global__ __launch_bounds__(512, 4) void stem_ws_kernel(const StemParams prm) {
                                          (__attribute__((address_space(3))) void*)(Ws + g * 1024), 16, 0, 0);
     }
 
-    // padded-raster position -> (image, row, column); advanced by BM positions per tile with carries
+    // padded-raster position -> (image, row, column); advanced with carries
     auto locate = [&](long q, int& img, int& y, int& xx) {
         if (q < 0) {  // before the batch (q >= -(2 Wp + 2) > -Hp Wp): the pad rows of "image -1"
             img = -1;
@@ -96,10 +96,9 @@ __global__ __launch_bounds__(512, 4) void stem_ws_kernel(const StemParams prm) {
         y = (int)fast_div(rem, prm.div_wp);
         xx = (int)(rem - (unsigned)y * (unsigned)Wp);
     };
-    const int adv_y = BM / Wp, adv_x = BM - adv_y * Wp;
-    auto advance = [&](int& img, int& y, int& xx) {
-        xx += adv_x;
-        y += adv_y;
+    auto advance = [&](int by_y, int by_x, int& img, int& y, int& xx) {
+        xx += by_x;
+        y += by_y;
         if (xx >= Wp) {
             xx -= Wp;
             ++y;
@@ -111,17 +110,17 @@ __global__ __launch_bounds__(512, 4) void stem_ws_kernel(const StemParams prm) {
     };
 
     // halo staging: chunk i*512 + tid -> (halo position, 16-byte half); halo position hr <-> q0 - 2 Wp - 2 + hr
-    int a_lds[AL], a_img[AL], a_y[AL], a_x[AL];
+    int a_img[AL], a_y[AL], a_x[AL];
     bool a_in[AL];
-    const int half = tid & 1;
+    const int half = tid & 1, a_lds = halo_off(tid >> 1, half);  // of chunk 0; NT / 2 positions on it differs by a constant
+    static_assert(NT / 2 % 16 == 0, "the swizzle repeats");
 #pragma unroll
     for (int i = 0; i < AL; ++i) {
         const int hr = (i * NT + tid) >> 1;
         a_in[i] = hr < BM + 3 * Wp + 3;
-        a_lds[i] = halo_off(hr < Cfg::HALO ? hr : 0, half);
-        if (hr >= Cfg::HALO) a_lds[i] = -1;
         locate((long)t_beg * BM - 2 * Wp - 2 + hr, a_img[i], a_y[i], a_x[i]);
     }
+    const int adv_y = BM / Wp, adv_x = BM - adv_y * Wp;  // a tile
     uint4 a_reg[AL];
     auto load_A = [&]() {  // loads the tile the slot positions point at, then advances them to the next tile
 #pragma unroll
@@ -129,16 +128,17 @@ __global__ __launch_bounds__(512, 4) void stem_ws_kernel(const StemParams prm) {
             a_reg[i] = make_uint4(0, 0, 0, 0);
             if (a_in[i] && (unsigned)a_img[i] < (unsigned)prm.N && a_y[i] < H && a_x[i] < W)
                 a_reg[i] = *reinterpret_cast<const uint4*>(x + (((long)a_img[i] * H + a_y[i]) * W + a_x[i]) * 16 + half * VEC);
-            advance(a_img[i], a_y[i], a_x[i]);
+            advance(adv_y, adv_x, a_img[i], a_y[i], a_x[i]);
         }
     };
 
-    // row pass: chunk cc of rows rr + ps*64; the output position of each of this thread's rows, advanced per tile
+    // row pass: chunk cc of rows rr + ps*64; one output position, which steps through this thread's rows (a position for each of the
+    // four took nine registers more, and scratch)
     constexpr int CPR = BN / VEC, RPP = NT / CPR, NP = BM / RPP;  // 8 chunks per row, 64 rows per pass, 4 passes
     const int cc = tid % CPR, rr = tid / CPR;
-    int o_img[NP], o_y[NP], o_x[NP];
-#pragma unroll
-    for (int ps = 0; ps < NP; ++ps) locate((long)t_beg * BM + rr + ps * RPP, o_img[ps], o_y[ps], o_x[ps]);
+    const int row_y = RPP / Wp, row_x = RPP - row_y * Wp;
+    int o_img, o_y, o_x;
+    locate((long)t_beg * BM + rr, o_img, o_y, o_x);
     float ssum[VEC], ssq[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) ssum[e] = ssq[e] = 0.f;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(512, 4) void stem_ws_kernel(const StemParams prm) {
         __syncthreads();  // the previous tile's row pass is done with the bytes the halo shares
 #pragma unroll
         for (int i = 0; i < AL; ++i)
-            if (a_lds[i] >= 0) *reinterpret_cast<uint4*>(As + a_lds[i]) = a_reg[i];
+            if ((i * NT + tid) >> 1 < Cfg::HALO) *reinterpret_cast<uint4*>(As + a_lds + i * (NT / 2 * 32)) = a_reg[i];
         __syncthreads();
         if (tile + 1 < t_end) load_A();  // in flight while the MFMAs run
 
@@ -193,10 +193,10 @@ __global__ __launch_bounds__(512, 4) void stem_ws_kernel(const StemParams prm) {
         __syncthreads();
 #pragma unroll
         for (int ps = 0; ps < NP; ++ps) {
-            if ((unsigned)o_img[ps] < (unsigned)prm.N && o_y[ps] < H && o_x[ps] < W) {  // pad positions produce nothing
+            if ((unsigned)o_img < (unsigned)prm.N && o_y < H && o_x < W) {  // pad positions produce nothing
                 const int row = rr + ps * RPP;
                 const uint4 v = *reinterpret_cast<const uint4*>(Cs + row * LDC + cc * VEC);
-                *reinterpret_cast<uint4*>(out + (((long)o_img[ps] * H + o_y[ps]) * W + o_x[ps]) * 64 + cc * VEC) = v;
+                *reinterpret_cast<uint4*>(out + (((long)o_img * H + o_y) * W + o_x) * 64 + cc * VEC) = v;
                 if (prm.stats != nullptr) {
                     float f[VEC];
                     unpack16<T>(v, f);
@@ -207,7 +207,7 @@ __global__ __launch_bounds__(512, 4) void stem_ws_kernel(const StemParams prm) {
                     }
                 }
             }
-            advance(o_img[ps], o_y[ps], o_x[ps]);
+            advance(row_y, row_x, o_img, o_y, o_x);
         }
     }
 
