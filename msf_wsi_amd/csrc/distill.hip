@@ -175,8 +175,10 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int c, int n, con
 // DEEP: a list of more than 16 from a row that one wave takes.  The k-th of only 64 maxima would leave most of the row for candidates,
 // so the maxima are those of single chunks (65536 rows of 1000 bf16, k = 64: 186 us; 726 with one maximum a thread).
 // ---------------------------------------------------------------------------------------------------------------------
+// Seven waves a SIMD of a segment's 256 threads leave 72 registers each; fp16 needs a few more and spilled: six (4096 x 65536 at
+// k = 32: 156 -> 147 us).
 template <typename T, int NT, int NCH, bool DEEP>
-__global__ void __launch_bounds__(NT, NT == 256 ? 7 : DEEP ? 4 : 5) top_segment_kernel(const T* __restrict__ x, long ld, int C, int nseg, int k, float inv_t,
+__global__ void __launch_bounds__(NT, NT == 256 ? (__is_same(T, _Float16) ? 6 : 7) : DEEP ? 4 : 5) top_segment_kernel(const T* __restrict__ x, long ld, int C, int nseg, int k, float inv_t,
                                                          float* __restrict__ values, int* __restrict__ indices, float* __restrict__ rest,
                                                          long* __restrict__ part_keys, Sum* __restrict__ part_sums) {
     constexpr int VEC = ElemTraits<T>::VEC;
