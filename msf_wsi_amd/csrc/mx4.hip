@@ -762,8 +762,8 @@ struct GemmPlan {
 constexpr long kCus = 256;
 constexpr int NWR = 8;  // waves that share 16 columns of few rows
 // Few rows are multiplied straight from memory up to 32 (16) MB of b: below, tiles cannot fill the machine (4096 x 4096 at 16
-// rows 5.1 us, as tiles 9.9); above, DMA reads faster than the waves' own loads (18432 x 18432 at 2 / 16 / 32 rows 33 / 46 / 68 us, as
-// tiles 31 / 32 / 34).
+// rows 8.9 us, as tiles 14.3; 9216 x 4608 14.7, 17.3); above, DMA reads faster than the waves' own loads (9216 x 9216 at 16 rows 21.5,
+// as tiles 19.7; 18432 x 18432 at 2 / 16 / 32 rows 41 / 54 / 74, as tiles 38 / 40 / 42).  From x to y, over weights that are in no cache.
 // Tiles of 256 x 256 take a tenth less time than 128 x 128 (4096 x 4096 x 8192: 74 / 81 us, 4096 x 8192 x 8192: 146 / 162) where their
 // rounds of 256 are at most 15 % more than their number (8192 x 9216 x 9216, 4.5 rounds: 378 / 401 us), and are slower where the last
 // round leaves more idle (4608 x 4096 x 4096, 1.13 rounds: 70 / 58 us; 6144, 1.5 rounds: 73 / 68; 8192 x 5120, 2.5: 112 / 110).
@@ -879,10 +879,11 @@ extern "C" int msfwsi_mx4_gemm(int dtype, const void* a_codes, const void* a_sca
 }
 
 // A single row is quantised by the waves that multiply it, in one launch and without a workspace, unless the weight is so large that
-// its time exceeds that of a launch more (18432 x 18432: 40 us, in two launches 34; 512 x 18432: 8 us, 11 + 3 in two)
+// its slower reads cost what the other launches do (from x to y, over weights that are in no cache: 512 x 18432 8.8 us, in more launches
+// 10.9; 9216 x 18432 21.6, 25.3; 18432 x 18432 38.1, 37.9)
 static bool row_alone(long M, long N, long cols) {
     const long G = groups_of(cols);
-    return M == 1 && G <= kRowGroups && N * G * (kGroupBytes + 8) <= 1L << 26;
+    return M == 1 && G <= kRowGroups && N * G * (kGroupBytes + 8) <= 1L << 27;
 }
 // workspace of a linear call: x's codes, its scales, the partial sums
 extern "C" int msfwsi_mx4_linear_workspace(long M, long N, long cols, long* bytes) {

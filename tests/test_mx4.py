@@ -618,3 +618,17 @@ def test_resnet_with_a_4_bit_head(hip_lib, arch, classes):
     crit(student(x), top).backward()
     assert not [n for n, _ in student.named_parameters() if n.startswith("fc.")]
     assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) and float(p.grad.abs().max()) > 0 for p in student.parameters())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,N", [(18432, 9216), (18000, 15000), (33000, 9000)])
+def test_one_row_of_large_weights(hip_lib, K, N):
+    """either side of the size up to which a single row takes one launch, against the widened weight in float64"""
+    from msf_wsi_amd import quant
+
+    w4 = quant.quantize_mx4(features(256, K, torch.float32, K).repeat((N + 255) // 256, 1)[:N].cuda() / 100)
+    x = features(1, K, torch.bfloat16, N).cuda()
+    y = quant.mx4_linear(x, w4, out_dtype=torch.float32)
+    w, xq = w4.dequantize().double(), quant.quantize_mx4(x).dequantize().double()
+    want, mass = xq @ w.t(), xq.abs() @ w.abs().t()
+    assert bool(((y.double() - want).abs() <= bound(K, mass, want, torch.float32)).all())
