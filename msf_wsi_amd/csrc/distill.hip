@@ -73,7 +73,7 @@ __device__ __forceinline__ Sum one(float x) { return {x, x == -INFINITY ? 0.f : 
 // The same taken by one lane over any number of logits, 32 at a time: the sums of 32 are added with what the additions before lost
 // put back (compensated), and the reference moves only where a logit exceeds it by more than kRaise powers of two, so the error
 // is that of 32 additions whatever the number (70001 equal logits behind one a little larger, added one by one: the logarithm 6.5e-4 off).
-constexpr float kRaise = 8.f;
+constexpr float kRaise = 1.f;
 constexpr int kAtOnce = 32;
 struct LongSum {
     float ref = -INFINITY, total = 0.f, lost = 0.f;
@@ -479,11 +479,11 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
     }
     LongSum sum;
     float part = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < C; ++j) {
-        float out;
+    bool infinite = false;
+    // class j's logit goes in, what it throws out of the list comes back
+    auto insert = [&](T x_, int j) {
         if constexpr (SMALL) {
-            int a = order16<T>(p[j * inner]) << 16 | (0xffff - j);
+            int a = order16<T>(x_) << 16 | (0xffff - j);
 #pragma unroll
             for (int s = 0; s < KM; ++s)
                 if (s < k) {
@@ -491,9 +491,9 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
                     v[s] = max(v[s], a);
                     a = low;
                 }
-            out = a == kNothing ? -INFINITY : value16<T>(a >> 16);
+            return a == kNothing ? -INFINITY : value16<T>(a >> 16);
         } else {
-            int a = order_of(load_elem<T>(p, j * inner)), ai = j;
+            int a = order_of((float)x_), ai = j;
             bool in = false;
 #pragma unroll
             for (int s = 0; s < KM; ++s)
@@ -505,14 +505,44 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
                     a = in ? ov : a;
                     ai = in ? oi : ai;
                 }
-            out = value_of(a);
+            return value_of(a);
         }
-        if (sum.raises(out, c)) part *= sum.raise(out, c);
-        part += out == -INFINITY ? 0.f : term<true>(out, sum.ref, c);
-        if ((j & (kAtOnce - 1)) == kAtOnce - 1) {
+    };
+    auto sum_up = [&](float (&out)[4]) {
+        float high = fmaxf(fmaxf(out[0], out[1]), fmaxf(out[2], out[3]));
+        if (sum.raises(high, c)) {
+            if (high == INFINITY) {  // kept apart: the sum has no term for it
+                infinite = true;
+                high = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (out[u] == INFINITY) out[u] = -INFINITY;
+                    high = fmaxf(high, out[u]);
+                }
+            }
+            if (sum.raises(high, c)) part *= sum.raise(high, c);
+        }
+        const float ref = finite_ref(sum.ref);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) part += exp2_((out[u] - ref) * c);
+    };
+    int j = 0;
+    for (; j + 4 <= C; j += 4) {
+        T raw[4];
+        float out[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) raw[u] = p[(j + u) * inner];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) out[u] = insert(raw[u], j + u);
+        sum_up(out);
+        if ((j & (kAtOnce - 1)) == kAtOnce - 4) {
             sum.add(part);
             part = 0.f;
         }
+    }
+    for (; j < C; ++j) {
+        float out[4] = {insert(p[j * inner], j), -INFINITY, -INFINITY, -INFINITY};
+        sum_up(out);
     }
     sum.add(part);
 #pragma unroll
@@ -522,7 +552,7 @@ __global__ void __launch_bounds__(kT) top_thread_kernel(const T* __restrict__ x,
             else values[(o * k + s) * inner + i] = value_of(v[s]);
             indices[(o * k + s) * inner + i] = SMALL ? 0xffff - (v[s] & 0xffff) : at[s];
         }
-    rest[row] = log_of({sum.ref, sum.total}, inv_t);
+    rest[row] = infinite && sum.total == sum.total ? INFINITY : log_of({sum.ref, sum.total}, inv_t);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
