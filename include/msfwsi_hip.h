@@ -526,8 +526,8 @@ int msfwsi_inverse_perm(const long* perm, long* inv, long rows, int K, void* str
  * `cols` elements takes G = ceil(cols / 256) groups (zeros behind the last column):
  *   codes  [G][rows][128] bytes, element 2i of a group in the low, 2i + 1 in the high four bits of byte i
  *   scales [G][rows][8]   bytes E; 255 = the block is NaN
- * both 16-byte aligned.  These serve frozen layers beside the fp32 / 16-bit 1x1 convolutions (nn.Linear of
- * src/models/backbone.py:12-31); the reference has no 4-bit storage: no parity to pin, the checks are against the formulas.
+ * both 16-byte aligned.  These serve frozen nn.Linear heads (ResNet.fc, src/models/resnet.py) beside the fp32 / 16-bit 1x1
+ * convolutions; the reference has no 4-bit storage: no parity to pin, the checks are against the formulas.
  *   msfwsi_mx4_quantize:   x [rows][cols], rows `ld` elements apart, any alignment.  E = max(exponent field of the block's
  *                          largest magnitude - 2, 0), 255 when it is not finite; to nearest, ties to the even code, saturating
  *   msfwsi_mx4_dequantize: y [rows][cols] in `dtype`

@@ -169,7 +169,7 @@ __device__ __forceinline__ void store_chunk(T* __restrict__ p, int c, int n, con
 // chunk at nearly every step: looking at them in place cost all lanes the walk twice over, 166 us instead of 149); what is
 // not below the bound goes into a list and is ranked by counting.  Everything else is summed for `rest`, each thread its own and the
 // list's surplus once it is in order: the lists fill in any order, no sum depends on it.
-// 4096 rows of 65536 bf16, k = 32: 134 us, 4.0 TB/s; 4 such rows of fp32 9 us.
+// 4096 rows of 65536 bf16, k = 32: 132 us, 4.1 TB/s, the vector units busy throughout; 4 such rows of fp32 8 us.
 // A queue or list that runs over (long ties, a masked-out segment) sends the segment through k rounds of a plain maximum instead.
 // Rows longer than a segment leave their segments' lists and sums to a merge.
 // DEEP: a list of more than 16 from a row that one wave takes.  The k-th of only 64 maxima would leave most of the row for candidates,
@@ -789,8 +789,8 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
 }
 
 // One thread per row: maps, and rows of a few classes.  A class costs about 7 instructions: the listed ones are taken out of the
-// sum by a bit each, their own logits are asked for early and handled apart.  32 maps of 21 x 256 x 256 fp32, k = 4: forward 99 us
-// (2.9 TB/s; bound by instructions and latency at 4 waves per SIMD), backward 106 us (4.4 TB/s).  KM > 0: lists of up to KM entries whose indices stay in registers;
+// sum by a bit each, their own logits are asked for early and handled apart.  32 maps of 21 x 256 x 256 fp32, k = 4: forward 100 us
+// (2.9 TB/s; bound by latency and instructions: at 4 waves per SIMD the vector units are busy half the time), backward 106 us (4.4 TB/s).  KM > 0: lists of up to KM entries whose indices stay in registers;
 // KM = 0: any length, read again where needed.
 template <int KM>
 struct List {
@@ -1014,10 +1014,11 @@ __global__ void __launch_bounds__(kT) distill_thread_bwd_kernel(const T* __restr
     }
 }
 
-// Rows that one thread takes: maps, whose classes are not adjacent, and short rows where there are very many.  A wave per row costs
-// about 1 ns a row, a thread per row 0.2 us a class however few the rows are (selection: 0.2 us up to k = 4, 0.4 - 0.9 up to 16).
-// bf16, k = 4, selection / loss by a wave and by a thread: 65536 rows of 64 classes 78 / 61 and 18 / 23 us, 65536 of 128 78 / 66 and
-// 29 / 37, 16384 of 64 23 / 21 and 17 / 22, 1024 of 64 7 / 8 and 16 / 21.
+// Rows that one thread takes: maps, whose classes are not adjacent (every map, also one of so few positions that most of the machine
+// idles), and short rows where there are very many.  A wave per row costs about 1 ns a row, a thread per row 0.2 us a class however
+// few the rows are (selection: 0.2 us up to k = 4, 0.3 (fp32 0.9) up to 16).
+// bf16, k = 4, selection / loss by a wave and by a thread: 65536 rows of 64 classes 75 / 61 and 12 / 17 us, 65536 of 128 75 / 65 and
+// 21 / 26, 16384 of 64 23 / 20 and 12 / 16, 1024 of 64 7 / 7 and 12 / 16.
 bool by_thread(long rows, int classes, long inner, int k, bool select) {
     return inner > 1 || (classes <= 128 && k <= 16 && rows >= classes * (select && k > 4 ? 1024L : 256L));
 }

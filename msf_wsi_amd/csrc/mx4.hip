@@ -342,7 +342,7 @@ struct GemmArgs {
 // stages in LDS filled by DMA.  A row's eight 16-byte chunks lie at (chunk ^ (row / 2 & 7)): the sixteen rows that a read takes
 // at a time then fall on all 64 banks.  The columns of a wave's 64 are dealt to its two fragments in turn (2 l + j: b's rows lie in
 // LDS in that order), so that a lane ends up with neighbours of a row and a wave writes whole 128-byte lines.
-// 8192 x 9216 x 9216: 382 us, 3.6 PFLOP/s (4.5 rounds of tiles); 8192 x 8192 x 8192: 268 us, 4.1 PFLOP/s (registers alone reach 6.5
+// 8192 x 9216 x 9216: 376 us, 3.7 PFLOP/s (4.5 rounds of tiles); 8192 x 8192 x 8192: 290 us, 3.8 PFLOP/s (registers alone reach 6.5
 // at this card's power).  Requests and
 // products share the CU's LDS and issue slots; a four-stage ring of half groups (64-byte lines: 0.8 of the rate), fragments
 // read a step ahead by hand, a workgroup that runs through its tiles, and four waves of 128 x 128 were all 2 - 20 % slower.
@@ -499,8 +499,8 @@ __global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy,
 // weights are taken relative to the largest scale of their 32 columns over all rows of W (dy is at most 65504: no sum can overflow), which
 // holds scales that are at most 2^26 apart exactly; where a workgroup finds them further apart it cuts each dy value into two bf16
 // parts (8 + 3 bits) instead.
-// Bound by the 16-bit matrix rate and the widening beside it: 8192 x 8192 x 8192 bf16 991 us, 1.1 PFLOP/s (the library's product of 16-bit
-// matrices 1.38); 8192 x 9216 x 9216 fp16 1516 us.
+// Bound by the 16-bit matrix rate and the widening beside it: 8192 x 8192 x 8192 bf16 967 us, 1.1 PFLOP/s (the library's product of 16-bit
+// matrices 1.38); 8192 x 9216 x 9216 fp16 1370 - 1510 us as the card's power allows (matrix units busy 42 % of the cycles, vector units 22 %).
 template <typename T, bool CUT>
 __device__ __forceinline__ void dgrad_mma(f32x16& acc, const uint4& a, const uint4& b) {
     if constexpr (!CUT) {
