@@ -529,7 +529,8 @@ int msfwsi_inverse_perm(const long* perm, long* inv, long rows, int K, void* str
  * both 16-byte aligned.  These serve frozen nn.Linear heads (ResNet.fc, src/models/resnet.py) beside the fp32 / 16-bit 1x1
  * convolutions; the reference has no 4-bit storage: no parity to pin, the checks are against the formulas.
  *   msfwsi_mx4_quantize:   x [rows][cols], rows `ld` elements apart, any alignment.  E = max(exponent field of the block's
- *                          largest magnitude - 2, 0), 255 when it is not finite; to nearest, ties to the even code, saturating
+ *                          largest magnitude - 2, 0), 255 when it is not finite; to nearest, ties to the even code, saturating.
+ *                          Fewer than 2^27 rows, at most 262140 groups (mx4_dequantize too)
  *   msfwsi_mx4_dequantize: y [rows][cols] in `dtype`
  *   msfwsi_mx4_gemm:       y[m][n] = sum_k a[m][k] b[n][k] (+ bias[n], fp32), both operands quantised, fp32 sums, y [M][N]
  *   msfwsi_mx4_linear:     mx4_quantize of x [M][cols] and mx4_gemm of the result with w [N][cols], in one call

@@ -734,3 +734,33 @@ def test_too_many_classes_are_refused(hip_lib):
         assert hip_lib.msfwsi_top_logits(1, at, C, 1, C, 1, 2, 1.0, at, at, at, at, None) == -1
         assert hip_lib.msfwsi_distill_fwd(1, at, C, 1, C, 1, 2, at, at, None, None, 1.0, 1, at, None, at, at, at, None) == -1
         assert hip_lib.msfwsi_distill_bwd(1, at, C, 1, C, 1, 2, at, at, None, 1.0, at, None, at, 0, at, None) == -1
+
+
+@pytest.mark.gpu
+def test_hooknet_maps(hip_lib):
+    """the framework's segmentation model as teacher and student: its maps go into selection and loss as they are, the gradient back
+    into its weights"""
+    from test_hooknet_gpu import CLASSES, _build, _inputs
+
+    from msf_wsi_amd import losses
+
+    teacher, student = _build().cuda().eval(), _build().cuda().train()
+    x1, x2, _, m2 = (t.cuda() for t in _inputs())
+    k, T, mask = 3, 2.0, (m2 != 0)
+    with torch.no_grad():
+        tl = teacher(x1, x2)[1]
+        top = losses.top_logits(tl, k, T, dim=1)
+    z = student(x1, x2)[1]
+    z.retain_grad()
+    row = losses.TopLogitDistillLoss(T, "none", dim=1)(z, top, mask)
+    assert row.shape == mask.shape and z.shape[1] == CLASSES + 1
+    row.sum().backward()
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for n, p in student.named_parameters() if n.startswith("target_branch"))
+    pick = torch.randint(0, mask.numel(), (300,), generator=torch.Generator().manual_seed(1)).cuda()
+
+    def rows_of(a):
+        return a.detach().movedim(1, -1).reshape(mask.numel(), -1)[pick].cpu()
+
+    some = losses.TopLogits(rows_of(top.values), rows_of(top.indices), top.rest.reshape(-1)[pick].cpu())
+    same_top(rows_of(tl), k, T, some)
+    check(rows_of(z).to(z.dtype), some.values, some.indices, some.rest, mask.reshape(-1)[pick].cpu(), T, row.detach().reshape(-1)[pick], rows_of(z.grad), z.dtype)
