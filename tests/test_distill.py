@@ -632,7 +632,7 @@ def test_long_sums_of_one_lane(hip_lib, dt, kind, C, k):
     E = (3 * float((x.double().amax(1) - x.double().amin(1)).max()) + 34 + 64) * U
     maps = x.view(2, 2, C).movedim(-1, 1).contiguous().cuda()
     got = losses.top_logits(maps, k, dim=1)
-    v, i = torch.sort(x.double(), 1, descending=True, stable=True)   # the definition, without a loop over 131072 classes
+    v, i = torch.sort(x.double(), dim=1, descending=True, stable=True)   # the definition, without a loop over 131072 classes
     i, r = i[:, :k], torch.logsumexp(v[:, k:], 1)
     assert torch.equal(got.indices.movedim(1, -1).reshape(4, k).cpu().long(), i)
     assert bool(((got.rest.reshape(4).cpu().double() - r).abs() <= E + 2 * U * r.abs()).all())
