@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(NT, NT == 256 ? (__is_same(T, _Float16) ? 6 : 
             const float x2 = exp2_(fmaf(f[e], c, shift));
             part += f[e] >= lim ? 0.f : x2;
         }
-        const bool queue_it = !(high < lim);
+        // a row of fewer than k chunks has no bound: its own chunks go in, those past its end do not
+        const bool queue_it = !(high < lim) && (NT == 256 || (j * NT + t) * VEC < n);
         s += part;
         if (queue_it) {
             const int slot = atomicAdd(&queued, 1);
@@ -441,7 +442,8 @@ __global__ void __launch_bounds__(64) top_merge_long_kernel(const long* __restri
 // ---------------------------------------------------------------------------------------------------------------------
 // Selection, one thread per row: maps (neighbouring threads, neighbouring positions) and rows of a few classes.  The list is
 // kept sorted in registers; every class throws one value out of it (itself, a displaced one or an empty slot), which goes to
-// the running sum for `rest`, so the logits are read once.
+// the running sum for `rest`, so the logits are read once.  KM places: 4, 16 or 64 (16 maps of 21 x 256 x 256 bf16: k = 4 in 4 / 16 / 64
+// places 30 / 58 / 268 us, k = 16 in 16 / 64 63 / 272).
 // ---------------------------------------------------------------------------------------------------------------------
 // 16-bit logits: order and index fit one int (up to 65536 classes), and a step of the insertion is a max and a min.
 template <typename T>
@@ -791,7 +793,8 @@ __global__ void __launch_bounds__(NT) distill_bwd_kernel(const T* __restrict__ z
 // One thread per row: maps, and rows of a few classes.  A class costs about 7 instructions: the listed ones are taken out of the
 // sum by a bit each, their own logits are asked for early and handled apart.  32 maps of 21 x 256 x 256 fp32, k = 4: forward 100 us
 // (2.9 TB/s; bound by latency and instructions: at 4 waves per SIMD the vector units are busy half the time), backward 106 us (4.4 TB/s).  KM > 0: lists of up to KM entries whose indices stay in registers;
-// KM = 0: any length, read again where needed.
+// KM = 0: any length, read again where needed (the same maps, forward / with the gradient: k = 4 as KM 4 92 / 211 us, as 16 129 / 294, as
+// 0 145 / 428; k = 16 as KM 16 305 / 626, as 0 693 / 2163).
 template <int KM>
 struct List {
     int idx[KM > 0 ? KM : 1];

@@ -491,7 +491,8 @@ __global__ void __launch_bounds__(kT) mx4_parts_kernel(const T* __restrict__ dy,
     }
 }
 
-// dx = dy W for a frozen W: 256 rows x 256 columns (one group of W's) per workgroup of 8 waves, 64 rows of W a step.  dy comes
+// dx = dy W for a frozen W: 256 rows x 256 columns (one group of W's) per workgroup of 8 waves, 64 rows of W a step; the only
+// tile there is: fewer rows cost what 256 do.  dy comes
 // by DMA like the tiles above; W's codes (8 KB a step) are widened to 16 bits on the way into LDS [n][column] and read transposed
 // (ds_read_b64_tr_b16), even and odd columns apart as above.  The scale of a weight varies along the sum, so it is applied while
 // widening.  bf16 holds every weight as it is (subnormals too, which conversion and products keep), so that sums overflow where the
